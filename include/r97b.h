@@ -595,6 +595,102 @@ int r97b_gemm_i8g_gated(const int8_t* a, int64_t lda, const float* a_scale, int6
                         int32_t act_sigmoid, int8_t* q, int64_t ldq, float* q_scale, int64_t ld_qs,
                         uint16_t* out_bf16, int64_t ld_ob, void* stream);
 
+/* ------------------------------------------------------------------------------ packed sequences */
+/* Ragged sequences laid end to end (token-major rows, no padding): what the GatedDeltaNet entry points take
+ * through cu_seqlens, for the rotary positions and the attention core. */
+
+/* A packed batch: sequence s holds tokens [cu[s], cu[s + 1]) of T = cu[n_seq]; cu[0] = 0, empty sequences
+ * allowed. q_blocks and k_blocks are device tables of n_blocks int32[4] rows {first token of the sequence,
+ * its length, block index in the sequence, 0}, one per 128-token block, filled by r97b_packed_blocks on the
+ * host: q_blocks with the most keys to visit first, k_blocks with the most queries first. */
+typedef struct R97bPacked {
+    int32_t n_seq, n_blocks;
+    int64_t T;
+    const int32_t* q_blocks;
+    const int32_t* k_blocks;
+} R97bPacked;
+
+/* Fills both block tables (host arrays of int32[4] rows, either may be null) and returns the block count, or
+ * -1 on a bad cu (null, n_seq < 0, cu[0] != 0, decreasing). */
+int32_t r97b_packed_blocks(const int32_t* cu_host, int32_t n_seq, int32_t* q_blocks_host, int32_t* k_blocks_host);
+
+/* Token-major head rows: row (token t, head h) is at ptr + t * tok + h * head (strides in elements). 16-byte
+ * aligned, strides multiples of 8, head >= D, tok >= (heads - 1) * head + D. */
+typedef struct R97bHeadRows {
+    void* ptr;
+    int64_t tok, head;
+} R97bHeadRows;
+
+/* Causal grouped-query attention inside each sequence: o_t = sum_{j <= t} softmax_j(scale q_t . k_j) v_j over the
+ * sequence's own tokens; query head h reads key/value head h / (Hq / Hkv). bf16, D 128 or 256; lse f32
+ * [Hq, ld_lse >= T], the natural-log log-sum-exp of each row's scaled scores. Rows behind token T are neither
+ * read nor written, and a row outside a sequence never reaches that sequence's results whatever it holds.
+ * Replaces: attention_twin, src/adjoint/host/attention.cpp:261-313, over the ragged batch of
+ * include/r97/batch.h. */
+typedef struct R97bAttnPackedFwd {
+    int32_t Hq, Hkv, D;
+    float scale;
+    R97bHeadRows q, k, v, o;
+    float* lse;
+    int64_t ld_lse;
+} R97bAttnPackedFwd;
+
+int r97b_attn_packed_fwd(const R97bPacked* p, const R97bAttnPackedFwd* a, void* stream);
+
+/* Its backward from the forward's o and lse, the probabilities recomputed tile by tile: dq, dk, dv (bf16) of the
+ * cotangent dout. The memory beside the operands is `ws` (256-byte aligned,
+ * r97b_attn_packed_bwd_workspace_bytes bytes, linear in T; calls that share it must not overlap on the GPU).
+ * The same inputs give the same bits.
+ * Replaces: attention_host_adjoint, src/adjoint/host/attention.cpp:315-414. */
+typedef struct R97bAttnPackedBwd {
+    int32_t Hq, Hkv, D;
+    float scale;
+    R97bHeadRows q, k, v, o, dout;
+    const float* lse;
+    int64_t ld_lse;
+    R97bHeadRows dq, dk, dv;
+    void* ws;
+    int64_t ws_bytes;
+} R97bAttnPackedBwd;
+
+int r97b_attn_packed_bwd(const R97bPacked* p, const R97bAttnPackedBwd* a, void* stream);
+int64_t r97b_attn_packed_bwd_workspace_bytes(const R97bPacked* p, int32_t Hq, int32_t Hkv, int32_t D);
+
+/* Rotary tables: cos_tab, sin_tab f32 [n_pos, rot / 2] = amp cos / sin(pos * inv_i), formed in f64.
+ * inv_i = theta^(-2 i / rot), then by `scaling`: R97B_ROPE_NONE; R97B_ROPE_LINEAR: inv_i / factor;
+ * R97B_ROPE_YARN: inv_i (1 - ramp_i) + inv_i / factor ramp_i, ramp rising from 0 to 1 between the pairs that
+ * turn beta_fast and beta_slow times over `original` positions, and amp = 0.1 ln(factor) + 1 (else 1).
+ * rot even, factor >= 1 (YaRN: original > 0, beta_fast > beta_slow > 0). */
+enum { R97B_ROPE_NONE = 0, R97B_ROPE_LINEAR = 1, R97B_ROPE_YARN = 2 };
+int r97b_rope_tables(float* cos_tab, float* sin_tab, int64_t n_pos, int32_t rot, double theta, int32_t scaling,
+                     double factor, double original, double beta_fast, double beta_slow, void* stream);
+
+/* One tensor of head rows of a rotary call: x -> y = rope(rmsnorm(x) w) (w f32 [D]), or rope(x) when w is null.
+ * The backward reads x (unless w is null), y as the cotangent of the output, and writes dx. */
+typedef struct R97bRopePart {
+    int64_t heads;
+    const float* w;
+    R97bHeadRows x, y, dx;
+} R97bRopePart;
+
+/* Up to two tensors (queries and keys) of T token rows in one launch: pos i32 [T] indexes the tables' rows; the
+ * first `rot` dims of a head rotate, in pairs (i, i + rot / 2), or (2 i, 2 i + 1) when interleaved. D 64, 128 or
+ * 256, rot a multiple of 16 up to D. A token whose pos is outside [0, n_pos) gets zero rows and sets bit 1 of
+ * the device error word. Replaces: src/adjoint/host/qk.cpp and rope.cpp over a ragged batch's positions. */
+typedef struct R97bRope {
+    int32_t D, rot, interleaved, n_parts;
+    int64_t T, n_pos;
+    float eps;
+    int32_t _pad;
+    const float* cos_tab;
+    const float* sin_tab;
+    const int32_t* pos;
+    R97bRopePart part[2];
+} R97bRope;
+
+int r97b_qk_rope_fwd(const R97bRope* a, void* stream);
+int r97b_qk_rope_bwd(const R97bRope* a, void* stream);
+
 /* How many kernels this library has launched in this process (a diagnostic for the bench). */
 uint64_t r97b_launch_count(void);
 

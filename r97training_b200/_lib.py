@@ -63,6 +63,36 @@ class R97bQLinearLoraBwd(ctypes.Structure):
                 ("dA", c_vp), ("dB", c_vp), ("ws", c_vp), ("ws_bytes", c_i64)]
 
 
+class R97bPacked(ctypes.Structure):
+    _fields_ = [("n_seq", c_i32), ("n_blocks", c_i32), ("T", c_i64), ("q_blocks", c_vp), ("k_blocks", c_vp)]
+
+
+class R97bHeadRows(ctypes.Structure):
+    _fields_ = [("ptr", c_vp), ("tok", c_i64), ("head", c_i64)]
+
+
+class R97bAttnPackedFwd(ctypes.Structure):
+    _fields_ = [("Hq", c_i32), ("Hkv", c_i32), ("D", c_i32), ("scale", c_f32), ("q", R97bHeadRows),
+                ("k", R97bHeadRows), ("v", R97bHeadRows), ("o", R97bHeadRows), ("lse", c_vp), ("ld_lse", c_i64)]
+
+
+class R97bAttnPackedBwd(ctypes.Structure):
+    _fields_ = [("Hq", c_i32), ("Hkv", c_i32), ("D", c_i32), ("scale", c_f32), ("q", R97bHeadRows),
+                ("k", R97bHeadRows), ("v", R97bHeadRows), ("o", R97bHeadRows), ("dout", R97bHeadRows), ("lse", c_vp),
+                ("ld_lse", c_i64), ("dq", R97bHeadRows), ("dk", R97bHeadRows), ("dv", R97bHeadRows), ("ws", c_vp),
+                ("ws_bytes", c_i64)]
+
+
+class R97bRopePart(ctypes.Structure):
+    _fields_ = [("heads", c_i64), ("w", c_vp), ("x", R97bHeadRows), ("y", R97bHeadRows), ("dx", R97bHeadRows)]
+
+
+class R97bRope(ctypes.Structure):
+    _fields_ = [("D", c_i32), ("rot", c_i32), ("interleaved", c_i32), ("n_parts", c_i32), ("T", c_i64),
+                ("n_pos", c_i64), ("eps", c_f32), ("_pad", c_i32), ("cos_tab", c_vp), ("sin_tab", c_vp), ("pos", c_vp),
+                ("part", R97bRopePart * 2)]
+
+
 class R97IqrDecodeDesc(ctypes.Structure):
     """Field-for-field the C struct of include/r97b_iqr.h (the reference's R97IqrDecodeDesc layout)."""
     _fields_ = [
@@ -165,6 +195,14 @@ _SIGS = {
                                   c_vp]),
     "r97b_embed": (c_i32, [c_vp, c_i64, c_i64, c_vp, c_i64, c_i64, c_vp, c_vp]),
     "r97b_cast_f32_bf16": (c_i32, [c_vp, c_i64, c_vp, c_i64, c_i64, c_i64, c_vp]),
+    "r97b_packed_blocks": (c_i32, [c_vp, c_i32, c_vp, c_vp]),
+    "r97b_attn_packed_fwd": (c_i32, [c_vp, c_vp, c_vp]),
+    "r97b_attn_packed_bwd": (c_i32, [c_vp, c_vp, c_vp]),
+    "r97b_attn_packed_bwd_workspace_bytes": (c_i64, [c_vp, c_i32, c_i32, c_i32]),
+    "r97b_rope_tables": (c_i32, [c_vp, c_vp, c_i64, c_i32, ctypes.c_double, c_i32, ctypes.c_double, ctypes.c_double,
+                                 ctypes.c_double, ctypes.c_double, c_vp]),
+    "r97b_qk_rope_fwd": (c_i32, [c_vp, c_vp]),
+    "r97b_qk_rope_bwd": (c_i32, [c_vp, c_vp]),
     "r97b_launch_count": (ctypes.c_uint64, []),
     "r97b_adamw_step_dev": (c_i32, [c_vp, c_vp, c_vp, c_vp, c_i64, c_vp, c_f32, c_f32, c_f32, c_f32, c_f32, c_vp,
                                     c_i32, c_vp]),

@@ -39,6 +39,14 @@ unsigned attn_fwd_error_word();
 unsigned gdn_error_word();
 unsigned loss_error_word();
 unsigned gemm_i8_error_word();
+unsigned rope_error_word();
+
+// Whether token-major head rows (R97bHeadRows) follow the ABI's rules for `heads` rows of D a token.
+inline bool head_rows_ok(const R97bHeadRows& r, int64_t heads, int32_t D) {
+    if (!r.ptr || (reinterpret_cast<uintptr_t>(r.ptr) & 15) || heads < 1 || heads > 65536) return false;
+    if (r.head % 8 || r.tok % 8 || r.head < D || r.head > (1 << 24)) return false;
+    return r.tok >= (heads - 1) * r.head + D && r.tok <= (1 << 30);
+}
 
 inline cudaStream_t as_stream(void* s) { return reinterpret_cast<cudaStream_t>(s); }
 
