@@ -7,7 +7,9 @@
 //   dk_j = scale sum_t ds_tj q_t                                          (dk, dv summed over the group's heads)
 //
 // One warp a row, f32 throughout.
+#include "sm100.cuh"
 #include "r97b_internal.h"
+#include "fastmath.cuh"
 
 #include <algorithm>
 #include <cuda_bf16.h>
@@ -16,6 +18,9 @@
 #include <vector>
 
 namespace r97b {
+
+R97B_ERROR_READER(attn_packed_error_word)
+
 namespace {
 
 struct Rows {
@@ -52,32 +57,409 @@ __device__ __forceinline__ float dot(const float (&a)[N], const float (&b)[N]) {
     return sum32(s);
 }
 
-// grid (block, head, 16): 8 warps, one row each
-template <int N>
-__global__ void __launch_bounds__(256) fwd_simple(const Args a) {
-    const int4 b = a.blocks[blockIdx.x];
-    const int h = blockIdx.y, lane = threadIdx.x & 31, r = b.z * 128 + blockIdx.z * 8 + (threadIdx.x >> 5);
-    if (r >= b.y) return;
-    float q[N], o[N], x[N];
-    ld<N>(a.q.at(b.x + r, h) + lane, q);
-#pragma unroll
-    for (int i = 0; i < N; ++i) o[i] = 0.0f;
-    float m = -INFINITY, l = 0.0f;
-    for (int j = 0; j <= r; ++j) {
-        ld<N>(a.k.at(b.x + j, h / a.grp) + lane, x);
-        const float s = dot<N>(q, x) * a.scale, mn = fmaxf(m, s);
-        const float c = mn == -INFINITY ? 1.0f : expf(m - mn), p = mn == -INFINITY ? 0.0f : expf(s - mn);
-        ld<N>(a.v.at(b.x + j, h / a.grp) + lane, x);
-#pragma unroll
-        for (int i = 0; i < N; ++i) o[i] = o[i] * c + p * x[i];
-        l = l * c + p;
-        m = mn;
-    }
-    __nv_bfloat16* op = a.o.at(b.x + r, h) + lane;
-#pragma unroll
-    for (int i = 0; i < N; ++i) op[32 * i] = __float2bfloat16_rn(o[i] / l);
-    if (lane == 0) a.lse[h * a.ld_lse + b.x + r] = m + logf(l);
+// ------------------------------------------------------------------------------------------ forward
+
+constexpr int kBlk = 128;           // queries of a unit, keys of a tile
+constexpr int kChunk = 16384;       // one ring stage
+constexpr int kThreads = 384;       // warp 0: TMA, warp 1: MMA, warps 4-7 and 8-11: two softmax warpgroups
+constexpr int kCtrlRegs = 56, kSoftRegs = 224;  // 128 x 56 + 256 x 224 = 384 x 168, what the launch holds
+static_assert(128 * kCtrlRegs + 256 * kSoftRegs <= 384 * 168, "register split");
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+constexpr float kLazy = 8.0f;       // log2 units a row's maximum may outgrow the reference before O is rescaled
+
+// mbar_wait by every lane of a warp with one outcome for all: the warp stays together when a wait gives up.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort) {
+    return __all_sync(0xFFFFFFFFu, mbar_wait(bar, parity, abort));
 }
+
+template <int D>
+struct FCfg {
+    static constexpr int kQBytes = kBlk * D * 2;
+    static constexpr int kQStages = D == 128 ? 2 : 1;
+    static constexpr int kORing = D == 128 ? 2 : 1;      // O accumulators in TMEM
+    static constexpr int kStages = 9;
+    static constexpr int kRingOff = kQStages * kQBytes;
+    static constexpr int kBarOff = kRingOff + kStages * kChunk;
+    static constexpr int kMaxOff = kBarOff + 512;        // float [2][128]: the reference each warpgroup used last
+    static constexpr int kFinOff = kMaxOff + 1024;       // float2 [2 (unit parity)][2][128]: (reference, sum)
+    static constexpr int kSmemBytes = kFinOff + 4096 + 1024;
+    static constexpr int kVRows = kChunk / (D * 2);      // keys of one V chunk
+};
+
+struct FwdArgs {
+    const int4* blocks;
+    __nv_bfloat16* o;
+    float* lse;
+    int64_t o_tok, o_head, ld_lse;
+    int32_t Hq, grp, units;
+    int32_t q_head, k_head, v_head;
+    float sl2;   // |scale| log2 e (1 for a scale of 0), so that the row maximum is the scores'
+    float sign;  // of the scale: 1, -1 or 0
+};
+
+struct Unit {
+    int h, tok0, i, n;  // head, the block's first token, its index in the sequence, its tokens
+};
+
+// A CTA's t-th unit: a snake over the longest-first order, so a heavy unit of one round meets a light one in the next.
+__device__ __forceinline__ int unit_of(int t, int c, int G) { return t * G + ((t & 1) ? (G - 1 - c) : c); }
+
+__device__ __forceinline__ Unit unit_geom(const int4* blocks, int heads, int u) {
+    const int b = u / heads;
+    const int4 e = blocks[b];
+    return Unit{u - b * heads, e.x + e.z * kBlk, e.z, min(kBlk, e.y - e.z * kBlk)};
+}
+
+// One pass over the keys. A unit is one 128-query block of one head; key tile j of it: S_j = Q K_j^T into one of two
+// TMEM buffers, P_j = 2^(S_j c - m) as bf16 over the same buffer's columns, O += P_j V_j in TMEM. The two softmax
+// warpgroups take the tiles in turn (a thread a row), so the exponentials of one tile run beside the row maximum of the
+// next and both beside the products: S_{j+1} is issued before P_j V_j. The reference m a row's exponentials use is
+// handed from tile to tile; it is moved (and O rescaled, by the threads that own the rows) only when the row's maximum
+// has outgrown it by 2^8, which f32 sums and bf16 probabilities carry without loss.
+template <int D>
+__global__ void __launch_bounds__(kThreads, 1)
+    fwd_kernel(const __grid_constant__ CUtensorMap tQ, const __grid_constant__ CUtensorMap tK,
+               const __grid_constant__ CUtensorMap tV, const FwdArgs args) {
+    using C = FCfg<D>;
+    constexpr int ND = D / 64;
+    constexpr int kVC = kBlk / C::kVRows;  // V chunks of a tile
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+    uint8_t* ring = smem + C::kRingOff;
+    uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + C::kBarOff);
+    uint64_t* empty_bar = full_bar + C::kStages;
+    uint64_t* q_full = empty_bar + C::kStages;  // [2]
+    uint64_t* q_empty = q_full + 2;             // [2]
+    uint64_t* s_full = q_empty + 2;             // [2]
+    uint64_t* p_full = s_full + 2;              // [2]
+    uint64_t* o_full = p_full + 2;              // [2]
+    uint64_t* o_empty = o_full + 2;             // [2]
+    uint64_t* pv_done = o_empty + 2;            // [2]
+    uint64_t* max_bar = pv_done + 2;            // [2][4]: warpgroup w's warp of lane quarter q published its reference
+    uint64_t* fin_bar = max_bar + 8;            // [2][4]: both warps of a lane quarter published a unit's sums
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(fin_bar + 8);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    float* ref_m = reinterpret_cast<float*>(smem + C::kMaxOff);
+    float2* fin = reinterpret_cast<float2*>(smem + C::kFinOff);
+
+    const int warp = threadIdx.x >> 5;
+    const int lane = threadIdx.x & 31;
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < C::kStages; ++s) {
+            mbar_init(&full_bar[s], 1);
+            mbar_init(&empty_bar[s], 1);
+        }
+        for (int b = 0; b < 2; ++b) {
+            mbar_init(&q_full[b], 1);
+            mbar_init(&q_empty[b], 1);
+            mbar_init(&s_full[b], 1);
+            mbar_init(&p_full[b], 4);
+            mbar_init(&o_full[b], 1);
+            mbar_init(&o_empty[b], 8);
+            mbar_init(&pv_done[b], 1);
+        }
+        for (int b = 0; b < 8; ++b) {
+            mbar_init(&max_bar[b], 1);
+            mbar_init(&fin_bar[b], 2);
+        }
+        *abort_flag = 0;
+        fence_mbar_init();
+    }
+    if (warp == 1) {
+        tmem_alloc(tmem_slot, 512);
+        tmem_relinquish();
+    }
+    if (warp == 0 && lane == 0) {
+        tma_prefetch(&tQ);
+        tma_prefetch(&tK);
+        tma_prefetch(&tV);
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    const int G = gridDim.x, c = blockIdx.x;
+
+    if (warp < 4) {
+        set_max_regs_dec<kCtrlRegs>();
+        if (warp == 0 && lane == 0) {
+            // --------------------------------------------------------- TMA producer
+            int stage = 0, lt = 0;
+            uint32_t phase = 0;
+            bool ok = true;
+            for (int t = 0; ok && t * G < args.units; ++t) {
+                const int u = unit_of(t, c, G);
+                if (u >= args.units) continue;
+                const Unit un = unit_geom(args.blocks, args.Hq, u);
+                const int shift = kBlk - un.n, kvh = un.h / args.grp;
+                const int seq0 = un.tok0 - un.i * kBlk;
+                const int qs = lt % C::kQStages;
+                if (!mbar_wait(&q_empty[qs], (uint32_t)((lt / C::kQStages) & 1) ^ 1u, abort_flag)) break;
+                mbar_expect_tx(&q_full[qs], C::kQBytes);
+                for (int s = 0; s < ND; ++s)
+                    tma_load_3d(smem + qs * C::kQBytes + s * kChunk, &tQ, &q_full[qs], un.h * args.q_head + 64 * s, -shift,
+                                un.tok0);
+                auto load = [&](const CUtensorMap* map, bool v, int j) {
+                    const int tok = seq0 + j * kBlk, r0 = j == un.i ? -shift : 0;
+                    for (int ch = 0; ch < (v ? kVC : ND); ++ch) {
+                        if (!(ok = ok && mbar_wait(&empty_bar[stage], phase ^ 1u, abort_flag))) return;
+                        uint8_t* st = ring + stage * kChunk;
+                        mbar_expect_tx(&full_bar[stage], kChunk);
+                        if (v) {
+                            for (int n = 0; n < ND; ++n)
+                                tma_load_3d(st + n * (C::kVRows * 128), map, &full_bar[stage],
+                                            kvh * args.v_head + 64 * n, r0 + ch * C::kVRows, tok);
+                        } else {
+                            tma_load_3d(st, map, &full_bar[stage], kvh * args.k_head + 64 * ch, r0, tok);
+                        }
+                        if (++stage == C::kStages) {
+                            stage = 0;
+                            phase ^= 1u;
+                        }
+                    }
+                };
+                load(&tK, false, 0);
+                for (int j = 0; j <= un.i && ok; ++j) {
+                    if (j < un.i) load(&tK, false, j + 1);
+                    load(&tV, true, j);
+                }
+                ++lt;
+            }
+        } else if (warp == 1 && lane == 0) {
+            // --------------------------------------------------------- MMA issuer
+            constexpr uint32_t idesc_s = make_idesc_bf16(kBlk, kBlk, 0, 0);
+            constexpr uint32_t idesc_o = make_idesc_bf16(kBlk, D, 0, 1);
+            int stage = 0, lt = 0, g = 0;  // g: tiles whose S has been issued
+            uint32_t phase = 0;
+            bool ok = true;
+            auto next = [&]() {
+                umma_commit(&empty_bar[stage]);
+                if (++stage == C::kStages) {
+                    stage = 0;
+                    phase ^= 1u;
+                }
+            };
+            for (int t = 0; ok && t * G < args.units; ++t) {
+                const int u = unit_of(t, c, G);
+                if (u >= args.units) continue;
+                const int nt = unit_geom(args.blocks, args.Hq, u).i + 1;
+                const int qs = lt % C::kQStages, ob = lt % C::kORing;
+                if (!mbar_wait(&q_full[qs], (uint32_t)((lt / C::kQStages) & 1), abort_flag)) break;
+                tc_fence_after();
+                const uint32_t q_addr = smem_u32(smem + qs * C::kQBytes), o_tmem = tmem + 256u + (uint32_t)(ob * 128);
+                // S into buffer g & 1, whose last P the tensor core has taken: P V of two tiles back is before it in
+                // the issue order
+                auto issue_s = [&](bool last) {
+                    for (int kb = 0; kb < ND; ++kb) {
+                        if (!(ok = ok && mbar_wait(&full_bar[stage], phase, abort_flag))) return;
+                        tc_fence_after();
+                        const uint32_t sa = q_addr + kb * kChunk, sb = smem_u32(ring + stage * kChunk);
+#pragma unroll
+                        for (int kk = 0; kk < 4; ++kk)
+                            umma_f16(tmem + (uint32_t)((g & 1) * kBlk), make_sdesc_sw128(sa + kk * 32, 16, 1024),
+                                     make_sdesc_sw128(sb + kk * 32, 16, 1024), idesc_s, (kb > 0 || kk > 0) ? 1u : 0u);
+                        next();
+                    }
+                    umma_commit(&s_full[g & 1]);
+                    if (last) umma_commit(&q_empty[qs]);
+                    ++g;
+                };
+                const int g0 = g;
+                issue_s(nt == 1);
+                for (int j = 0; j < nt && ok; ++j) {
+                    if (j + 1 < nt) issue_s(j + 2 == nt);
+                    if (!ok) break;
+                    const int gj = g0 + j, b = gj & 1;
+                    if (!(ok = mbar_wait(&p_full[b], (uint32_t)((gj >> 1) & 1), abort_flag))) break;
+                    if (j == 0 &&
+                        !(ok = mbar_wait(&o_empty[ob], (uint32_t)((lt / C::kORing) & 1) ^ 1u, abort_flag)))
+                        break;
+                    tc_fence_after();
+                    for (int ch = 0; ch < kVC; ++ch) {
+                        if (!(ok = mbar_wait(&full_bar[stage], phase, abort_flag))) break;
+                        tc_fence_after();
+                        const uint32_t sv = smem_u32(ring + stage * kChunk);
+#pragma unroll
+                        for (int kk = 0; kk < C::kVRows / 16; ++kk)
+                            umma_f16_ts(o_tmem, tmem + (uint32_t)(b * kBlk + (ch * C::kVRows + kk * 16) / 2),
+                                        make_sdesc_sw128(sv + kk * 2048, C::kVRows * 128, 1024), idesc_o,
+                                        (j > 0 || ch > 0 || kk > 0) ? 1u : 0u);
+                        next();
+                    }
+                    if (!ok) break;
+                    umma_commit(&pv_done[b]);
+                }
+                if (!ok) break;
+                umma_commit(&o_full[ob]);
+                ++lt;
+            }
+        }
+    } else {
+        // ------------------------------------------------------------- softmax
+        set_max_regs_inc<kSoftRegs>();
+        const int q = warp & 3, w = (warp - 4) >> 2;
+        const int row = q * 32 + lane;
+        const uint32_t lane_off = (uint32_t)(q * 32) << 16;
+        const uint32_t s_tmem = tmem + lane_off + (uint32_t)(w * kBlk);
+        int g0 = 0, lt = 0;
+        bool ok = true;
+        for (int t = 0; ok && t * G < args.units; ++t) {
+            const int u = unit_of(t, c, G);
+            if (u >= args.units) continue;
+            const Unit un = unit_geom(args.blocks, args.Hq, u);
+            const int shift = kBlk - un.n, nt = un.i + 1, ob = lt % C::kORing;
+            const uint32_t o_tmem = tmem + lane_off + 256u + (uint32_t)(ob * 128);
+            float m = 0.0f, l = 0.0f;  // the reference of this warpgroup's last tile, its tiles' sum relative to it
+            for (int j = (g0 + w) & 1; j < nt; j += 2) {
+                const int g = g0 + j;
+                if (!(ok = warp_wait(&s_full[w], (uint32_t)((g >> 1) & 1), abort_flag))) break;
+                tc_fence_after();
+                float x[128];
+                __syncwarp();
+#pragma unroll
+                for (int cc = 0; cc < 4; ++cc)
+                    tmem_ld32(s_tmem + (uint32_t)(cc * 32), *reinterpret_cast<uint32_t(*)[32]>(&x[cc * 32]));
+                tmem_ld_wait();
+                if (args.sign != 1.0f) {
+#pragma unroll
+                    for (int e = 0; e < 128; ++e) x[e] *= args.sign;
+                }
+                if (j == un.i) {
+#pragma unroll
+                    for (int e = 0; e < 128; ++e)
+                        if (e > row || e < shift) x[e] = -INFINITY;
+                }
+                float mx[4] = {x[0], x[1], x[2], x[3]};
+#pragma unroll
+                for (int e = 4; e < 128; ++e) mx[e & 3] = fmaxf(mx[e & 3], x[e]);
+                const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * args.sl2;
+                float mn;
+                if (j == 0) {
+                    mn = top > -INFINITY ? top : 0.0f;  // a row of nothing visible (or of -inf scores) sums to 0
+                } else {
+                    if (!(ok = warp_wait(&max_bar[(w ^ 1) * 4 + q], (uint32_t)(((g - 1) >> 1) & 1), abort_flag))) break;
+                    const float mp = ref_m[(w ^ 1) * 128 + row];
+                    mn = top > mp + kLazy ? top : mp;
+                    if (__any_sync(0xFFFFFFFFu, mn != mp)) {
+                        // O still holds sums relative to mp: wait for the last P V, then move it to mn
+                        if (!(ok = warp_wait(&pv_done[(g - 1) & 1], (uint32_t)(((g - 1) >> 1) & 1), abort_flag))) break;
+                        tc_fence_after();
+                        const float f = ex2_ftz(mp - mn);
+#pragma unroll 1
+                        for (int cc = 0; cc < D / 32; ++cc) {
+                            uint32_t r[32];
+                            tmem_ld32(o_tmem + (uint32_t)(cc * 32), r);
+                            tmem_ld_wait();
+#pragma unroll
+                            for (int e = 0; e < 32; ++e) r[e] = __float_as_uint(__uint_as_float(r[e]) * f);
+                            tmem_st32(o_tmem + (uint32_t)(cc * 32), r);
+                        }
+                    }
+                }
+                ref_m[w * 128 + row] = mn;
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&max_bar[w * 4 + q]);
+                if (j >= 2) l *= ex2_ftz(m - mn);
+                m = mn;
+                float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int cc = 0; cc < 2; ++cc) {
+                    uint32_t pk[32];
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) {
+                        const float p0 = ex2_ftz(fmaf(x[cc * 64 + 2 * e], args.sl2, -m));
+                        const float p1 = ex2_ftz(fmaf(x[cc * 64 + 2 * e + 1], args.sl2, -m));
+                        s[(2 * e) & 3] += p0;
+                        s[(2 * e + 1) & 3] += p1;
+                        const __nv_bfloat162 b2 = __floats2bfloat162_rn(p0, p1);
+                        pk[e] = *reinterpret_cast<const uint32_t*>(&b2);
+                    }
+                    tmem_st32(s_tmem + (uint32_t)(cc * 32), pk);
+                }
+                tmem_st_wait();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&p_full[w]);
+                l += (s[0] + s[1]) + (s[2] + s[3]);
+            }
+            if (!ok) break;
+            // both warpgroups' sums of the row, moved to the last tile's reference
+            float2* mine = fin + (lt & 1) * 256;
+            mine[w * 128 + row] = make_float2(m, l);
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&fin_bar[(lt & 1) * 4 + q]);
+            if (!(ok = warp_wait(&fin_bar[(lt & 1) * 4 + q], (uint32_t)((lt >> 1) & 1), abort_flag))) break;
+            const int wl = (g0 + nt - 1) & 1;  // the warpgroup of the last tile
+            const float2 last = mine[wl * 128 + row], other = mine[(wl ^ 1) * 128 + row];
+            const float sum = last.y + (nt > 1 ? other.y * ex2_ftz(other.x - last.x) : 0.0f);
+            if (!(ok = warp_wait(&o_full[ob], (uint32_t)((lt / C::kORing) & 1), abort_flag))) break;
+            tc_fence_after();
+            const int64_t tok = un.tok0 + row - shift;
+            if (w == 0 && row >= shift) args.lse[un.h * args.ld_lse + tok] = fmaf(last.x, kLn2, logf(sum));
+            const float inv = 1.0f / sum;
+            __nv_bfloat16* op = args.o + tok * args.o_tok + un.h * args.o_head + w * (D / 2);
+#pragma unroll 1
+            for (int cc = 0; cc < D / 64; ++cc) {
+                uint32_t r[32];
+                __syncwarp();
+                tmem_ld32(o_tmem + (uint32_t)(w * (D / 2) + cc * 32), r);
+                tmem_ld_wait();
+                if (row >= shift) {
+#pragma unroll
+                    for (int v = 0; v < 4; ++v) {
+                        uint32_t pk[4];
+#pragma unroll
+                        for (int h2 = 0; h2 < 4; ++h2) {
+                            const __nv_bfloat162 b2 =
+                                __floats2bfloat162_rn(__uint_as_float(r[v * 8 + h2 * 2]) * inv,
+                                                      __uint_as_float(r[v * 8 + h2 * 2 + 1]) * inv);
+                            pk[h2] = *reinterpret_cast<const uint32_t*>(&b2);
+                        }
+                        *reinterpret_cast<uint4*>(op + cc * 32 + v * 8) = make_uint4(pk[0], pk[1], pk[2], pk[3]);
+                    }
+                }
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&o_empty[ob]);
+            g0 += nt;
+            ++lt;
+        }
+        if (!ok) *abort_flag = 1;
+    }
+
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        tc_fence_after();
+        tmem_dealloc(tmem, 512);
+    }
+}
+
+template <int D>
+int launch_fwd(const R97bPacked& p, const R97bAttnPackedFwd& a, cudaStream_t st) {
+    using C = FCfg<D>;
+    static_assert(C::kSmemBytes <= 232448, "shared memory");
+    CUtensorMap q, k, v;
+    if (!make_rows_map(&q, a.q, a.Hq, D, p.T, kBlk) || !make_rows_map(&k, a.k, a.Hkv, D, p.T, kBlk) ||
+        !make_rows_map(&v, a.v, a.Hkv, D, p.T, C::kVRows))
+        return R97B_EINVAL;
+    FwdArgs r{};
+    r.blocks = reinterpret_cast<const int4*>(p.q_blocks);
+    r.o = reinterpret_cast<__nv_bfloat16*>(a.o.ptr);
+    r.lse = a.lse;
+    r.o_tok = a.o.tok, r.o_head = a.o.head, r.ld_lse = a.ld_lse;
+    r.Hq = a.Hq, r.grp = a.Hq / a.Hkv, r.units = p.n_blocks * a.Hq;
+    r.q_head = (int32_t)a.q.head, r.k_head = (int32_t)a.k.head, r.v_head = (int32_t)a.v.head;
+    r.sl2 = a.scale == 0.0f ? 1.0f : fabsf(a.scale) * kLog2e;
+    r.sign = a.scale == 0.0f ? 0.0f : (a.scale < 0.0f ? -1.0f : 1.0f);
+    if (!smem_opt_in(fwd_kernel<D>, C::kSmemBytes)) return R97B_ELAUNCH;
+    fwd_kernel<D><<<min(num_sms(), r.units), kThreads, C::kSmemBytes, st>>>(q, k, v, r);
+    return launch_status();
+}
+
+// ------------------------------------------------------------------------------------------ backward
 
 template <int N>
 __global__ void __launch_bounds__(256) dq_simple(const Args a) {
@@ -147,6 +529,7 @@ bool plan_ok(const R97bPacked* p) {
 bool heads_ok(int32_t Hq, int32_t Hkv, int32_t D) {
     return Hq > 0 && Hkv > 0 && Hq % Hkv == 0 && Hq <= 65535 && (D == 128 || D == 256);
 }
+bool units_ok(const R97bPacked* p, int32_t H) { return (int64_t)p->n_blocks * H <= 0x3FFFFFFF; }
 bool lse_ok(const float* lse, int64_t ld, int64_t T) { return lse && !(reinterpret_cast<uintptr_t>(lse) & 3) && ld >= T; }
 
 }  // namespace
@@ -187,19 +570,11 @@ extern "C" int r97b_attn_packed_fwd(const R97bPacked* p, const R97bAttnPackedFwd
     using namespace r97b;
     if (!plan_ok(p) || !a || !heads_ok(a->Hq, a->Hkv, a->D)) return R97B_EINVAL;
     if (!head_rows_ok(a->q, a->Hq, a->D) || !head_rows_ok(a->k, a->Hkv, a->D) || !head_rows_ok(a->v, a->Hkv, a->D) ||
-        !head_rows_ok(a->o, a->Hq, a->D) || !lse_ok(a->lse, a->ld_lse, p->T))
+        !head_rows_ok(a->o, a->Hq, a->D) || !lse_ok(a->lse, a->ld_lse, p->T) || !units_ok(p, a->Hq))
         return R97B_EINVAL;
     if (p->T == 0) return R97B_OK;
-    Args r{};
-    r.blocks = reinterpret_cast<const int4*>(p->q_blocks);
-    r.q = rows_of(a->q), r.k = rows_of(a->k), r.v = rows_of(a->v), r.o = rows_of(a->o);
-    r.lse = a->lse, r.ld_lse = a->ld_lse, r.Hq = a->Hq, r.grp = a->Hq / a->Hkv, r.scale = a->scale;
-    const dim3 grid(p->n_blocks, a->Hq, 16);
-    if (a->D == 256)
-        fwd_simple<8><<<grid, 256, 0, as_stream(stream)>>>(r);
-    else
-        fwd_simple<4><<<grid, 256, 0, as_stream(stream)>>>(r);
-    return launch_status();
+    cudaStream_t st = as_stream(stream);
+    return a->D == 256 ? launch_fwd<256>(*p, *a, st) : launch_fwd<128>(*p, *a, st);
 }
 
 extern "C" int64_t r97b_attn_packed_bwd_workspace_bytes(const R97bPacked* p, int32_t Hq, int32_t Hkv, int32_t D) {

@@ -53,7 +53,7 @@ extern "C" const char* r97b_launch_error_name(int code) { return cudaGetErrorNam
 extern "C" int r97b_device_error(unsigned int* out_bits) {
     unsigned bits = r97b::gemm_error_word() | r97b::attn_error_word() | r97b::attn_fwd_error_word() |
                     r97b::gdn_error_word() | r97b::loss_error_word() | r97b::gemm_i8_error_word() |
-                    r97b::rope_error_word();
+                    r97b::rope_error_word() | r97b::attn_packed_error_word();
     if (out_bits) *out_bits = bits;
     return cudaGetLastError() == cudaSuccess ? R97B_OK : R97B_ELAUNCH;
 }

@@ -727,6 +727,18 @@ bool make_map(CUtensorMap* map, const void* ptr, int64_t inner, int64_t outer, i
     return r == CUDA_SUCCESS;
 }
 
+bool make_rows_map(CUtensorMap* map, const R97bHeadRows& r, int64_t heads, int32_t D, int64_t T, int box_rows) {
+    if (!encode_fn()) return false;
+    cuuint64_t dims[3] = {(cuuint64_t)((heads - 1) * r.head + D), 128, (cuuint64_t)T};
+    cuuint64_t strides[2] = {(cuuint64_t)(r.tok * 2), (cuuint64_t)(r.tok * 2)};
+    cuuint32_t box[3] = {64, (cuuint32_t)box_rows, 1};
+    cuuint32_t estr[3] = {1, 1, 1};
+    CUresult rc = g_encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, r.ptr, dims, strides, box, estr,
+                           CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return rc == CUDA_SUCCESS;
+}
+
 // Operand X of logical shape [rows, K] (rows = M for A, N for B) with its majorness.
 bool operand_map(CUtensorMap* map, const R97bMat& m, int64_t rows, int64_t K, int box_rows) {
     if (m.mn_major)  // stored [K, rows]

@@ -22,6 +22,11 @@ int gemm_run(const R97bGemm& g, cudaStream_t stream);
 // (box_inner, box_outer) box and the 128-byte swizzle (gemm_tc.cu).
 bool make_map(CUtensorMap* map, const void* ptr, int64_t inner, int64_t outer, int64_t ld, int box_inner,
               int box_outer);
+// Token-major head rows as a 3D TMA map (column, row of a 128-token block, block's first token) with a
+// (64, box_rows, 1) box: the block at token t is (x, r, t), r < 128, row r of it being token t + r. The rows and
+// the tokens step by the same stride, so a box that starts at a negative r is zero there: a block of n < 128 tokens
+// is loaded from r = n - 128 and lies at the end of its tile, with zero rows -- never a neighbour's -- before it.
+bool make_rows_map(CUtensorMap* map, const R97bHeadRows& r, int64_t heads, int32_t D, int64_t T, int box_rows);
 int num_sms();
 // Opts kernel `fn` into at least `bytes` of dynamic shared memory on the device that is current. The
 // runtime keeps this attribute per device; it is raised (never lowered) per (kernel, device), under a lock;
@@ -40,6 +45,7 @@ unsigned gdn_error_word();
 unsigned loss_error_word();
 unsigned gemm_i8_error_word();
 unsigned rope_error_word();
+unsigned attn_packed_error_word();
 
 // Whether token-major head rows (R97bHeadRows) follow the ABI's rules for `heads` rows of D a token.
 inline bool head_rows_ok(const R97bHeadRows& r, int64_t heads, int32_t D) {
