@@ -6,7 +6,8 @@
 //   dv_j = sum_t p_tj do_t,  ds_tj = p_tj (do_t . v_j - do_t . o_t),  dq_t = scale sum_j ds_tj k_j,
 //   dk_j = scale sum_t ds_tj q_t                                          (dk, dv summed over the group's heads)
 //
-// One warp a row, f32 throughout.
+// All products on tcgen05 with f32 accumulators in TMEM; P and dS are rounded to bf16 for the second products (half
+// a bf16 step of each, what an output's own rounding costs), statistics and sums stay in f32.
 #include "sm100.cuh"
 #include "r97b_internal.h"
 #include "fastmath.cuh"
@@ -23,46 +24,12 @@ R97B_ERROR_READER(attn_packed_error_word)
 
 namespace {
 
-struct Rows {
-    __nv_bfloat16* p;
-    int64_t tok, head;
-    __device__ __nv_bfloat16* at(int64_t t, int h) const { return p + t * tok + (int64_t)h * head; }
-};
-Rows rows_of(const R97bHeadRows& r) { return Rows{reinterpret_cast<__nv_bfloat16*>(r.ptr), r.tok, r.head}; }
-
-struct Args {
-    const int4* blocks;
-    Rows q, k, v, o, dout, dq, dk, dv;
-    float* lse;
-    int64_t ld_lse;
-    int32_t Hq, grp;
-    float scale;
-};
-
-__device__ __forceinline__ float sum32(float v) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
-    return v;
-}
-template <int N>
-__device__ __forceinline__ void ld(const __nv_bfloat16* p, float (&v)[N]) {
-#pragma unroll
-    for (int i = 0; i < N; ++i) v[i] = __bfloat162float(p[32 * i]);
-}
-template <int N>
-__device__ __forceinline__ float dot(const float (&a)[N], const float (&b)[N]) {
-    float s = 0.0f;
-#pragma unroll
-    for (int i = 0; i < N; ++i) s = fmaf(a[i], b[i], s);
-    return sum32(s);
-}
-
 // ------------------------------------------------------------------------------------------ forward
 
 constexpr int kBlk = 128;           // queries of a unit, keys of a tile
 constexpr int kChunk = 16384;       // one ring stage
 constexpr int kThreads = 384;       // warp 0: TMA, warp 1: MMA, warps 4-7 and 8-11: two softmax warpgroups
-constexpr int kCtrlRegs = 56, kSoftRegs = 224;  // 128 x 56 + 256 x 224 = 384 x 168, what the launch holds
+constexpr int kCtrlRegs = 104, kSoftRegs = 200;  // 128 x 104 + 256 x 200 = 384 x 168, what the launch holds
 static_assert(128 * kCtrlRegs + 256 * kSoftRegs <= 384 * 168, "register split");
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
@@ -461,63 +428,570 @@ int launch_fwd(const R97bPacked& p, const R97bAttnPackedFwd& a, cudaStream_t st)
 
 // ------------------------------------------------------------------------------------------ backward
 
-template <int N>
-__global__ void __launch_bounds__(256) dq_simple(const Args a) {
-    const int4 b = a.blocks[blockIdx.x];
-    const int h = blockIdx.y, lane = threadIdx.x & 31, r = b.z * 128 + blockIdx.z * 8 + (threadIdx.x >> 5);
-    if (r >= b.y) return;
-    float q[N], d[N], g[N], x[N], y[N];
-    ld<N>(a.q.at(b.x + r, h) + lane, q);
-    ld<N>(a.dout.at(b.x + r, h) + lane, d);
-    ld<N>(a.o.at(b.x + r, h) + lane, x);
-    const float delta = dot<N>(d, x), lse = a.lse[h * a.ld_lse + b.x + r];
-#pragma unroll
-    for (int i = 0; i < N; ++i) g[i] = 0.0f;
-    for (int j = 0; j <= r; ++j) {
-        ld<N>(a.k.at(b.x + j, h / a.grp) + lane, x);
-        ld<N>(a.v.at(b.x + j, h / a.grp) + lane, y);
-        const float ds = expf(dot<N>(q, x) * a.scale - lse) * (dot<N>(d, y) - delta);
-#pragma unroll
-        for (int i = 0; i < N; ++i) g[i] = fmaf(ds, x[i], g[i]);
-    }
-    __nv_bfloat16* op = a.dq.at(b.x + r, h) + lane;
-#pragma unroll
-    for (int i = 0; i < N; ++i) op[32 * i] = __float2bfloat16_rn(g[i] * a.scale);
-}
+// The tiles of the backward, recomputed from q, k and the forward's lse. Four kinds of pass share one kernel; each
+// keeps its accumulators in TMEM over a unit's tiles and writes every result once, in a fixed order (no atomics):
+//
+//   kDQ   rows = queries: S = Q K^T, dP = dO V^T, dS = P o (dP - delta);        dQ += dS K
+//   kDKV  rows = keys:    S^T = K Q^T, dP^T = V dO^T;   dV += P^T dO and dK += dS^T Q     (D = 128)
+//   kDV   rows = keys:    S^T = K Q^T;                  dV += P^T dO                      (D = 256)
+//   kDK   rows = keys:    S^T = K Q^T, dP^T = V dO^T;   dK += dS^T Q                      (D = 256)
+//
+// At D = 256 dV and dK of 128 keys fill the 512 TMEM columns by themselves, so they are two passes, the second computing
+// S^T again. The rows' operands stay in shared memory for the unit; the others stream through a ring of 16 KB chunks,
+// K-major for the score products and MN-major for the accumulating ones, whose A operand (P or dS, bf16) the
+// elementwise threads write over the scores' own TMEM columns. Each thread owns a row and one of two warpgroups half of
+// its columns, and the products of one tile run beside the exponentials of the next.
+enum Kind { kDQ = 0, kDKV = 1, kDV = 2, kDK = 3 };
 
-// one warp a key row of one key/value head
-template <int N>
-__global__ void __launch_bounds__(256) dkv_simple(const Args a) {
-    const int4 b = a.blocks[blockIdx.x];
-    const int g = blockIdx.y, lane = threadIdx.x & 31, j = b.z * 128 + blockIdx.z * 8 + (threadIdx.x >> 5);
-    if (j >= b.y) return;
-    float k[N], v[N], dk[N], dv[N], x[N], y[N];
-    ld<N>(a.k.at(b.x + j, g) + lane, k);
-    ld<N>(a.v.at(b.x + j, g) + lane, v);
+template <int D, int KIND>
+struct BCfg {
+    static constexpr bool kDP = KIND != kDV;          // needs dP (a second resident operand, delta)
+    static constexpr bool kKeys = KIND != kDQ;        // rows are keys: lse and delta run along the columns
+    static constexpr int kABytes = kBlk * D * 2;
+    static constexpr int kStages = D == 256 && kDP ? 6 : 9;
+    static constexpr int kRingOff = (kDP ? 2 : 1) * kABytes;
+    static constexpr int kBarOff = kRingOff + kStages * kChunk;
+    static constexpr int kStatOff = kBarOff + 512;    // kKeys: float [2 (stage)][lse, delta][128]
+    static constexpr int kSmemBytes = kStatOff + (kKeys ? 2048 : 0);
+    static constexpr int kVRows = kChunk / (D * 2);
+};
+
+struct BwdArgs {
+    const int4* blocks;
+    const float* lse;
+    const float* delta;
+    int64_t ld_lse, ld_delta;
+    __nv_bfloat16 *out0, *out1;        // kDQ: dq; kDKV: dv, dk; kDV: dv; kDK: dk
+    int64_t tok0, head0, tok1, head1;
+    int32_t a0_head, a1_head, b0_head, b1_head, c0_head, c1_head;
+    int32_t heads, grp, units;         // the rows' heads (query heads for kDQ, key/value heads else)
+    float sl2, scale;
+};
+
+// A unit's tiles: kDQ walks the key blocks up to its own; the others every query block from their own on, head by head.
+template <int KIND>
+struct Walk {
+    int h, i, n, seq0, tok0, len, m, tiles, grp;
+    __device__ Walk(const BwdArgs& a, int u) {
+        const int b = u / a.heads;
+        const int4 e = a.blocks[b];
+        h = u - b * a.heads;
+        i = e.z;
+        seq0 = e.x;
+        len = e.y;
+        tok0 = seq0 + i * kBlk;
+        n = min(kBlk, len - i * kBlk);
+        grp = a.grp;
+        m = KIND == kDQ ? i + 1 : (len + kBlk - 1) / kBlk - i;
+        tiles = KIND == kDQ ? m : m * a.grp;
+    }
+    __device__ int shift() const { return kBlk - n; }
+    __device__ int block(int t) const { return KIND == kDQ ? t : i + t % m; }           // the tile's column block
+    __device__ int head(int t) const { return KIND == kDQ ? h / grp : h * grp + t / m; }  // and its head
+    __device__ int shift_of(int blk) const { return kBlk - min(kBlk, len - blk * kBlk); }
+};
+
+template <int D, int KIND>
+__global__ void __launch_bounds__(kThreads, 1)
+    bwd_kernel(const __grid_constant__ CUtensorMap tA0, const __grid_constant__ CUtensorMap tA1,
+               const __grid_constant__ CUtensorMap tB0, const __grid_constant__ CUtensorMap tB1,
+               const __grid_constant__ CUtensorMap tC0, const __grid_constant__ CUtensorMap tC1, const BwdArgs args) {
+    using C = BCfg<D, KIND>;
+    constexpr int ND = D / 64;
+    constexpr int kVC = kBlk / C::kVRows;
+    extern __shared__ __align__(1024) uint8_t smem[];
+    uint8_t* ring = smem + C::kRingOff;
+    uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + C::kBarOff);
+    uint64_t* empty_bar = full_bar + C::kStages;
+    uint64_t* a_full = empty_bar + C::kStages;   // [2]
+    uint64_t* a_empty = a_full + 2;              // [2]
+    uint64_t* s_full = a_empty + 2;              // [2]
+    uint64_t* s_free = s_full + 2;               // kDQ, kDK: S read into registers
+    uint64_t* p_full = s_free + 1;               // [2] kDV, kDKV: P written
+    uint64_t* dp_full = p_full + 2;
+    uint64_t* ds_full = dp_full + 1;
+    uint64_t* acc_full = ds_full + 1;
+    uint64_t* acc_empty = acc_full + 1;
+    uint64_t* stat_full = acc_empty + 1;         // [2]
+    uint64_t* stat_empty = stat_full + 2;        // [2]
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(stat_empty + 2);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    float* stats = reinterpret_cast<float*>(smem + C::kStatOff);
+
+    const int warp = threadIdx.x >> 5;
+    const int lane = threadIdx.x & 31;
+    if (smem_u32(smem) & 1023u) {  // the swizzled tiles need it; the attribute above asks for it
+        if (threadIdx.x == 0) atomicOr(&g_device_error, kErrArgs);
+        return;
+    }
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < C::kStages; ++s) {
+            mbar_init(&full_bar[s], 1);
+            mbar_init(&empty_bar[s], 1);
+        }
+        for (int b = 0; b < 2; ++b) {
+            mbar_init(&a_full[b], 1);
+            mbar_init(&a_empty[b], 1);
+            mbar_init(&s_full[b], 1);
+            mbar_init(&p_full[b], 8);
+            mbar_init(&stat_full[b], 1);
+            mbar_init(&stat_empty[b], 8);
+        }
+        mbar_init(s_free, 8);
+        mbar_init(dp_full, 1);
+        mbar_init(ds_full, 8);
+        mbar_init(acc_full, 1);
+        mbar_init(acc_empty, 8);
+        *abort_flag = 0;
+        fence_mbar_init();
+    }
+    if (warp == 1) {
+        tmem_alloc(tmem_slot, 512);
+        tmem_relinquish();
+    }
+    if (warp == 0 && lane == 0) {
+        tma_prefetch(&tA0);
+        tma_prefetch(&tB0);
+        tma_prefetch(&tC0);
+        if (C::kDP) {
+            tma_prefetch(&tA1);
+            tma_prefetch(&tB1);
+        }
+        if (KIND == kDKV) tma_prefetch(&tC1);
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    const uint32_t acc0 = tmem + 256u, acc1 = tmem + 384u;  // acc1: kDKV's dK
+    const int G = gridDim.x, c = blockIdx.x;
+
+    if (warp < 4) {
+        set_max_regs_dec<kCtrlRegs>();
+        if (warp == 0 && lane == 0) {
+            // --------------------------------------------------------- TMA producer
+            int stage = 0, lt = 0;
+            uint32_t phase = 0;
+            bool ok = true;
+            auto slot = [&]() -> uint8_t* {
+                if (!(ok = ok && mbar_wait(&empty_bar[stage], phase ^ 1u, abort_flag))) return nullptr;
+                mbar_expect_tx(&full_bar[stage], kChunk);
+                return ring + stage * kChunk;
+            };
+            auto next = [&]() {
+                if (++stage == C::kStages) {
+                    stage = 0;
+                    phase ^= 1u;
+                }
+            };
+            for (int t = 0; ok && t * G < args.units; ++t) {
+                const int u = unit_of(t, c, G);
+                if (u >= args.units) continue;
+                const Walk<KIND> wk(args, u);
+                for (int r = 0; r < (C::kDP ? 2 : 1); ++r) {
+                    if (!(ok = ok && mbar_wait(&a_empty[r], (uint32_t)(lt & 1) ^ 1u, abort_flag))) break;
+                    mbar_expect_tx(&a_full[r], C::kABytes);
+                    for (int s = 0; s < ND; ++s)
+                        tma_load_3d(smem + r * C::kABytes + s * kChunk, r ? &tA1 : &tA0, &a_full[r],
+                                    wk.h * (r ? args.a1_head : args.a0_head) + 64 * s, -wk.shift(), wk.tok0);
+                }
+                // a column block K-major (the score products), or MN-major (the accumulating ones)
+                auto load_b = [&](const CUtensorMap* map, int head_stride, int tile) {
+                    const int blk = wk.block(tile), x = wk.head(tile) * head_stride;
+                    for (int ch = 0; ch < ND; ++ch) {
+                        uint8_t* st = slot();
+                        if (!st) return;
+                        tma_load_3d(st, map, &full_bar[stage], x + 64 * ch, -wk.shift_of(blk), wk.seq0 + blk * kBlk);
+                        next();
+                    }
+                };
+                auto load_c = [&](const CUtensorMap* map, int head_stride, int tile) {
+                    const int blk = wk.block(tile), x = wk.head(tile) * head_stride;
+                    for (int ch = 0; ch < kVC; ++ch) {
+                        uint8_t* st = slot();
+                        if (!st) return;
+                        for (int n = 0; n < ND; ++n)
+                            tma_load_3d(st + n * (C::kVRows * 128), map, &full_bar[stage], x + 64 * n,
+                                        ch * C::kVRows - wk.shift_of(blk), wk.seq0 + blk * kBlk);
+                        next();
+                    }
+                };
+                load_b(&tB0, args.b0_head, 0);
+                if (C::kDP) load_b(&tB1, args.b1_head, 0);
+                for (int j = 0; j < wk.tiles && ok; ++j) {
+                    const bool more = j + 1 < wk.tiles;
+                    if (KIND == kDKV) load_c(&tC0, args.c0_head, j);
+                    if (more) load_b(&tB0, args.b0_head, j + 1);
+                    if (KIND == kDKV)
+                        load_c(&tC1, args.c1_head, j);
+                    else
+                        load_c(&tC0, args.c0_head, j);
+                    if (more && C::kDP) load_b(&tB1, args.b1_head, j + 1);
+                }
+                ++lt;
+            }
+        } else if (warp == 1 && lane == 0) {
+            // --------------------------------------------------------- MMA issuer
+            constexpr uint32_t idesc_s = make_idesc_bf16(kBlk, kBlk, 0, 0);
+            constexpr uint32_t idesc_c = make_idesc_bf16(kBlk, D, 0, 1);
+            int stage = 0, lt = 0, g = 0;  // g: the current unit's first tile
+            uint32_t phase = 0;
+            bool ok = true;
+            auto chunk = [&]() -> uint32_t {  // the next ring chunk's address, or 0 when a wait gave up
+                if (!(ok = ok && mbar_wait(&full_bar[stage], phase, abort_flag))) return 0u;
+                tc_fence_after();
+                return smem_u32(ring + stage * kChunk);
+            };
+            auto next = [&]() {
+                umma_commit(&empty_bar[stage]);
+                if (++stage == C::kStages) {
+                    stage = 0;
+                    phase ^= 1u;
+                }
+            };
+            auto score = [&](int resident, uint32_t d) {
+                const uint32_t sa = smem_u32(smem + resident * C::kABytes);
+                for (int kb = 0; kb < ND; ++kb) {
+                    const uint32_t sb = chunk();
+                    if (!sb) return;
 #pragma unroll
-    for (int i = 0; i < N; ++i) dk[i] = dv[i] = 0.0f;
-    for (int h = g * a.grp; h < (g + 1) * a.grp; ++h) {
-        for (int t = j; t < b.y; ++t) {
-            ld<N>(a.q.at(b.x + t, h) + lane, x);
-            const float p = expf(dot<N>(x, k) * a.scale - a.lse[h * a.ld_lse + b.x + t]);
-            ld<N>(a.dout.at(b.x + t, h) + lane, y);
-            float o[N];
-            ld<N>(a.o.at(b.x + t, h) + lane, o);
-            const float ds = p * (dot<N>(y, v) - dot<N>(y, o));
+                    for (int kk = 0; kk < 4; ++kk)
+                        umma_f16(d, make_sdesc_sw128(sa + kb * kChunk + kk * 32, 16, 1024),
+                                 make_sdesc_sw128(sb + kk * 32, 16, 1024), idesc_s, (kb > 0 || kk > 0) ? 1u : 0u);
+                    next();
+                }
+            };
+            auto accumulate = [&](uint32_t a, uint32_t d, bool first) {
+                for (int ch = 0; ch < kVC; ++ch) {
+                    const uint32_t sb = chunk();
+                    if (!sb) return;
 #pragma unroll
-            for (int i = 0; i < N; ++i) {
-                dv[i] = fmaf(p, y[i], dv[i]);
-                dk[i] = fmaf(ds, x[i], dk[i]);
+                    for (int kk = 0; kk < C::kVRows / 16; ++kk) {
+                        const int k16 = ch * (C::kVRows / 16) + kk;  // the halves' bf16 columns start 64 apart
+                        umma_f16_ts(d, a + (uint32_t)((k16 >> 2) * 64 + (k16 & 3) * 8),
+                                    make_sdesc_sw128(sb + kk * 2048, C::kVRows * 128, 1024), idesc_c,
+                                    (!first || ch > 0 || kk > 0) ? 1u : 0u);
+                    }
+                    next();
+                }
+            };
+            auto wait = [&](uint64_t* bar, int n) {  // the bar's n-th completion
+                ok = ok && mbar_wait(bar, (uint32_t)(n & 1), abort_flag);
+                tc_fence_after();
+            };
+            for (int t = 0; ok && t * G < args.units; ++t) {
+                const int u = unit_of(t, c, G);
+                if (u >= args.units) continue;
+                const Walk<KIND> wk(args, u);
+                const int n = wk.tiles;
+                auto issue_s = [&](int j) {
+                    const int gj = g + j, b = KIND == kDV ? (gj & 1) : 0;
+                    if ((KIND == kDQ || KIND == kDK) && gj > 0) wait(s_free, gj - 1);
+                    if (j == 0) wait(&a_full[0], lt);
+                    if (!ok) return;
+                    score(0, tmem + (uint32_t)(b * kBlk));
+                    umma_commit(&s_full[b]);
+                    if (j + 1 == n) umma_commit(&a_empty[0]);
+                };
+                auto issue_dp = [&](int j) {
+                    if (j == 0) wait(&a_full[1], lt);
+                    if (!ok) return;
+                    score(1, tmem + (uint32_t)kBlk);
+                    umma_commit(dp_full);
+                    if (j + 1 == n) umma_commit(&a_empty[1]);
+                };
+                issue_s(0);
+                if (C::kDP) issue_dp(0);
+                for (int j = 0; j < n && ok; ++j) {
+                    const int gj = g + j;
+                    const bool more = j + 1 < n;
+                    if (KIND == kDKV) {
+                        wait(&p_full[0], gj);
+                        if (j == 0) wait(acc_empty, lt + 1);
+                        if (!ok) break;
+                        accumulate(tmem, acc0, j == 0);
+                        if (more) issue_s(j + 1);
+                        wait(ds_full, gj);
+                        if (!ok) break;
+                        accumulate(tmem + (uint32_t)kBlk, acc1, j == 0);
+                        if (more) issue_dp(j + 1);
+                    } else {
+                        if (more) issue_s(j + 1);
+                        const int b = KIND == kDV ? (gj & 1) : 0;
+                        if (KIND == kDV)
+                            wait(&p_full[b], gj >> 1);
+                        else
+                            wait(ds_full, gj);
+                        if (j == 0) wait(acc_empty, lt + 1);
+                        if (!ok) break;
+                        accumulate(tmem + (uint32_t)(KIND == kDV ? b * kBlk : kBlk), acc0, j == 0);
+                        if (more && C::kDP) issue_dp(j + 1);
+                    }
+                }
+                if (!ok) break;
+                umma_commit(acc_full);
+                g += n;
+                ++lt;
+            }
+        } else if (C::kKeys && warp == 2) {
+            // --------------------------------------------------------- the columns' lse and delta, a tile ahead
+            int g = 0;
+            bool ok = true;
+            for (int t = 0; ok && t * G < args.units; ++t) {
+                const int u = unit_of(t, c, G);
+                if (u >= args.units) continue;
+                const Walk<KIND> wk(args, u);
+                for (int j = 0; j < wk.tiles; ++j, ++g) {
+                    const int blk = wk.block(j), shift = wk.shift_of(blk), h = wk.head(j), st = g & 1;
+                    const int64_t tok = (int64_t)wk.seq0 + blk * kBlk - shift;
+                    float v[8];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int col = e * 32 + lane;
+                        // a column before the block's first token: probability 2^-inf = 0
+                        v[e] = col >= shift ? args.lse[h * args.ld_lse + tok + col] * kLog2e : INFINITY;
+                        v[4 + e] = C::kDP && col >= shift ? args.delta[h * args.ld_delta + tok + col] : 0.0f;
+                    }
+                    if (!(ok = warp_wait(&stat_empty[st], (uint32_t)((g >> 1) & 1) ^ 1u, abort_flag))) break;
+                    float* s = stats + st * 256;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) s[e * 32 + lane] = v[e];
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&stat_full[st]);
+                }
             }
         }
-    }
-    __nv_bfloat16* kp = a.dk.at(b.x + j, g) + lane;
-    __nv_bfloat16* vp = a.dv.at(b.x + j, g) + lane;
+    } else {
+        // ------------------------------------------------------------- probabilities, dS, and the results' rows
+        set_max_regs_inc<kSoftRegs>();
+        const int q = warp & 3, w = (warp - 4) >> 2;
+        const int row = q * 32 + lane;
+        const uint32_t lane_off = (uint32_t)(q * 32) << 16;
+        const uint32_t half = tmem + lane_off + (uint32_t)(w * 64);  // this thread's columns of S (and, 128 on, of dP)
+        int g = 0, lt = 0;
+        bool ok = true;
+        for (int t = 0; ok && t * G < args.units; ++t) {
+            const int u = unit_of(t, c, G);
+            if (u >= args.units) continue;
+            const Walk<KIND> wk(args, u);
+            const int shift = wk.shift();
+            const int64_t tok = (int64_t)wk.tok0 + row - shift;
+            float lse2 = 0.0f, delta = 0.0f;
+            if (!C::kKeys && row >= shift) {
+                lse2 = args.lse[wk.h * args.ld_lse + tok] * kLog2e;
+                delta = args.delta[wk.h * args.ld_delta + tok];
+            }
+            for (int j = 0; j < wk.tiles; ++j, ++g) {
+                const int b = KIND == kDV ? (g & 1) : 0;
+                const bool diag = wk.block(j) == wk.i;
+                const float* st = stats + (g & 1) * 256 + w * 64;
+                if (C::kKeys && !(ok = warp_wait(&stat_full[g & 1], (uint32_t)((g >> 1) & 1), abort_flag))) break;
+                if (!(ok = warp_wait(&s_full[b], (uint32_t)((KIND == kDV ? g >> 1 : g) & 1), abort_flag))) break;
+                tc_fence_after();
+                float p[64];
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-        kp[32 * i] = __float2bfloat16_rn(dk[i] * a.scale);
-        vp[32 * i] = __float2bfloat16_rn(dv[i]);
+                for (int cc = 0; cc < 2; ++cc)
+                    tmem_ld32(half + (uint32_t)(b * kBlk + cc * 32), *reinterpret_cast<uint32_t(*)[32]>(&p[cc * 32]));
+                tmem_ld_wait();
+                if (KIND == kDQ || KIND == kDK) {
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(s_free);
+                }
+                if (C::kKeys) {
+#pragma unroll
+                    for (int e = 0; e < 64; e += 4) {
+                        const float4 l4 = *reinterpret_cast<const float4*>(st + e);
+                        p[e] = ex2_ftz(fmaf(p[e], args.sl2, -l4.x));
+                        p[e + 1] = ex2_ftz(fmaf(p[e + 1], args.sl2, -l4.y));
+                        p[e + 2] = ex2_ftz(fmaf(p[e + 2], args.sl2, -l4.z));
+                        p[e + 3] = ex2_ftz(fmaf(p[e + 3], args.sl2, -l4.w));
+                    }
+                    if (diag) {
+#pragma unroll
+                        for (int e = 0; e < 64; ++e)
+                            if (w * 64 + e < row) p[e] = 0.0f;
+                    }
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 64; ++e) p[e] = ex2_ftz(fmaf(p[e], args.sl2, -lse2));
+                    if (diag) {
+#pragma unroll
+                        for (int e = 0; e < 64; ++e)
+                            if (w * 64 + e > row || w * 64 + e < shift) p[e] = 0.0f;
+                    }
+                }
+                if (KIND == kDV || KIND == kDKV) {
+                    uint32_t pk[32];
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) {
+                        const __nv_bfloat162 b2 = __floats2bfloat162_rn(p[2 * e], p[2 * e + 1]);
+                        pk[e] = *reinterpret_cast<const uint32_t*>(&b2);
+                    }
+                    tmem_st32(half + (uint32_t)(b * kBlk), pk);
+                    tmem_st_wait();
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&p_full[b]);
+                }
+                if (C::kDP) {
+                    if (!(ok = warp_wait(dp_full, (uint32_t)(g & 1), abort_flag))) break;
+                    tc_fence_after();
+                    float d[64];
+#pragma unroll
+                    for (int cc = 0; cc < 2; ++cc)
+                        tmem_ld32(half + (uint32_t)(kBlk + cc * 32), *reinterpret_cast<uint32_t(*)[32]>(&d[cc * 32]));
+                    tmem_ld_wait();
+                    uint32_t pk[32];
+#pragma unroll
+                    for (int e = 0; e < 64; e += 4) {
+                        float4 d4 = make_float4(delta, delta, delta, delta);
+                        if (C::kKeys) d4 = *reinterpret_cast<const float4*>(st + 128 + e);
+                        const __nv_bfloat162 lo = __floats2bfloat162_rn(p[e] * (d[e] - d4.x), p[e + 1] * (d[e + 1] - d4.y));
+                        const __nv_bfloat162 hi =
+                            __floats2bfloat162_rn(p[e + 2] * (d[e + 2] - d4.z), p[e + 3] * (d[e + 3] - d4.w));
+                        pk[e / 2] = *reinterpret_cast<const uint32_t*>(&lo);
+                        pk[e / 2 + 1] = *reinterpret_cast<const uint32_t*>(&hi);
+                    }
+                    tmem_st32(half + (uint32_t)kBlk, pk);
+                    tmem_st_wait();
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(ds_full);
+                }
+                if (C::kKeys) {
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&stat_empty[g & 1]);
+                }
+            }
+            if (!ok) break;
+            if (!(ok = warp_wait(acc_full, (uint32_t)(lt & 1), abort_flag))) break;
+            tc_fence_after();
+#pragma unroll
+            for (int r = 0; r < (KIND == kDKV ? 2 : 1); ++r) {
+                // dV takes no scale; dS is kept unscaled in bf16, so dQ and dK take it here
+                const float f = (KIND == kDV || (KIND == kDKV && r == 0)) ? 1.0f : args.scale;
+                __nv_bfloat16* op = r ? args.out1 + tok * args.tok1 + wk.h * args.head1
+                                      : args.out0 + tok * args.tok0 + wk.h * args.head0;
+                const uint32_t src = (r ? acc1 : acc0) + lane_off + (uint32_t)(w * (D / 2));
+#pragma unroll 1
+                for (int cc = 0; cc < D / 64; ++cc) {
+                    uint32_t v[32];
+                    __syncwarp();
+                    tmem_ld32(src + (uint32_t)(cc * 32), v);
+                    tmem_ld_wait();
+                    if (row >= shift) {
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            uint32_t pk[4];
+#pragma unroll
+                            for (int h2 = 0; h2 < 4; ++h2) {
+                                const __nv_bfloat162 b2 = __floats2bfloat162_rn(__uint_as_float(v[k * 8 + h2 * 2]) * f,
+                                                                                __uint_as_float(v[k * 8 + h2 * 2 + 1]) * f);
+                                pk[h2] = *reinterpret_cast<const uint32_t*>(&b2);
+                            }
+                            *reinterpret_cast<uint4*>(op + w * (D / 2) + cc * 32 + k * 8) =
+                                make_uint4(pk[0], pk[1], pk[2], pk[3]);
+                        }
+                    }
+                }
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(acc_empty);
+            ++lt;
+        }
+        if (!ok) *abort_flag = 1;
     }
+
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        tc_fence_after();
+        tmem_dealloc(tmem, 512);
+    }
+}
+
+// delta[h, t] = sum_d dO[t, h, d] O[t, h, d]: D / 8 lanes a row, 16 bytes a lane.
+struct DeltaArgs {
+    R97bHeadRows o, dout;
+    float* delta;
+    int64_t ld, rows;
+    int32_t heads;
+};
+template <int D>
+__global__ void __launch_bounds__(256) delta_kernel(const DeltaArgs a) {
+    constexpr int kLanes = D / 8;
+    const int64_t r = ((int64_t)blockIdx.x * 256 + threadIdx.x) / kLanes;
+    const int l = threadIdx.x % kLanes;
+    float s = 0.0f;
+    const int64_t t = r / a.heads;
+    const int h = (int)(r - t * a.heads);
+    if (r < a.rows) {
+        const uint4 x = *reinterpret_cast<const uint4*>(reinterpret_cast<const __nv_bfloat16*>(a.o.ptr) + t * a.o.tok +
+                                                        h * a.o.head + 8 * l);
+        const uint4 y = *reinterpret_cast<const uint4*>(reinterpret_cast<const __nv_bfloat16*>(a.dout.ptr) +
+                                                        t * a.dout.tok + h * a.dout.head + 8 * l);
+        const __nv_bfloat162* xp = reinterpret_cast<const __nv_bfloat162*>(&x);
+        const __nv_bfloat162* yp = reinterpret_cast<const __nv_bfloat162*>(&y);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float2 xf = __bfloat1622float2(xp[i]), yf = __bfloat1622float2(yp[i]);
+            s = fmaf(xf.x, yf.x, s);
+            s = fmaf(xf.y, yf.y, s);
+        }
+    }
+#pragma unroll
+    for (int o = kLanes / 2; o > 0; o >>= 1) s += __shfl_xor_sync(0xFFFFFFFFu, s, o);
+    if (r < a.rows && l == 0) a.delta[h * a.ld + t] = s;
+}
+
+int64_t delta_ld(int64_t T) { return (T + 63) / 64 * 64; }
+
+template <int D, int KIND>
+int launch_bwd(const R97bPacked& p, const R97bAttnPackedBwd& a, const float* delta, cudaStream_t st) {
+    using C = BCfg<D, KIND>;
+    static_assert(C::kSmemBytes <= 232448, "shared memory");
+    const bool dq = KIND == kDQ;
+    // the rows' operands, the columns' and the accumulating products'
+    const R97bHeadRows &a0 = dq ? a.q : a.k, &a1 = dq ? a.dout : a.v, &b0 = dq ? a.k : a.q, &b1 = dq ? a.v : a.dout;
+    const R97bHeadRows &c0 = dq ? a.k : (KIND == kDK ? a.q : a.dout), &c1 = a.q;
+    const int ha = dq ? a.Hq : a.Hkv, hb = dq ? a.Hkv : a.Hq;
+    CUtensorMap m[6];
+    if (!make_rows_map(&m[0], a0, ha, D, p.T, kBlk) || !make_rows_map(&m[1], a1, ha, D, p.T, kBlk) ||
+        !make_rows_map(&m[2], b0, hb, D, p.T, kBlk) || !make_rows_map(&m[3], b1, hb, D, p.T, kBlk) ||
+        !make_rows_map(&m[4], c0, hb, D, p.T, C::kVRows) || !make_rows_map(&m[5], c1, a.Hq, D, p.T, C::kVRows))
+        return R97B_EINVAL;
+    BwdArgs r{};
+    r.blocks = reinterpret_cast<const int4*>(dq ? p.q_blocks : p.k_blocks);
+    r.lse = a.lse, r.ld_lse = a.ld_lse, r.delta = delta, r.ld_delta = delta_ld(p.T);
+    const R97bHeadRows &o0 = dq ? a.dq : (KIND == kDK ? a.dk : a.dv), &o1 = a.dk;
+    r.out0 = reinterpret_cast<__nv_bfloat16*>(o0.ptr), r.tok0 = o0.tok, r.head0 = o0.head;
+    r.out1 = reinterpret_cast<__nv_bfloat16*>(o1.ptr), r.tok1 = o1.tok, r.head1 = o1.head;
+    r.a0_head = (int32_t)a0.head, r.a1_head = (int32_t)a1.head, r.b0_head = (int32_t)b0.head, r.b1_head = (int32_t)b1.head;
+    r.c0_head = (int32_t)c0.head, r.c1_head = (int32_t)c1.head;
+    r.heads = ha, r.grp = a.Hq / a.Hkv, r.units = p.n_blocks * ha;
+    r.sl2 = a.scale * kLog2e, r.scale = a.scale;
+    if (!smem_opt_in(bwd_kernel<D, KIND>, C::kSmemBytes)) return R97B_ELAUNCH;
+    bwd_kernel<D, KIND><<<min(num_sms(), r.units), kThreads, C::kSmemBytes, st>>>(m[0], m[1], m[2], m[3], m[4], m[5], r);
+    return launch_status();
+}
+
+template <int D>
+int run_bwd(const R97bPacked& p, const R97bAttnPackedBwd& a, cudaStream_t st) {
+    float* delta = reinterpret_cast<float*>(a.ws);
+    const DeltaArgs d{a.o, a.dout, delta, delta_ld(p.T), p.T * a.Hq, a.Hq};
+    const int64_t grid = (d.rows * (D / 8) + 255) / 256;
+    if (grid > 0x7FFFFFFF) return R97B_EINVAL;
+    delta_kernel<D><<<(unsigned)grid, 256, 0, st>>>(d);
+    int rc = launch_status();
+    if (D == 256) {
+        if (rc == R97B_OK) rc = launch_bwd<D, D == 256 ? kDV : kDKV>(p, a, delta, st);
+        if (rc == R97B_OK) rc = launch_bwd<D, D == 256 ? kDK : kDKV>(p, a, delta, st);
+    } else {
+        if (rc == R97B_OK) rc = launch_bwd<D, D == 256 ? kDV : kDKV>(p, a, delta, st);
+    }
+    return rc == R97B_OK ? launch_bwd<D, kDQ>(p, a, delta, st) : rc;
 }
 
 bool plan_ok(const R97bPacked* p) {
@@ -579,7 +1053,7 @@ extern "C" int r97b_attn_packed_fwd(const R97bPacked* p, const R97bAttnPackedFwd
 
 extern "C" int64_t r97b_attn_packed_bwd_workspace_bytes(const R97bPacked* p, int32_t Hq, int32_t Hkv, int32_t D) {
     if (!r97b::plan_ok(p) || !r97b::heads_ok(Hq, Hkv, D)) return -1;
-    return 0;
+    return (int64_t)Hq * r97b::delta_ld(p->T) * 4;
 }
 
 extern "C" int r97b_attn_packed_bwd(const R97bPacked* p, const R97bAttnPackedBwd* a, void* stream) {
@@ -587,26 +1061,12 @@ extern "C" int r97b_attn_packed_bwd(const R97bPacked* p, const R97bAttnPackedBwd
     if (!plan_ok(p) || !a || !heads_ok(a->Hq, a->Hkv, a->D)) return R97B_EINVAL;
     if (!head_rows_ok(a->q, a->Hq, a->D) || !head_rows_ok(a->k, a->Hkv, a->D) || !head_rows_ok(a->v, a->Hkv, a->D) ||
         !head_rows_ok(a->o, a->Hq, a->D) || !head_rows_ok(a->dout, a->Hq, a->D) || !head_rows_ok(a->dq, a->Hq, a->D) ||
-        !head_rows_ok(a->dk, a->Hkv, a->D) || !head_rows_ok(a->dv, a->Hkv, a->D) || !lse_ok(a->lse, a->ld_lse, p->T))
+        !head_rows_ok(a->dk, a->Hkv, a->D) || !head_rows_ok(a->dv, a->Hkv, a->D) || !lse_ok(a->lse, a->ld_lse, p->T) ||
+        !units_ok(p, a->Hq))
         return R97B_EINVAL;
     const int64_t need = r97b_attn_packed_bwd_workspace_bytes(p, a->Hq, a->Hkv, a->D);
     if (need < 0 || a->ws_bytes < need || (need > 0 && !a->ws) || (reinterpret_cast<uintptr_t>(a->ws) & 255)) return R97B_EINVAL;
     if (p->T == 0) return R97B_OK;
-    Args r{};
-    r.q = rows_of(a->q), r.k = rows_of(a->k), r.v = rows_of(a->v), r.o = rows_of(a->o), r.dout = rows_of(a->dout);
-    r.dq = rows_of(a->dq), r.dk = rows_of(a->dk), r.dv = rows_of(a->dv);
-    r.lse = const_cast<float*>(a->lse), r.ld_lse = a->ld_lse, r.Hq = a->Hq, r.grp = a->Hq / a->Hkv, r.scale = a->scale;
     cudaStream_t st = as_stream(stream);
-    r.blocks = reinterpret_cast<const int4*>(p->q_blocks);
-    const dim3 gq(p->n_blocks, a->Hq, 16), gk(p->n_blocks, a->Hkv, 16);
-    if (a->D == 256)
-        dq_simple<8><<<gq, 256, 0, st>>>(r);
-    else
-        dq_simple<4><<<gq, 256, 0, st>>>(r);
-    r.blocks = reinterpret_cast<const int4*>(p->k_blocks);
-    if (a->D == 256)
-        dkv_simple<8><<<gk, 256, 0, st>>>(r);
-    else
-        dkv_simple<4><<<gk, 256, 0, st>>>(r);
-    return launch_status(2);
+    return a->D == 256 ? run_bwd<256>(*p, *a, st) : run_bwd<128>(*p, *a, st);
 }
