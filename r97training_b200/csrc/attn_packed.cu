@@ -193,7 +193,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
                 ++lt;
             }
-        } else if (warp == 1 && lane == 0) {
+        } else if (warp == 1) {
+            const uint32_t lead = elect_one();
             // --------------------------------------------------------- MMA issuer
             constexpr uint32_t idesc_s = make_idesc_bf16(kBlk, kBlk, 0, 0);
             constexpr uint32_t idesc_o = make_idesc_bf16(kBlk, D, 0, 1);
@@ -201,7 +202,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             uint32_t phase = 0;
             bool ok = true;
             auto next = [&]() {
-                umma_commit(&empty_bar[stage]);
+                umma_commit_by(lead, &empty_bar[stage]);
                 if (++stage == C::kStages) {
                     stage = 0;
                     phase ^= 1u;
@@ -212,24 +213,24 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (u >= args.units) continue;
                 const int nt = unit_geom(args.blocks, args.Hq, u).i + 1;
                 const int qs = lt % C::kQStages, ob = lt % C::kORing;
-                if (!mbar_wait(&q_full[qs], (uint32_t)((lt / C::kQStages) & 1), abort_flag)) break;
+                if (!warp_wait(&q_full[qs], (uint32_t)((lt / C::kQStages) & 1), abort_flag)) break;
                 tc_fence_after();
                 const uint32_t q_addr = smem_u32(smem + qs * C::kQBytes), o_tmem = tmem + 256u + (uint32_t)(ob * 128);
                 // S into buffer g & 1, whose last P the tensor core has taken: P V of two tiles back is before it in
                 // the issue order
                 auto issue_s = [&](bool last) {
                     for (int kb = 0; kb < ND; ++kb) {
-                        if (!(ok = ok && mbar_wait(&full_bar[stage], phase, abort_flag))) return;
+                        if (!(ok = ok && warp_wait(&full_bar[stage], phase, abort_flag))) return;
                         tc_fence_after();
                         const uint32_t sa = q_addr + kb * kChunk, sb = smem_u32(ring + stage * kChunk);
 #pragma unroll
                         for (int kk = 0; kk < 4; ++kk)
-                            umma_f16(tmem + (uint32_t)((g & 1) * kBlk), make_sdesc_sw128(sa + kk * 32, 16, 1024),
+                            umma_f16_by(lead, tmem + (uint32_t)((g & 1) * kBlk), make_sdesc_sw128(sa + kk * 32, 16, 1024),
                                      make_sdesc_sw128(sb + kk * 32, 16, 1024), idesc_s, (kb > 0 || kk > 0) ? 1u : 0u);
                         next();
                     }
-                    umma_commit(&s_full[g & 1]);
-                    if (last) umma_commit(&q_empty[qs]);
+                    umma_commit_by(lead, &s_full[g & 1]);
+                    if (last) umma_commit_by(lead, &q_empty[qs]);
                     ++g;
                 };
                 const int g0 = g;
@@ -238,27 +239,27 @@ __global__ void __launch_bounds__(kThreads, 1)
                     if (j + 1 < nt) issue_s(j + 2 == nt);
                     if (!ok) break;
                     const int gj = g0 + j, b = gj & 1;
-                    if (!(ok = mbar_wait(&p_full[b], (uint32_t)((gj >> 1) & 1), abort_flag))) break;
+                    if (!(ok = warp_wait(&p_full[b], (uint32_t)((gj >> 1) & 1), abort_flag))) break;
                     if (j == 0 &&
-                        !(ok = mbar_wait(&o_empty[ob], (uint32_t)((lt / C::kORing) & 1) ^ 1u, abort_flag)))
+                        !(ok = warp_wait(&o_empty[ob], (uint32_t)((lt / C::kORing) & 1) ^ 1u, abort_flag)))
                         break;
                     tc_fence_after();
                     for (int ch = 0; ch < kVC; ++ch) {
-                        if (!(ok = mbar_wait(&full_bar[stage], phase, abort_flag))) break;
+                        if (!(ok = warp_wait(&full_bar[stage], phase, abort_flag))) break;
                         tc_fence_after();
                         const uint32_t sv = smem_u32(ring + stage * kChunk);
 #pragma unroll
                         for (int kk = 0; kk < C::kVRows / 16; ++kk)
-                            umma_f16_ts(o_tmem, tmem + (uint32_t)(b * kBlk + (ch * C::kVRows + kk * 16) / 2),
+                            umma_f16_ts_by(lead, o_tmem, tmem + (uint32_t)(b * kBlk + (ch * C::kVRows + kk * 16) / 2),
                                         make_sdesc_sw128(sv + kk * 2048, C::kVRows * 128, 1024), idesc_o,
                                         (j > 0 || ch > 0 || kk > 0) ? 1u : 0u);
                         next();
                     }
                     if (!ok) break;
-                    umma_commit(&pv_done[b]);
+                    umma_commit_by(lead, &pv_done[b]);
                 }
                 if (!ok) break;
-                umma_commit(&o_full[ob]);
+                umma_commit_by(lead, &o_full[ob]);
                 ++lt;
             }
         }
@@ -630,7 +631,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
                 ++lt;
             }
-        } else if (warp == 1 && lane == 0) {
+        } else if (warp == 1) {
+            const uint32_t lead = elect_one();
             // --------------------------------------------------------- MMA issuer
             constexpr uint32_t idesc_s = make_idesc_bf16(kBlk, kBlk, 0, 0);
             constexpr uint32_t idesc_c = make_idesc_bf16(kBlk, D, 0, 1);
@@ -638,12 +640,12 @@ __global__ void __launch_bounds__(kThreads, 1)
             uint32_t phase = 0;
             bool ok = true;
             auto chunk = [&]() -> uint32_t {  // the next ring chunk's address, or 0 when a wait gave up
-                if (!(ok = ok && mbar_wait(&full_bar[stage], phase, abort_flag))) return 0u;
+                if (!(ok = ok && warp_wait(&full_bar[stage], phase, abort_flag))) return 0u;
                 tc_fence_after();
                 return smem_u32(ring + stage * kChunk);
             };
             auto next = [&]() {
-                umma_commit(&empty_bar[stage]);
+                umma_commit_by(lead, &empty_bar[stage]);
                 if (++stage == C::kStages) {
                     stage = 0;
                     phase ^= 1u;
@@ -656,7 +658,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     if (!sb) return;
 #pragma unroll
                     for (int kk = 0; kk < 4; ++kk)
-                        umma_f16(d, make_sdesc_sw128(sa + kb * kChunk + kk * 32, 16, 1024),
+                        umma_f16_by(lead, d, make_sdesc_sw128(sa + kb * kChunk + kk * 32, 16, 1024),
                                  make_sdesc_sw128(sb + kk * 32, 16, 1024), idesc_s, (kb > 0 || kk > 0) ? 1u : 0u);
                     next();
                 }
@@ -668,7 +670,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
                     for (int kk = 0; kk < C::kVRows / 16; ++kk) {
                         const int k16 = ch * (C::kVRows / 16) + kk;  // the halves' bf16 columns start 64 apart
-                        umma_f16_ts(d, a + (uint32_t)((k16 >> 2) * 64 + (k16 & 3) * 8),
+                        umma_f16_ts_by(lead, d, a + (uint32_t)((k16 >> 2) * 64 + (k16 & 3) * 8),
                                     make_sdesc_sw128(sb + kk * 2048, C::kVRows * 128, 1024), idesc_c,
                                     (!first || ch > 0 || kk > 0) ? 1u : 0u);
                     }
@@ -676,7 +678,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
             };
             auto wait = [&](uint64_t* bar, int n) {  // the bar's n-th completion
-                ok = ok && mbar_wait(bar, (uint32_t)(n & 1), abort_flag);
+                ok = ok && warp_wait(bar, (uint32_t)(n & 1), abort_flag);
                 tc_fence_after();
             };
             for (int t = 0; ok && t * G < args.units; ++t) {
@@ -690,15 +692,15 @@ __global__ void __launch_bounds__(kThreads, 1)
                     if (j == 0) wait(&a_full[0], lt);
                     if (!ok) return;
                     score(0, tmem + (uint32_t)(b * kBlk));
-                    umma_commit(&s_full[b]);
-                    if (j + 1 == n) umma_commit(&a_empty[0]);
+                    umma_commit_by(lead, &s_full[b]);
+                    if (j + 1 == n) umma_commit_by(lead, &a_empty[0]);
                 };
                 auto issue_dp = [&](int j) {
                     if (j == 0) wait(&a_full[1], lt);
                     if (!ok) return;
                     score(1, tmem + (uint32_t)kBlk);
-                    umma_commit(dp_full);
-                    if (j + 1 == n) umma_commit(&a_empty[1]);
+                    umma_commit_by(lead, dp_full);
+                    if (j + 1 == n) umma_commit_by(lead, &a_empty[1]);
                 };
                 issue_s(0);
                 if (C::kDP) issue_dp(0);
@@ -729,7 +731,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     }
                 }
                 if (!ok) break;
-                umma_commit(acc_full);
+                umma_commit_by(lead, acc_full);
                 g += n;
                 ++lt;
             }
