@@ -28,16 +28,34 @@ namespace {
 
 constexpr int kBlk = 128;           // queries of a unit, keys of a tile
 constexpr int kChunk = 16384;       // one ring stage
-constexpr int kThreads = 384;       // warp 0: TMA, warp 1: MMA, warps 4-7 and 8-11: two softmax warpgroups
+constexpr int kChunkLo = kChunk >> 4;               // and its step in a matrix descriptor
+constexpr uint32_t kDescHi = sdesc_hi_sw128(1024);  // 8 rows of 128 bytes a swizzle atom
+constexpr int kThreads = 384;       // warps 0, 3: TMA, warp 1: MMA, warp 2: row statistics; warps 4-7, 8-11: softmax
 constexpr int kCtrlRegs = 104, kSoftRegs = 200;  // 128 x 104 + 256 x 200 = 384 x 168, what the launch holds
 static_assert(128 * kCtrlRegs + 256 * kSoftRegs <= 384 * 168, "register split");
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
+constexpr long long kWaitCycles = 4000000000ll;  // a wait's limit, about two seconds
 constexpr float kLazy = 8.0f;       // log2 units a row's maximum may outgrow the reference before O is rescaled
 
-// mbar_wait by every lane of a warp with one outcome for all: the warp stays together when a wait gives up.
+// mbar_wait by every lane of a warp with one outcome for all: the warp stays converged, in the wait and when it gives up
+// (a satisfied wait through divergent control flow costs 60 cycles more, a quarter of what a 16 KB chunk's products take).
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort) {
-    return __all_sync(0xFFFFFFFFu, mbar_wait(bar, parity, abort));
+    uint32_t n = 0;
+    long long t0 = 0;
+    while (!__all_sync(0xFFFFFFFFu, mbar_try_wait(bar, parity))) {
+        if ((++n & 255u) == 0) {
+            const long long now = clock64();
+            if (n == 256) t0 = now;
+            const bool late = now - t0 > kWaitCycles;
+            if (late) {
+                atomicOr(&g_device_error, kErrTimeout);
+                *abort = 1;
+            }
+            if (__any_sync(0xFFFFFFFFu, late || *abort != 0)) return false;
+        }
+    }
+    return true;
 }
 
 template <int D>
@@ -110,7 +128,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     float* ref_m = reinterpret_cast<float*>(smem + C::kMaxOff);
     float2* fin = reinterpret_cast<float2*>(smem + C::kFinOff);
 
-    const int warp = threadIdx.x >> 5;
+    const int warp = __shfl_sync(0xFFFFFFFFu, threadIdx.x >> 5, 0);
     const int lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
         for (int s = 0; s < C::kStages; ++s) {
@@ -118,7 +136,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             mbar_init(&empty_bar[s], 1);
         }
         for (int b = 0; b < 2; ++b) {
-            mbar_init(&q_full[b], 1);
+            mbar_init(&q_full[b], 2);
             mbar_init(&q_empty[b], 1);
             mbar_init(&s_full[b], 1);
             mbar_init(&p_full[b], 4);
@@ -145,14 +163,16 @@ __global__ void __launch_bounds__(kThreads, 1)
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = *tmem_slot;
+    const uint32_t tmem = __shfl_sync(0xFFFFFFFFu, *tmem_slot, 0);
     const int G = gridDim.x, c = blockIdx.x;
 
     if (warp < 4) {
         set_max_regs_dec<kCtrlRegs>();
-        if (warp == 0 && lane == 0) {
-            // --------------------------------------------------------- TMA producer
-            int stage = 0, lt = 0;
+        if (warp == 0 || warp == 3) {
+            // --------------------------------------------------------- TMA producers: every other chunk each
+            const uint32_t lead = elect_one();
+            const int p = warp == 3;
+            int stage = p, lt = 0;
             uint32_t phase = 0;
             bool ok = true;
             for (int t = 0; ok && t * G < args.units; ++t) {
@@ -162,34 +182,41 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const int shift = kBlk - un.n, kvh = un.h / args.grp;
                 const int seq0 = un.tok0 - un.i * kBlk;
                 const int qs = lt % C::kQStages;
-                if (!mbar_wait(&q_empty[qs], (uint32_t)((lt / C::kQStages) & 1) ^ 1u, abort_flag)) break;
-                mbar_expect_tx(&q_full[qs], C::kQBytes);
-                for (int s = 0; s < ND; ++s)
-                    tma_load_3d(smem + qs * C::kQBytes + s * kChunk, &tQ, &q_full[qs], un.h * args.q_head + 64 * s, -shift,
-                                un.tok0);
-                auto load = [&](const CUtensorMap* map, bool v, int j) {
+                if (!warp_wait(&q_empty[qs], (uint32_t)((lt / C::kQStages) & 1) ^ 1u, abort_flag)) break;
+                if (lead) {
+                    mbar_expect_tx(&q_full[qs], C::kQBytes / 2);
+                    for (int s = p; s < ND; s += 2)
+                        tma_load_3d(smem + qs * C::kQBytes + s * kChunk, &tQ, &q_full[qs], un.h * args.q_head + 64 * s, -shift,
+                                    un.tok0);
+                }
+                auto load = [&](bool v, int j) {
                     const int tok = seq0 + j * kBlk, r0 = j == un.i ? -shift : 0;
-                    for (int ch = 0; ch < (v ? kVC : ND); ++ch) {
-                        if (!(ok = ok && mbar_wait(&empty_bar[stage], phase ^ 1u, abort_flag))) return;
-                        uint8_t* st = ring + stage * kChunk;
-                        mbar_expect_tx(&full_bar[stage], kChunk);
-                        if (v) {
-                            for (int n = 0; n < ND; ++n)
-                                tma_load_3d(st + n * (C::kVRows * 128), map, &full_bar[stage],
-                                            kvh * args.v_head + 64 * n, r0 + ch * C::kVRows, tok);
-                        } else {
-                            tma_load_3d(st, map, &full_bar[stage], kvh * args.k_head + 64 * ch, r0, tok);
+                    const int x = kvh * (v ? args.v_head : args.k_head);
+#pragma unroll
+                    for (int ch = p; ch < (v ? kVC : ND); ch += 2) {
+                        if (!(ok = ok && warp_wait(&empty_bar[stage], phase ^ 1u, abort_flag))) return;
+                        if (lead) {
+                            uint8_t* st = ring + stage * kChunk;
+                            mbar_expect_tx(&full_bar[stage], kChunk);
+                            if (v) {
+#pragma unroll
+                                for (int n = 0; n < ND; ++n)
+                                    tma_load_3d(st + n * (C::kVRows * 128), &tV, &full_bar[stage], x + 64 * n,
+                                                r0 + ch * C::kVRows, tok);
+                            } else {
+                                tma_load_3d(st, &tK, &full_bar[stage], x + 64 * ch, r0, tok);
+                            }
                         }
-                        if (++stage == C::kStages) {
-                            stage = 0;
+                        if ((stage += 2) >= C::kStages) {
+                            stage -= C::kStages;
                             phase ^= 1u;
                         }
                     }
                 };
-                load(&tK, false, 0);
+                load(false, 0);
                 for (int j = 0; j <= un.i && ok; ++j) {
-                    if (j < un.i) load(&tK, false, j + 1);
-                    load(&tV, true, j);
+                    if (j < un.i) load(false, j + 1);
+                    load(true, j);
                 }
                 ++lt;
             }
@@ -198,6 +225,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             // --------------------------------------------------------- MMA issuer
             constexpr uint32_t idesc_s = make_idesc_bf16(kBlk, kBlk, 0, 0);
             constexpr uint32_t idesc_o = make_idesc_bf16(kBlk, D, 0, 1);
+            const uint32_t k_lo = sdesc_lo(smem_u32(ring), 16), v_lo = sdesc_lo(smem_u32(ring), C::kVRows * 128);
             int stage = 0, lt = 0, g = 0;  // g: tiles whose S has been issued
             uint32_t phase = 0;
             bool ok = true;
@@ -215,18 +243,19 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const int qs = lt % C::kQStages, ob = lt % C::kORing;
                 if (!warp_wait(&q_full[qs], (uint32_t)((lt / C::kQStages) & 1), abort_flag)) break;
                 tc_fence_after();
-                const uint32_t q_addr = smem_u32(smem + qs * C::kQBytes), o_tmem = tmem + 256u + (uint32_t)(ob * 128);
+                const uint32_t q_lo = sdesc_lo(smem_u32(smem), 16) + (uint32_t)(qs * (C::kQBytes >> 4));
+                const uint32_t o_tmem = tmem + 256u + (uint32_t)(ob * 128);
                 // S into buffer g & 1, whose last P the tensor core has taken: P V of two tiles back is before it in
                 // the issue order
                 auto issue_s = [&](bool last) {
                     for (int kb = 0; kb < ND; ++kb) {
                         if (!(ok = ok && warp_wait(&full_bar[stage], phase, abort_flag))) return;
                         tc_fence_after();
-                        const uint32_t sa = q_addr + kb * kChunk, sb = smem_u32(ring + stage * kChunk);
+                        const uint32_t a = q_lo + (uint32_t)(kb * kChunkLo), b = k_lo + (uint32_t)(stage * kChunkLo);
 #pragma unroll
                         for (int kk = 0; kk < 4; ++kk)
-                            umma_f16_by(lead, tmem + (uint32_t)((g & 1) * kBlk), make_sdesc_sw128(sa + kk * 32, 16, 1024),
-                                     make_sdesc_sw128(sb + kk * 32, 16, 1024), idesc_s, (kb > 0 || kk > 0) ? 1u : 0u);
+                            umma_f16_by(lead, tmem + (uint32_t)((g & 1) * kBlk), sdesc(a + kk * 2, kDescHi),
+                                        sdesc(b + kk * 2, kDescHi), idesc_s, (kb > 0 || kk > 0) ? 1u : 0u);
                         next();
                     }
                     umma_commit_by(lead, &s_full[g & 1]);
@@ -247,12 +276,12 @@ __global__ void __launch_bounds__(kThreads, 1)
                     for (int ch = 0; ch < kVC; ++ch) {
                         if (!(ok = warp_wait(&full_bar[stage], phase, abort_flag))) break;
                         tc_fence_after();
-                        const uint32_t sv = smem_u32(ring + stage * kChunk);
+                        const uint32_t v = v_lo + (uint32_t)(stage * kChunkLo);
 #pragma unroll
                         for (int kk = 0; kk < C::kVRows / 16; ++kk)
                             umma_f16_ts_by(lead, o_tmem, tmem + (uint32_t)(b * kBlk + (ch * C::kVRows + kk * 16) / 2),
-                                        make_sdesc_sw128(sv + kk * 2048, C::kVRows * 128, 1024), idesc_o,
-                                        (j > 0 || ch > 0 || kk > 0) ? 1u : 0u);
+                                           sdesc(v + kk * 128, kDescHi), idesc_o,
+                                           (j > 0 || ch > 0 || kk > 0) ? 1u : 0u);
                         next();
                     }
                     if (!ok) break;
@@ -519,7 +548,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
     float* stats = reinterpret_cast<float*>(smem + C::kStatOff);
 
-    const int warp = threadIdx.x >> 5;
+    const int warp = __shfl_sync(0xFFFFFFFFu, threadIdx.x >> 5, 0);
     const int lane = threadIdx.x & 31;
     if (smem_u32(smem) & 1023u) {  // the swizzled tiles need it; the attribute above asks for it
         if (threadIdx.x == 0) atomicOr(&g_device_error, kErrArgs);
@@ -563,71 +592,68 @@ __global__ void __launch_bounds__(kThreads, 1)
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = *tmem_slot;
+    const uint32_t tmem = __shfl_sync(0xFFFFFFFFu, *tmem_slot, 0);
     const uint32_t acc0 = tmem + 256u, acc1 = tmem + 384u;  // acc1: kDKV's dK
     const int G = gridDim.x, c = blockIdx.x;
 
     if (warp < 4) {
         set_max_regs_dec<kCtrlRegs>();
-        if (warp == 0 && lane == 0) {
-            // --------------------------------------------------------- TMA producer
-            int stage = 0, lt = 0;
+        if (warp == 0 || warp == 3) {
+            // --------------------------------------------------------- TMA producers: every other chunk each
+            const uint32_t lead = elect_one();
+            const int p = warp == 3;
+            int stage = p, lt = 0;
             uint32_t phase = 0;
             bool ok = true;
-            auto slot = [&]() -> uint8_t* {
-                if (!(ok = ok && mbar_wait(&empty_bar[stage], phase ^ 1u, abort_flag))) return nullptr;
-                mbar_expect_tx(&full_bar[stage], kChunk);
-                return ring + stage * kChunk;
-            };
-            auto next = [&]() {
-                if (++stage == C::kStages) {
-                    stage = 0;
-                    phase ^= 1u;
-                }
-            };
             for (int t = 0; ok && t * G < args.units; ++t) {
                 const int u = unit_of(t, c, G);
                 if (u >= args.units) continue;
                 const Walk<KIND> wk(args, u);
-                for (int r = 0; r < (C::kDP ? 2 : 1); ++r) {
-                    if (!(ok = ok && mbar_wait(&a_empty[r], (uint32_t)(lt & 1) ^ 1u, abort_flag))) break;
-                    mbar_expect_tx(&a_full[r], C::kABytes);
-                    for (int s = 0; s < ND; ++s)
-                        tma_load_3d(smem + r * C::kABytes + s * kChunk, r ? &tA1 : &tA0, &a_full[r],
-                                    wk.h * (r ? args.a1_head : args.a0_head) + 64 * s, -wk.shift(), wk.tok0);
+                if (p == 0 || C::kDP) {  // a resident operand each
+                    if (!(ok = warp_wait(&a_empty[p], (uint32_t)(lt & 1) ^ 1u, abort_flag))) break;
+                    if (lead) {
+                        mbar_expect_tx(&a_full[p], C::kABytes);
+                        for (int s = 0; s < ND; ++s)
+                            tma_load_3d(smem + p * C::kABytes + s * kChunk, p ? &tA1 : &tA0, &a_full[p],
+                                        wk.h * (p ? args.a1_head : args.a0_head) + 64 * s, -wk.shift(), wk.tok0);
+                    }
                 }
                 // a column block K-major (the score products), or MN-major (the accumulating ones)
-                auto load_b = [&](const CUtensorMap* map, int head_stride, int tile) {
+                auto load = [&](const CUtensorMap* map, bool mn, int head_stride, int tile) {
                     const int blk = wk.block(tile), x = wk.head(tile) * head_stride;
-                    for (int ch = 0; ch < ND; ++ch) {
-                        uint8_t* st = slot();
-                        if (!st) return;
-                        tma_load_3d(st, map, &full_bar[stage], x + 64 * ch, -wk.shift_of(blk), wk.seq0 + blk * kBlk);
-                        next();
+                    const int r0 = -wk.shift_of(blk), tok = wk.seq0 + blk * kBlk;
+#pragma unroll
+                    for (int ch = p; ch < (mn ? kVC : ND); ch += 2) {
+                        if (!(ok = ok && warp_wait(&empty_bar[stage], phase ^ 1u, abort_flag))) return;
+                        if (lead) {
+                            uint8_t* st = ring + stage * kChunk;
+                            mbar_expect_tx(&full_bar[stage], kChunk);
+                            if (mn) {
+#pragma unroll
+                                for (int n = 0; n < ND; ++n)
+                                    tma_load_3d(st + n * (C::kVRows * 128), map, &full_bar[stage], x + 64 * n,
+                                                ch * C::kVRows + r0, tok);
+                            } else {
+                                tma_load_3d(st, map, &full_bar[stage], x + 64 * ch, r0, tok);
+                            }
+                        }
+                        if ((stage += 2) >= C::kStages) {
+                            stage -= C::kStages;
+                            phase ^= 1u;
+                        }
                     }
                 };
-                auto load_c = [&](const CUtensorMap* map, int head_stride, int tile) {
-                    const int blk = wk.block(tile), x = wk.head(tile) * head_stride;
-                    for (int ch = 0; ch < kVC; ++ch) {
-                        uint8_t* st = slot();
-                        if (!st) return;
-                        for (int n = 0; n < ND; ++n)
-                            tma_load_3d(st + n * (C::kVRows * 128), map, &full_bar[stage], x + 64 * n,
-                                        ch * C::kVRows - wk.shift_of(blk), wk.seq0 + blk * kBlk);
-                        next();
-                    }
-                };
-                load_b(&tB0, args.b0_head, 0);
-                if (C::kDP) load_b(&tB1, args.b1_head, 0);
+                load(&tB0, false, args.b0_head, 0);
+                if (C::kDP) load(&tB1, false, args.b1_head, 0);
                 for (int j = 0; j < wk.tiles && ok; ++j) {
                     const bool more = j + 1 < wk.tiles;
-                    if (KIND == kDKV) load_c(&tC0, args.c0_head, j);
-                    if (more) load_b(&tB0, args.b0_head, j + 1);
+                    if (KIND == kDKV) load(&tC0, true, args.c0_head, j);
+                    if (more) load(&tB0, false, args.b0_head, j + 1);
                     if (KIND == kDKV)
-                        load_c(&tC1, args.c1_head, j);
+                        load(&tC1, true, args.c1_head, j);
                     else
-                        load_c(&tC0, args.c0_head, j);
-                    if (more && C::kDP) load_b(&tB1, args.b1_head, j + 1);
+                        load(&tC0, true, args.c0_head, j);
+                    if (more && C::kDP) load(&tB1, false, args.b1_head, j + 1);
                 }
                 ++lt;
             }
@@ -639,10 +665,12 @@ __global__ void __launch_bounds__(kThreads, 1)
             int stage = 0, lt = 0, g = 0;  // g: the current unit's first tile
             uint32_t phase = 0;
             bool ok = true;
-            auto chunk = [&]() -> uint32_t {  // the next ring chunk's address, or 0 when a wait gave up
-                if (!(ok = ok && warp_wait(&full_bar[stage], phase, abort_flag))) return 0u;
+            const uint32_t a_lo = sdesc_lo(smem_u32(smem), 16);
+            const uint32_t b_lo = sdesc_lo(smem_u32(ring), 16), c_lo = sdesc_lo(smem_u32(ring), C::kVRows * 128);
+            auto chunk = [&]() -> bool {  // the next ring chunk is there
+                ok = ok && warp_wait(&full_bar[stage], phase, abort_flag);
                 tc_fence_after();
-                return smem_u32(ring + stage * kChunk);
+                return ok;
             };
             auto next = [&]() {
                 umma_commit_by(lead, &empty_bar[stage]);
@@ -652,27 +680,26 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
             };
             auto score = [&](int resident, uint32_t d) {
-                const uint32_t sa = smem_u32(smem + resident * C::kABytes);
                 for (int kb = 0; kb < ND; ++kb) {
-                    const uint32_t sb = chunk();
-                    if (!sb) return;
+                    if (!chunk()) return;
+                    const uint32_t a = a_lo + (uint32_t)(resident * (C::kABytes >> 4) + kb * kChunkLo);
+                    const uint32_t b = b_lo + (uint32_t)(stage * kChunkLo);
 #pragma unroll
                     for (int kk = 0; kk < 4; ++kk)
-                        umma_f16_by(lead, d, make_sdesc_sw128(sa + kb * kChunk + kk * 32, 16, 1024),
-                                 make_sdesc_sw128(sb + kk * 32, 16, 1024), idesc_s, (kb > 0 || kk > 0) ? 1u : 0u);
+                        umma_f16_by(lead, d, sdesc(a + kk * 2, kDescHi), sdesc(b + kk * 2, kDescHi), idesc_s,
+                                    (kb > 0 || kk > 0) ? 1u : 0u);
                     next();
                 }
             };
             auto accumulate = [&](uint32_t a, uint32_t d, bool first) {
                 for (int ch = 0; ch < kVC; ++ch) {
-                    const uint32_t sb = chunk();
-                    if (!sb) return;
+                    if (!chunk()) return;
+                    const uint32_t b = c_lo + (uint32_t)(stage * kChunkLo);
 #pragma unroll
                     for (int kk = 0; kk < C::kVRows / 16; ++kk) {
                         const int k16 = ch * (C::kVRows / 16) + kk;  // the halves' bf16 columns start 64 apart
                         umma_f16_ts_by(lead, d, a + (uint32_t)((k16 >> 2) * 64 + (k16 & 3) * 8),
-                                    make_sdesc_sw128(sb + kk * 2048, C::kVRows * 128, 1024), idesc_c,
-                                    (!first || ch > 0 || kk > 0) ? 1u : 0u);
+                                       sdesc(b + kk * 128, kDescHi), idesc_c, (!first || ch > 0 || kk > 0) ? 1u : 0u);
                     }
                     next();
                 }

@@ -322,6 +322,14 @@ __device__ __forceinline__ uint64_t make_sdesc_sw128(uint32_t saddr, uint32_t lb
     return d;
 }
 
+// The same descriptor as two words, for issue loops that step through tiles: the low one (address and leading offset)
+// takes an added byte offset >> 4 as long as the address stays inside shared memory, the high one is a constant.
+__device__ __forceinline__ uint32_t sdesc_lo(uint32_t saddr, uint32_t lbo_bytes) {
+    return (saddr >> 4) | ((lbo_bytes >> 4) << 16);
+}
+constexpr uint32_t sdesc_hi_sw128(uint32_t sbo_bytes) { return (sbo_bytes >> 4) | (1u << 14) | (2u << 29); }
+__device__ __forceinline__ uint64_t sdesc(uint32_t lo, uint32_t hi) { return ((uint64_t)hi << 32) | lo; }
+
 // Instruction descriptor for kind::f16 with bf16 A/B and an f32 accumulator, M x N, and the
 // operand majorness (0 = K-major, 1 = MN-major).
 __host__ __device__ constexpr uint32_t make_idesc_bf16(int M, int N, int a_mn, int b_mn) {
