@@ -30,9 +30,10 @@ constexpr int kBlk = 128;           // queries of a unit, keys of a tile
 constexpr int kChunk = 16384;       // one ring stage
 constexpr int kChunkLo = kChunk >> 4;               // and its step in a matrix descriptor
 constexpr uint32_t kDescHi = sdesc_hi_sw128(1024);  // 8 rows of 128 bytes a swizzle atom
-constexpr int kThreads = 384;       // warps 0, 3: TMA, warp 1: MMA, warp 2: row statistics; warps 4-7, 8-11: softmax
-constexpr int kCtrlRegs = 104, kSoftRegs = 200;  // 128 x 104 + 256 x 200 = 384 x 168, what the launch holds
-static_assert(128 * kCtrlRegs + 256 * kSoftRegs <= 384 * 168, "register split");
+constexpr int kThreads = 640;       // warps 0, 3: TMA, warp 1: MMA, warp 2: statistics; four softmax warpgroups after
+constexpr int kSoftWarps = 16;
+constexpr int kCtrlRegs = 64, kSoftRegs = 104;  // 128 x 64 + 512 x 104 = 640 x 96, what the launch holds
+static_assert(128 * kCtrlRegs + 512 * kSoftRegs <= 640 * 96, "register split");
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr long long kWaitCycles = 4000000000ll;  // a wait's limit, about two seconds
@@ -58,6 +59,39 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volati
     return true;
 }
 
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 d;
+    asm("{\n .reg .b64 x, y, z;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n mov.b64 z, {%6, %7};\n"
+        " fma.rn.f32x2 x, x, y, z;\n mov.b64 {%0, %1}, x;\n}\n"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 d;
+    asm("{\n .reg .b64 x, y;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n add.rn.f32x2 x, x, y;\n mov.b64 {%0, %1}, x;\n}\n"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    float2 d;
+    asm("{\n .reg .b64 x, y;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n mul.rn.f32x2 x, x, y;\n mov.b64 {%0, %1}, x;\n}\n"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+    const __nv_bfloat162 b = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&b);
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+    return d;
+}
+
 template <int D>
 struct FCfg {
     static constexpr int kQBytes = kBlk * D * 2;
@@ -66,9 +100,10 @@ struct FCfg {
     static constexpr int kStages = 9;
     static constexpr int kRingOff = kQStages * kQBytes;
     static constexpr int kBarOff = kRingOff + kStages * kChunk;
-    static constexpr int kMaxOff = kBarOff + 512;        // float [2][128]: the reference each warpgroup used last
-    static constexpr int kFinOff = kMaxOff + 1024;       // float2 [2 (unit parity)][2][128]: (reference, sum)
-    static constexpr int kSmemBytes = kFinOff + 4096 + 1024;
+    static constexpr int kMaxOff = kBarOff + 640;        // float [2][128]: the reference each tile parity used last
+    static constexpr int kPartOff = kMaxOff + 1024;      // float [2][2][128]: a tile's maxima by column half
+    static constexpr int kFinOff = kPartOff + 2048;      // float2 [2 (unit parity)][4][128]: (reference, sum)
+    static constexpr int kSmemBytes = kFinOff + 8192 + 1024;
     static constexpr int kVRows = kChunk / (D * 2);      // keys of one V chunk
 };
 
@@ -87,6 +122,23 @@ struct Unit {
     int h, tok0, i, n;  // head, the block's first token, its index in the sequence, its tokens
 };
 
+// 32 accumulator values of a thread's row, times f, as 64 bytes of bf16.
+__device__ __forceinline__ void store_row32(__nv_bfloat16* p, const uint32_t (&r)[32], float f) {
+#pragma unroll
+    for (int v = 0; v < 4; ++v) {
+        uint32_t pk[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            pk[k] = pack_bf16(__uint_as_float(r[v * 8 + k * 2]) * f, __uint_as_float(r[v * 8 + k * 2 + 1]) * f);
+        *reinterpret_cast<uint4*>(p + v * 8) = make_uint4(pk[0], pk[1], pk[2], pk[3]);
+    }
+}
+
+// The TMEM column of 16 consecutive k (k16-th) of a bf16 A operand whose writers own 64 (or 32) f32 columns each and
+// leave their values packed at the start of their own columns.
+__device__ __forceinline__ constexpr int half_col(int k16) { return (k16 >> 2) * 64 + (k16 & 3) * 8; }
+__device__ __forceinline__ constexpr int quarter_col(int k16) { return (k16 >> 1) * 32 + (k16 & 1) * 8; }
+
 // A CTA's t-th unit: a snake over the longest-first order, so a heavy unit of one round meets a light one in the next.
 __device__ __forceinline__ int unit_of(int t, int c, int G) { return t * G + ((t & 1) ? (G - 1 - c) : c); }
 
@@ -97,11 +149,11 @@ __device__ __forceinline__ Unit unit_geom(const int4* blocks, int heads, int u) 
 }
 
 // One pass over the keys. A unit is one 128-query block of one head; key tile j of it: S_j = Q K_j^T into one of two
-// TMEM buffers, P_j = 2^(S_j c - m) as bf16 over the same buffer's columns, O += P_j V_j in TMEM. The two softmax
-// warpgroups take the tiles in turn (a thread a row), so the exponentials of one tile run beside the row maximum of the
-// next and both beside the products: S_{j+1} is issued before P_j V_j. The reference m a row's exponentials use is
-// handed from tile to tile; it is moved (and O rescaled, by the threads that own the rows) only when the row's maximum
-// has outgrown it by 2^8, which f32 sums and bf16 probabilities carry without loss.
+// TMEM buffers, P_j = 2^(S_j c - m) as bf16 over the same buffer's columns, O += P_j V_j in TMEM. The four softmax
+// warpgroups are two pairs that take the tiles in turn, a thread a row and half of the columns, so the exponentials of
+// one tile run beside the row maximum of the next and both beside the products: S_{j+1} is issued before P_j V_j. The
+// reference m a row's exponentials use is handed from tile to tile; it is moved (and O rescaled, by the threads that own
+// the rows) only when the row's maximum has outgrown it by 2^8, which f32 sums and bf16 probabilities carry without loss.
 template <int D>
 __global__ void __launch_bounds__(kThreads, 1)
     fwd_kernel(const __grid_constant__ CUtensorMap tQ, const __grid_constant__ CUtensorMap tK,
@@ -121,11 +173,13 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint64_t* o_full = p_full + 2;              // [2]
     uint64_t* o_empty = o_full + 2;             // [2]
     uint64_t* pv_done = o_empty + 2;            // [2]
-    uint64_t* max_bar = pv_done + 2;            // [2][4]: warpgroup w's warp of lane quarter q published its reference
-    uint64_t* fin_bar = max_bar + 8;            // [2][4]: both warps of a lane quarter published a unit's sums
+    uint64_t* part_bar = pv_done + 2;           // [2][4]: both halves' maxima of a tile's lane quarter written
+    uint64_t* max_bar = part_bar + 8;           // [2][4]: its reference written, and the one before it read
+    uint64_t* fin_bar = max_bar + 8;            // [2][4]: the four warps of a lane quarter wrote a unit's sums
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(fin_bar + 8);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
     float* ref_m = reinterpret_cast<float*>(smem + C::kMaxOff);
+    float* part = reinterpret_cast<float*>(smem + C::kPartOff);
     float2* fin = reinterpret_cast<float2*>(smem + C::kFinOff);
 
     const int warp = __shfl_sync(0xFFFFFFFFu, threadIdx.x >> 5, 0);
@@ -139,14 +193,15 @@ __global__ void __launch_bounds__(kThreads, 1)
             mbar_init(&q_full[b], 2);
             mbar_init(&q_empty[b], 1);
             mbar_init(&s_full[b], 1);
-            mbar_init(&p_full[b], 4);
+            mbar_init(&p_full[b], kSoftWarps / 2);
             mbar_init(&o_full[b], 1);
-            mbar_init(&o_empty[b], 8);
+            mbar_init(&o_empty[b], kSoftWarps);
             mbar_init(&pv_done[b], 1);
         }
         for (int b = 0; b < 8; ++b) {
-            mbar_init(&max_bar[b], 1);
-            mbar_init(&fin_bar[b], 2);
+            mbar_init(&part_bar[b], 2);
+            mbar_init(&max_bar[b], 2);
+            mbar_init(&fin_bar[b], 4);
         }
         *abort_flag = 0;
         fence_mbar_init();
@@ -279,7 +334,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                         const uint32_t v = v_lo + (uint32_t)(stage * kChunkLo);
 #pragma unroll
                         for (int kk = 0; kk < C::kVRows / 16; ++kk)
-                            umma_f16_ts_by(lead, o_tmem, tmem + (uint32_t)(b * kBlk + (ch * C::kVRows + kk * 16) / 2),
+                            umma_f16_ts_by(lead, o_tmem, tmem + (uint32_t)(b * kBlk + half_col(ch * (C::kVRows / 16) + kk)),
                                            sdesc(v + kk * 128, kDescHi), idesc_o,
                                            (j > 0 || ch > 0 || kk > 0) ? 1u : 0u);
                         next();
@@ -295,10 +350,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     } else {
         // ------------------------------------------------------------- softmax
         set_max_regs_inc<kSoftRegs>();
-        const int q = warp & 3, w = (warp - 4) >> 2;
+        const int q = warp & 3, wg = (warp - 4) >> 2, w = wg >> 1, hf = wg & 1;  // tile parity, column half
         const int row = q * 32 + lane;
         const uint32_t lane_off = (uint32_t)(q * 32) << 16;
-        const uint32_t s_tmem = tmem + lane_off + (uint32_t)(w * kBlk);
+        const uint32_t s_tmem = tmem + lane_off + (uint32_t)(w * kBlk + hf * 64);
         int g0 = 0, lt = 0;
         bool ok = true;
         for (int t = 0; ok && t * G < args.units; ++t) {
@@ -307,115 +362,104 @@ __global__ void __launch_bounds__(kThreads, 1)
             const Unit un = unit_geom(args.blocks, args.Hq, u);
             const int shift = kBlk - un.n, nt = un.i + 1, ob = lt % C::kORing;
             const uint32_t o_tmem = tmem + lane_off + 256u + (uint32_t)(ob * 128);
-            float m = 0.0f, l = 0.0f;  // the reference of this warpgroup's last tile, its tiles' sum relative to it
+            float m = 0.0f, l = 0.0f;  // the reference of this warpgroup's last tile, its columns' sum relative to it
             for (int j = (g0 + w) & 1; j < nt; j += 2) {
                 const int g = g0 + j;
                 if (!(ok = warp_wait(&s_full[w], (uint32_t)((g >> 1) & 1), abort_flag))) break;
                 tc_fence_after();
-                float x[128];
-                __syncwarp();
+                float x[64];
 #pragma unroll
-                for (int cc = 0; cc < 4; ++cc)
+                for (int cc = 0; cc < 2; ++cc)
                     tmem_ld32(s_tmem + (uint32_t)(cc * 32), *reinterpret_cast<uint32_t(*)[32]>(&x[cc * 32]));
                 tmem_ld_wait();
                 if (args.sign != 1.0f) {
 #pragma unroll
-                    for (int e = 0; e < 128; ++e) x[e] *= args.sign;
+                    for (int e = 0; e < 64; ++e) x[e] *= args.sign;
                 }
                 if (j == un.i) {
 #pragma unroll
-                    for (int e = 0; e < 128; ++e)
-                        if (e > row || e < shift) x[e] = -INFINITY;
+                    for (int e = 0; e < 64; ++e)
+                        if (hf * 64 + e > row || hf * 64 + e < shift) x[e] = -INFINITY;
                 }
+                // a NaN score makes the maximum NaN, and with it the row
                 float mx[4] = {x[0], x[1], x[2], x[3]};
 #pragma unroll
-                for (int e = 4; e < 128; ++e) mx[e & 3] = fmaxf(mx[e & 3], x[e]);
-                const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * args.sl2;
+                for (int e = 4; e < 64; ++e) mx[e & 3] = max_nan(mx[e & 3], x[e]);
+                float top = max_nan(max_nan(mx[0], mx[1]), max_nan(mx[2], mx[3])) * args.sl2;
+                part[(w * 2 + hf) * 128 + row] = top;
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&part_bar[w * 4 + q]);
+                if (!(ok = warp_wait(&part_bar[w * 4 + q], (uint32_t)((g >> 1) & 1), abort_flag))) break;
+                top = max_nan(top, part[(w * 2 + (hf ^ 1)) * 128 + row]);
                 float mn;
                 if (j == 0) {
-                    mn = top > -INFINITY ? top : 0.0f;  // a row of nothing visible (or of -inf scores) sums to 0
+                    mn = top == -INFINITY ? 0.0f : top;  // a row of nothing visible (or of -inf scores) sums to 0
                 } else {
                     if (!(ok = warp_wait(&max_bar[(w ^ 1) * 4 + q], (uint32_t)(((g - 1) >> 1) & 1), abort_flag))) break;
                     const float mp = ref_m[(w ^ 1) * 128 + row];
-                    mn = top > mp + kLazy ? top : mp;
+                    mn = top <= mp + kLazy ? mp : top;
                     if (__any_sync(0xFFFFFFFFu, mn != mp)) {
-                        // O still holds sums relative to mp: wait for the last P V, then move it to mn
+                        // O still holds sums relative to mp: wait for the last P V, then move this thread's half to mn
                         if (!(ok = warp_wait(&pv_done[(g - 1) & 1], (uint32_t)(((g - 1) >> 1) & 1), abort_flag))) break;
                         tc_fence_after();
                         const float f = ex2_ftz(mp - mn);
 #pragma unroll 1
                         for (int cc = 0; cc < D / 32; ++cc) {
-                            uint32_t r[32];
-                            tmem_ld32(o_tmem + (uint32_t)(cc * 32), r);
+                            uint32_t r[16];
+                            tmem_ld16(o_tmem + (uint32_t)(hf * (D / 2) + cc * 16), r);
                             tmem_ld_wait();
 #pragma unroll
-                            for (int e = 0; e < 32; ++e) r[e] = __float_as_uint(__uint_as_float(r[e]) * f);
-                            tmem_st32(o_tmem + (uint32_t)(cc * 32), r);
+                            for (int e = 0; e < 16; ++e) r[e] = __float_as_uint(__uint_as_float(r[e]) * f);
+                            tmem_st16(o_tmem + (uint32_t)(hf * (D / 2) + cc * 16), r);
                         }
                     }
                 }
-                ref_m[w * 128 + row] = mn;
+                if (hf == 0) ref_m[w * 128 + row] = mn;
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&max_bar[w * 4 + q]);
                 if (j >= 2) l *= ex2_ftz(m - mn);
                 m = mn;
-                float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                float2 s[2] = {both(0.0f), both(0.0f)};
+                uint32_t pk[32];
+                const float2 sl2 = both(args.sl2), off = both(-m);
 #pragma unroll
-                for (int cc = 0; cc < 2; ++cc) {
-                    uint32_t pk[32];
-#pragma unroll
-                    for (int e = 0; e < 32; ++e) {
-                        const float p0 = ex2_ftz(fmaf(x[cc * 64 + 2 * e], args.sl2, -m));
-                        const float p1 = ex2_ftz(fmaf(x[cc * 64 + 2 * e + 1], args.sl2, -m));
-                        s[(2 * e) & 3] += p0;
-                        s[(2 * e + 1) & 3] += p1;
-                        const __nv_bfloat162 b2 = __floats2bfloat162_rn(p0, p1);
-                        pk[e] = *reinterpret_cast<const uint32_t*>(&b2);
-                    }
-                    tmem_st32(s_tmem + (uint32_t)(cc * 32), pk);
+                for (int e = 0; e < 32; ++e) {
+                    const float2 y = fma2(make_float2(x[2 * e], x[2 * e + 1]), sl2, off);
+                    const float2 p2 = make_float2(ex2_ftz(y.x), ex2_ftz(y.y));
+                    s[e & 1] = add2(s[e & 1], p2);
+                    pk[e] = pack_bf16(p2.x, p2.y);
                 }
+                tmem_st32(s_tmem, pk);
                 tmem_st_wait();
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&p_full[w]);
-                l += (s[0] + s[1]) + (s[2] + s[3]);
+                l += (s[0].x + s[0].y) + (s[1].x + s[1].y);
             }
             if (!ok) break;
-            // both warpgroups' sums of the row, moved to the last tile's reference
-            float2* mine = fin + (lt & 1) * 256;
-            mine[w * 128 + row] = make_float2(m, l);
+            // the row's four sums, moved to the last tile's reference
+            float2* mine = fin + (lt & 1) * 512;
+            mine[wg * 128 + row] = make_float2(m, l);
             __syncwarp();
             if (lane == 0) mbar_arrive(&fin_bar[(lt & 1) * 4 + q]);
             if (!(ok = warp_wait(&fin_bar[(lt & 1) * 4 + q], (uint32_t)((lt >> 1) & 1), abort_flag))) break;
-            const int wl = (g0 + nt - 1) & 1;  // the warpgroup of the last tile
-            const float2 last = mine[wl * 128 + row], other = mine[(wl ^ 1) * 128 + row];
-            const float sum = last.y + (nt > 1 ? other.y * ex2_ftz(other.x - last.x) : 0.0f);
+            const int wl = (g0 + nt - 1) & 1;  // the last tile's parity
+            const float2 last = mine[wl * 256 + row], other = mine[(wl ^ 1) * 256 + row];
+            float sum = last.y + mine[wl * 256 + 128 + row].y;
+            if (nt > 1) sum = fmaf(other.y + mine[(wl ^ 1) * 256 + 128 + row].y, ex2_ftz(other.x - last.x), sum);
             if (!(ok = warp_wait(&o_full[ob], (uint32_t)((lt / C::kORing) & 1), abort_flag))) break;
             tc_fence_after();
             const int64_t tok = un.tok0 + row - shift;
-            if (w == 0 && row >= shift) args.lse[un.h * args.ld_lse + tok] = fmaf(last.x, kLn2, logf(sum));
+            if (wg == 0 && row >= shift) args.lse[un.h * args.ld_lse + tok] = fmaf(last.x, kLn2, logf(sum));
             const float inv = 1.0f / sum;
-            __nv_bfloat16* op = args.o + tok * args.o_tok + un.h * args.o_head + w * (D / 2);
+            __nv_bfloat16* op = args.o + tok * args.o_tok + un.h * args.o_head + wg * (D / 4);
 #pragma unroll 1
-            for (int cc = 0; cc < D / 64; ++cc) {
+            for (int cc = 0; cc < D / 128; ++cc) {
                 uint32_t r[32];
                 __syncwarp();
-                tmem_ld32(o_tmem + (uint32_t)(w * (D / 2) + cc * 32), r);
+                tmem_ld32(o_tmem + (uint32_t)(wg * (D / 4) + cc * 32), r);
                 tmem_ld_wait();
-                if (row >= shift) {
-#pragma unroll
-                    for (int v = 0; v < 4; ++v) {
-                        uint32_t pk[4];
-#pragma unroll
-                        for (int h2 = 0; h2 < 4; ++h2) {
-                            const __nv_bfloat162 b2 =
-                                __floats2bfloat162_rn(__uint_as_float(r[v * 8 + h2 * 2]) * inv,
-                                                      __uint_as_float(r[v * 8 + h2 * 2 + 1]) * inv);
-                            pk[h2] = *reinterpret_cast<const uint32_t*>(&b2);
-                        }
-                        *reinterpret_cast<uint4*>(op + cc * 32 + v * 8) = make_uint4(pk[0], pk[1], pk[2], pk[3]);
-                    }
-                }
+                if (row >= shift) store_row32(op + cc * 32, r, inv);
             }
             tc_fence_before();
             __syncwarp();
@@ -469,8 +513,9 @@ int launch_fwd(const R97bPacked& p, const R97bAttnPackedFwd& a, cudaStream_t st)
 // At D = 256 dV and dK of 128 keys fill the 512 TMEM columns by themselves, so they are two passes, the second computing
 // S^T again. The rows' operands stay in shared memory for the unit; the others stream through a ring of 16 KB chunks,
 // K-major for the score products and MN-major for the accumulating ones, whose A operand (P or dS, bf16) the
-// elementwise threads write over the scores' own TMEM columns. Each thread owns a row and one of two warpgroups half of
-// its columns, and the products of one tile run beside the exponentials of the next.
+// elementwise threads write over their own columns of the scores' TMEM. Each thread owns a row and each of the four
+// warpgroups 32 of its columns; the next tile's S is issued before the accumulating products, so its exponentials run
+// beside them, and only dS (a product and a rounding) stands between dP and the products that read it.
 enum Kind { kDQ = 0, kDKV = 1, kDV = 2, kDK = 3 };
 
 template <int D, int KIND>
@@ -481,7 +526,7 @@ struct BCfg {
     static constexpr int kStages = D == 256 && kDP ? 6 : 9;
     static constexpr int kRingOff = (kDP ? 2 : 1) * kABytes;
     static constexpr int kBarOff = kRingOff + kStages * kChunk;
-    static constexpr int kStatOff = kBarOff + 512;    // kKeys: float [2 (stage)][lse, delta][128]
+    static constexpr int kStatOff = kBarOff + 512;    // kKeys: float [2 (stage)][-lse log2 e, -delta][128]
     static constexpr int kSmemBytes = kStatOff + (kKeys ? 2048 : 0);
     static constexpr int kVRows = kChunk / (D * 2);
 };
@@ -536,8 +581,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint64_t* a_full = empty_bar + C::kStages;   // [2]
     uint64_t* a_empty = a_full + 2;              // [2]
     uint64_t* s_full = a_empty + 2;              // [2]
-    uint64_t* s_free = s_full + 2;               // kDQ, kDK: S read into registers
-    uint64_t* p_full = s_free + 1;               // [2] kDV, kDKV: P written
+    uint64_t* s_free = s_full + 2;               // all but kDV: S read into registers
+    uint64_t* p_full = s_free + 1;               // [2] kDV: P written
     uint64_t* dp_full = p_full + 2;
     uint64_t* ds_full = dp_full + 1;
     uint64_t* acc_full = ds_full + 1;
@@ -563,15 +608,15 @@ __global__ void __launch_bounds__(kThreads, 1)
             mbar_init(&a_full[b], 1);
             mbar_init(&a_empty[b], 1);
             mbar_init(&s_full[b], 1);
-            mbar_init(&p_full[b], 8);
+            mbar_init(&p_full[b], kSoftWarps);
             mbar_init(&stat_full[b], 1);
-            mbar_init(&stat_empty[b], 8);
+            mbar_init(&stat_empty[b], kSoftWarps);
         }
-        mbar_init(s_free, 8);
+        mbar_init(s_free, kSoftWarps);
         mbar_init(dp_full, 1);
-        mbar_init(ds_full, 8);
+        mbar_init(ds_full, kSoftWarps);
         mbar_init(acc_full, 1);
-        mbar_init(acc_empty, 8);
+        mbar_init(acc_empty, kSoftWarps);
         *abort_flag = 0;
         fence_mbar_init();
     }
@@ -647,12 +692,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (C::kDP) load(&tB1, false, args.b1_head, 0);
                 for (int j = 0; j < wk.tiles && ok; ++j) {
                     const bool more = j + 1 < wk.tiles;
-                    if (KIND == kDKV) load(&tC0, true, args.c0_head, j);
                     if (more) load(&tB0, false, args.b0_head, j + 1);
-                    if (KIND == kDKV)
-                        load(&tC1, true, args.c1_head, j);
-                    else
-                        load(&tC0, true, args.c0_head, j);
+                    load(&tC0, true, args.c0_head, j);
+                    if (KIND == kDKV) load(&tC1, true, args.c1_head, j);
                     if (more && C::kDP) load(&tB1, false, args.b1_head, j + 1);
                 }
                 ++lt;
@@ -697,8 +739,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     const uint32_t b = c_lo + (uint32_t)(stage * kChunkLo);
 #pragma unroll
                     for (int kk = 0; kk < C::kVRows / 16; ++kk) {
-                        const int k16 = ch * (C::kVRows / 16) + kk;  // the halves' bf16 columns start 64 apart
-                        umma_f16_ts_by(lead, d, a + (uint32_t)((k16 >> 2) * 64 + (k16 & 3) * 8),
+                        umma_f16_ts_by(lead, d, a + (uint32_t)quarter_col(ch * (C::kVRows / 16) + kk),
                                        sdesc(b + kk * 128, kDescHi), idesc_c, (!first || ch > 0 || kk > 0) ? 1u : 0u);
                     }
                     next();
@@ -715,7 +756,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const int n = wk.tiles;
                 auto issue_s = [&](int j) {
                     const int gj = g + j, b = KIND == kDV ? (gj & 1) : 0;
-                    if ((KIND == kDQ || KIND == kDK) && gj > 0) wait(s_free, gj - 1);
+                    if (KIND != kDV && gj > 0) wait(s_free, gj - 1);
                     if (j == 0) wait(&a_full[0], lt);
                     if (!ok) return;
                     score(0, tmem + (uint32_t)(b * kBlk));
@@ -734,28 +775,17 @@ __global__ void __launch_bounds__(kThreads, 1)
                 for (int j = 0; j < n && ok; ++j) {
                     const int gj = g + j;
                     const bool more = j + 1 < n;
-                    if (KIND == kDKV) {
-                        wait(&p_full[0], gj);
-                        if (j == 0) wait(acc_empty, lt + 1);
-                        if (!ok) break;
-                        accumulate(tmem, acc0, j == 0);
-                        if (more) issue_s(j + 1);
+                    if (more) issue_s(j + 1);
+                    const int b = KIND == kDV ? (gj & 1) : 0;
+                    if (KIND == kDV)
+                        wait(&p_full[b], gj >> 1);
+                    else
                         wait(ds_full, gj);
-                        if (!ok) break;
-                        accumulate(tmem + (uint32_t)kBlk, acc1, j == 0);
-                        if (more) issue_dp(j + 1);
-                    } else {
-                        if (more) issue_s(j + 1);
-                        const int b = KIND == kDV ? (gj & 1) : 0;
-                        if (KIND == kDV)
-                            wait(&p_full[b], gj >> 1);
-                        else
-                            wait(ds_full, gj);
-                        if (j == 0) wait(acc_empty, lt + 1);
-                        if (!ok) break;
-                        accumulate(tmem + (uint32_t)(KIND == kDV ? b * kBlk : kBlk), acc0, j == 0);
-                        if (more && C::kDP) issue_dp(j + 1);
-                    }
+                    if (j == 0) wait(acc_empty, lt + 1);
+                    if (!ok) break;
+                    accumulate(tmem + (uint32_t)(KIND == kDV ? b * kBlk : kBlk), acc0, j == 0);
+                    if (KIND == kDKV) accumulate(tmem + (uint32_t)(kBlk + 16), acc1, j == 0);
+                    if (more && C::kDP) issue_dp(j + 1);
                 }
                 if (!ok) break;
                 umma_commit_by(lead, acc_full);
@@ -777,9 +807,9 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         const int col = e * 32 + lane;
-                        // a column before the block's first token: probability 2^-inf = 0
-                        v[e] = col >= shift ? args.lse[h * args.ld_lse + tok + col] * kLog2e : INFINITY;
-                        v[4 + e] = C::kDP && col >= shift ? args.delta[h * args.ld_delta + tok + col] : 0.0f;
+                        // negated, for the sums that take them; a column before the block's first token: 2^-inf = 0
+                        v[e] = col >= shift ? args.lse[h * args.ld_lse + tok + col] * -kLog2e : -INFINITY;
+                        v[4 + e] = C::kDP && col >= shift ? -args.delta[h * args.ld_delta + tok + col] : 0.0f;
                     }
                     if (!(ok = warp_wait(&stat_empty[st], (uint32_t)((g >> 1) & 1) ^ 1u, abort_flag))) break;
                     float* s = stats + st * 256;
@@ -796,7 +826,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int q = warp & 3, w = (warp - 4) >> 2;
         const int row = q * 32 + lane;
         const uint32_t lane_off = (uint32_t)(q * 32) << 16;
-        const uint32_t half = tmem + lane_off + (uint32_t)(w * 64);  // this thread's columns of S (and, 128 on, of dP)
+        const uint32_t mine = tmem + lane_off + (uint32_t)(w * 32);  // this thread's columns of S (and, 128 on, of dP)
         int g = 0, lt = 0;
         bool ok = true;
         for (int t = 0; ok && t * G < args.units; ++t) {
@@ -810,88 +840,74 @@ __global__ void __launch_bounds__(kThreads, 1)
                 lse2 = args.lse[wk.h * args.ld_lse + tok] * kLog2e;
                 delta = args.delta[wk.h * args.ld_delta + tok];
             }
-            for (int j = 0; j < wk.tiles; ++j, ++g) {
+            for (int j = 0, jm = 0; j < wk.tiles; ++j, ++g) {
                 const int b = KIND == kDV ? (g & 1) : 0;
-                const bool diag = wk.block(j) == wk.i;
-                const float* st = stats + (g & 1) * 256 + w * 64;
+                // the diagonal tile: the last of kDQ, the first of each query head else
+                const bool diag = C::kKeys ? jm == 0 : j + 1 == wk.tiles;
+                if (++jm == wk.m) jm = 0;
+                const float* st = stats + (g & 1) * 256 + w * 32;
                 if (C::kKeys && !(ok = warp_wait(&stat_full[g & 1], (uint32_t)((g >> 1) & 1), abort_flag))) break;
                 if (!(ok = warp_wait(&s_full[b], (uint32_t)((KIND == kDV ? g >> 1 : g) & 1), abort_flag))) break;
                 tc_fence_after();
-                float p[64];
-#pragma unroll
-                for (int cc = 0; cc < 2; ++cc)
-                    tmem_ld32(half + (uint32_t)(b * kBlk + cc * 32), *reinterpret_cast<uint32_t(*)[32]>(&p[cc * 32]));
+                float p[32];
+                tmem_ld32(mine + (uint32_t)(b * kBlk), *reinterpret_cast<uint32_t(*)[32]>(&p[0]));
                 tmem_ld_wait();
-                if (KIND == kDQ || KIND == kDK) {
+                if (KIND != kDV) {
                     tc_fence_before();
                     __syncwarp();
                     if (lane == 0) mbar_arrive(s_free);
                 }
-                if (C::kKeys) {
+                const float2 sl2 = both(args.sl2);
 #pragma unroll
-                    for (int e = 0; e < 64; e += 4) {
-                        const float4 l4 = *reinterpret_cast<const float4*>(st + e);
-                        p[e] = ex2_ftz(fmaf(p[e], args.sl2, -l4.x));
-                        p[e + 1] = ex2_ftz(fmaf(p[e + 1], args.sl2, -l4.y));
-                        p[e + 2] = ex2_ftz(fmaf(p[e + 2], args.sl2, -l4.z));
-                        p[e + 3] = ex2_ftz(fmaf(p[e + 3], args.sl2, -l4.w));
+                for (int e = 0; e < 16; ++e) {
+                    float2 y = make_float2(p[2 * e], p[2 * e + 1]);
+                    if (C::kKeys) {  // the column's -lse
+                        y = fma2(y, sl2, *reinterpret_cast<const float2*>(st + 2 * e));
+                    } else {
+                        y = fma2(y, sl2, both(-lse2));
                     }
-                    if (diag) {
-#pragma unroll
-                        for (int e = 0; e < 64; ++e)
-                            if (w * 64 + e < row) p[e] = 0.0f;
-                    }
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 64; ++e) p[e] = ex2_ftz(fmaf(p[e], args.sl2, -lse2));
-                    if (diag) {
-#pragma unroll
-                        for (int e = 0; e < 64; ++e)
-                            if (w * 64 + e > row || w * 64 + e < shift) p[e] = 0.0f;
-                    }
+                    p[2 * e] = ex2_ftz(y.x);
+                    p[2 * e + 1] = ex2_ftz(y.y);
                 }
-                if (KIND == kDV || KIND == kDKV) {
-                    uint32_t pk[32];
+                if (diag) {
 #pragma unroll
                     for (int e = 0; e < 32; ++e) {
-                        const __nv_bfloat162 b2 = __floats2bfloat162_rn(p[2 * e], p[2 * e + 1]);
-                        pk[e] = *reinterpret_cast<const uint32_t*>(&b2);
+                        const int col = w * 32 + e;
+                        if (C::kKeys ? col < row : (col > row || col < shift)) p[e] = 0.0f;
                     }
-                    tmem_st32(half + (uint32_t)(b * kBlk), pk);
+                }
+                uint32_t pk[16];
+                if (KIND == kDV || KIND == kDKV) {
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) pk[e] = pack_bf16(p[2 * e], p[2 * e + 1]);
+                }
+                if (KIND == kDV) {
+                    tmem_st16(mine + (uint32_t)(b * kBlk), pk);
                     tmem_st_wait();
                     tc_fence_before();
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&p_full[b]);
-                }
-                if (C::kDP) {
+                } else {
                     if (!(ok = warp_wait(dp_full, (uint32_t)(g & 1), abort_flag))) break;
                     tc_fence_after();
-                    float d[64];
-#pragma unroll
-                    for (int cc = 0; cc < 2; ++cc)
-                        tmem_ld32(half + (uint32_t)(kBlk + cc * 32), *reinterpret_cast<uint32_t(*)[32]>(&d[cc * 32]));
+                    float d[32];
+                    tmem_ld32(mine + (uint32_t)kBlk, *reinterpret_cast<uint32_t(*)[32]>(&d[0]));
                     tmem_ld_wait();
-                    uint32_t pk[32];
+                    if (KIND == kDKV) tmem_st16(mine + (uint32_t)kBlk, pk);  // P beside dS, over dP
 #pragma unroll
-                    for (int e = 0; e < 64; e += 4) {
-                        float4 d4 = make_float4(delta, delta, delta, delta);
-                        if (C::kKeys) d4 = *reinterpret_cast<const float4*>(st + 128 + e);
-                        const __nv_bfloat162 lo = __floats2bfloat162_rn(p[e] * (d[e] - d4.x), p[e + 1] * (d[e + 1] - d4.y));
-                        const __nv_bfloat162 hi =
-                            __floats2bfloat162_rn(p[e + 2] * (d[e + 2] - d4.z), p[e + 3] * (d[e + 3] - d4.w));
-                        pk[e / 2] = *reinterpret_cast<const uint32_t*>(&lo);
-                        pk[e / 2 + 1] = *reinterpret_cast<const uint32_t*>(&hi);
+                    for (int e = 0; e < 16; ++e) {
+                        float2 n = both(-delta);  // minus the row's delta, or the columns'
+                        if (C::kKeys) n = *reinterpret_cast<const float2*>(st + 128 + 2 * e);
+                        const float2 y = mul2(make_float2(p[2 * e], p[2 * e + 1]), add2(make_float2(d[2 * e], d[2 * e + 1]), n));
+                        pk[e] = pack_bf16(y.x, y.y);
                     }
-                    tmem_st32(half + (uint32_t)kBlk, pk);
+                    tmem_st16(mine + (uint32_t)(kBlk + (KIND == kDKV ? 16 : 0)), pk);
                     tmem_st_wait();
                     tc_fence_before();
                     __syncwarp();
                     if (lane == 0) mbar_arrive(ds_full);
                 }
-                if (C::kKeys) {
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(&stat_empty[g & 1]);
-                }
+                if (C::kKeys && lane == 0) mbar_arrive(&stat_empty[g & 1]);
             }
             if (!ok) break;
             if (!(ok = warp_wait(acc_full, (uint32_t)(lt & 1), abort_flag))) break;
@@ -902,27 +918,14 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const float f = (KIND == kDV || (KIND == kDKV && r == 0)) ? 1.0f : args.scale;
                 __nv_bfloat16* op = r ? args.out1 + tok * args.tok1 + wk.h * args.head1
                                       : args.out0 + tok * args.tok0 + wk.h * args.head0;
-                const uint32_t src = (r ? acc1 : acc0) + lane_off + (uint32_t)(w * (D / 2));
+                const uint32_t src = (r ? acc1 : acc0) + lane_off + (uint32_t)(w * (D / 4));
 #pragma unroll 1
-                for (int cc = 0; cc < D / 64; ++cc) {
+                for (int cc = 0; cc < D / 128; ++cc) {
                     uint32_t v[32];
                     __syncwarp();
                     tmem_ld32(src + (uint32_t)(cc * 32), v);
                     tmem_ld_wait();
-                    if (row >= shift) {
-#pragma unroll
-                        for (int k = 0; k < 4; ++k) {
-                            uint32_t pk[4];
-#pragma unroll
-                            for (int h2 = 0; h2 < 4; ++h2) {
-                                const __nv_bfloat162 b2 = __floats2bfloat162_rn(__uint_as_float(v[k * 8 + h2 * 2]) * f,
-                                                                                __uint_as_float(v[k * 8 + h2 * 2 + 1]) * f);
-                                pk[h2] = *reinterpret_cast<const uint32_t*>(&b2);
-                            }
-                            *reinterpret_cast<uint4*>(op + w * (D / 2) + cc * 32 + k * 8) =
-                                make_uint4(pk[0], pk[1], pk[2], pk[3]);
-                        }
-                    }
+                    if (row >= shift) store_row32(op + w * (D / 4) + cc * 32, v, f);
                 }
             }
             tc_fence_before();
