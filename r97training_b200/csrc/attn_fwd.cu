@@ -57,10 +57,6 @@ struct FwdArgs {
     __nv_bfloat16* out;        // [B*Hq*S, D]
 };
 
-__device__ __forceinline__ void fence_proxy_async_smem() {
-    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-}
-
 // A CTA's t-th unit: a snake over the longest-first order (query blocks descending), so a CTA's heavy
 // unit of one round meets a light one in the next.
 __device__ __forceinline__ int unit_of(int t, int c, int G) { return t * G + ((t & 1) ? (G - 1 - c) : c); }

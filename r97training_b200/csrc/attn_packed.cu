@@ -30,10 +30,6 @@ constexpr int kBlk = 128;           // queries of a unit, keys of a tile
 constexpr int kChunk = 16384;       // one ring stage
 constexpr int kChunkLo = kChunk >> 4;               // and its step in a matrix descriptor
 constexpr uint32_t kDescHi = sdesc_hi_sw128(1024);  // 8 rows of 128 bytes a swizzle atom
-constexpr int kThreads = 640;       // warps 0, 3: TMA, warp 1: MMA, warp 2: statistics; four softmax warpgroups after
-constexpr int kSoftWarps = 16;
-constexpr int kCtrlRegs = 64, kSoftRegs = 104;  // 128 x 64 + 512 x 104 = 640 x 96, what the launch holds
-static_assert(128 * kCtrlRegs + 512 * kSoftRegs <= 640 * 96, "register split");
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr long long kWaitCycles = 4000000000ll;  // a wait's limit, about two seconds
@@ -86,24 +82,24 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
     const __nv_bfloat162 b = __floats2bfloat162_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&b);
 }
-__device__ __forceinline__ float max_nan(float a, float b) {
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
     float d;
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
     return d;
 }
 
 template <int D>
 struct FCfg {
+    static constexpr int kBufs = D == 128 ? 3 : 2;       // S buffers, each with a softmax warpgroup of its own
+    static constexpr int kThreads = 128 + 128 * kBufs;   // warps 0, 3: TMA, warp 1: MMA; the softmax warpgroups after
     static constexpr int kQBytes = kBlk * D * 2;
     static constexpr int kQStages = D == 128 ? 2 : 1;
-    static constexpr int kORing = D == 128 ? 2 : 1;      // O accumulators in TMEM
     static constexpr int kStages = 9;
     static constexpr int kRingOff = kQStages * kQBytes;
     static constexpr int kBarOff = kRingOff + kStages * kChunk;
-    static constexpr int kMaxOff = kBarOff + 640;        // float [2][128]: the reference each tile parity used last
-    static constexpr int kPartOff = kMaxOff + 1024;      // float [2][2][128]: a tile's maxima by column half
-    static constexpr int kFinOff = kPartOff + 2048;      // float2 [2 (unit parity)][4][128]: (reference, sum)
-    static constexpr int kSmemBytes = kFinOff + 8192 + 1024;
+    static constexpr int kMaxOff = kBarOff + 768;        // float [kBufs][128]: the reference each buffer's tile used
+    static constexpr int kFinOff = kMaxOff + kBufs * 512;  // float2 [2 (unit parity)][kBufs][128]: (reference, sum)
+    static constexpr int kSmemBytes = kFinOff + 2 * kBufs * 1024 + 1024;
     static constexpr int kVRows = kChunk / (D * 2);      // keys of one V chunk
 };
 
@@ -112,7 +108,7 @@ struct FwdArgs {
     __nv_bfloat16* o;
     float* lse;
     int64_t o_tok, o_head, ld_lse;
-    int32_t Hq, grp, units;
+    int32_t Hq, grp;
     int32_t q_head, k_head, v_head;
     float sl2;   // |scale| log2 e (1 for a scale of 0), so that the row maximum is the scores'
     float sign;  // of the scale: 1, -1 or 0
@@ -134,13 +130,49 @@ __device__ __forceinline__ void store_row32(__nv_bfloat16* p, const uint32_t (&r
     }
 }
 
-// The TMEM column of 16 consecutive k (k16-th) of a bf16 A operand whose writers own 64 (or 32) f32 columns each and
-// leave their values packed at the start of their own columns.
-__device__ __forceinline__ constexpr int half_col(int k16) { return (k16 >> 2) * 64 + (k16 & 3) * 8; }
+// The TMEM column of 16 consecutive k (k16-th) of a bf16 A operand whose writers own 32 f32 columns each and leave their
+// values packed at the start of their own columns.
 __device__ __forceinline__ constexpr int quarter_col(int k16) { return (k16 >> 1) * 32 + (k16 & 1) * 8; }
 
-// A CTA's t-th unit: a snake over the longest-first order, so a heavy unit of one round meets a light one in the next.
-__device__ __forceinline__ int unit_of(int t, int c, int G) { return t * G + ((t & 1) ? (G - 1 - c) : c); }
+// The next unit of a CTA, for every role of it. The grid has one CTA a unit, longest units first; a CTA starts with its
+// own and then takes over (cancels) the launch of the next one that has not started, so the units go to whichever SM is
+// free. One role asks, as it loads the last tile of the unit before; the answers pass through kSlots shared-memory slots, each read by every warp that
+// walks the units (`readers` of them).
+struct UnitQueue {
+    static constexpr int kSlots = 4;
+    uint4* slot;      // [kSlots]
+    uint64_t* full;   // [kSlots]
+    uint64_t* empty;  // [kSlots]
+    volatile int* abort;
+
+    __device__ void init(int readers) const {
+        for (int i = 0; i < kSlots; ++i) {
+            mbar_init(&full[i], 1);
+            mbar_init(&empty[i], readers);
+        }
+    }
+    // Asks for the CTA's unit after its t-th (a whole warp, `lead` one lane of it); false when a wait gave up.
+    __device__ bool ask(int t, uint32_t lead) const {
+        const int i = t % kSlots;
+        if (!warp_wait(&empty[i], (uint32_t)((t / kSlots) & 1) ^ 1u, abort)) return false;
+        if (lead) {
+            mbar_expect_tx(&full[i], 16);
+            launch_cancel(&slot[i], &full[i]);
+        }
+        __syncwarp();
+        return true;
+    }
+    // The unit after the t-th, or -1 when there is none (or a wait gave up): by a whole warp that counts as a reader.
+    __device__ int next(int t) const {
+        const int i = t % kSlots;
+        if (!warp_wait(&full[i], (uint32_t)((t / kSlots) & 1), abort)) return -1;
+        const int u = launch_cancelled(&slot[i]);
+        fence_proxy_async_smem();  // the read, before the next answer's write
+        __syncwarp();
+        if ((threadIdx.x & 31) == 0) mbar_arrive(&empty[i]);
+        return u;
+    }
+};
 
 __device__ __forceinline__ Unit unit_geom(const int4* blocks, int heads, int u) {
     const int b = u / heads;
@@ -148,43 +180,46 @@ __device__ __forceinline__ Unit unit_geom(const int4* blocks, int heads, int u) 
     return Unit{u - b * heads, e.x + e.z * kBlk, e.z, min(kBlk, e.y - e.z * kBlk)};
 }
 
-// One pass over the keys. A unit is one 128-query block of one head; key tile j of it: S_j = Q K_j^T into one of two
-// TMEM buffers, P_j = 2^(S_j c - m) as bf16 over the same buffer's columns, O += P_j V_j in TMEM. The four softmax
-// warpgroups are two pairs that take the tiles in turn, a thread a row and half of the columns, so the exponentials of
-// one tile run beside the row maximum of the next and both beside the products: S_{j+1} is issued before P_j V_j. The
-// reference m a row's exponentials use is handed from tile to tile; it is moved (and O rescaled, by the threads that own
-// the rows) only when the row's maximum has outgrown it by 2^8, which f32 sums and bf16 probabilities carry without loss.
+// One pass over the keys. A unit is one 128-query block of one head; key tile j of it: S_j = Q K_j^T into one of kBufs
+// TMEM buffers, P_j = 2^(S_j c - m) as bf16 over the same buffer's columns, O += P_j V_j in TMEM. Each buffer has a
+// softmax warpgroup, a thread a row, so the tiles' exponentials overlap one another and the products: S is issued kBufs - 1
+// tiles ahead of P V, and P V starts on the first half of the keys while the second half's P is formed. The reference m a
+// row's exponentials use is handed from tile to tile; it is moved (and O rescaled, by the threads that own the rows) only
+// when the row's maximum has outgrown it by 2^8, which f32 sums and bf16 probabilities carry without loss. A unit's
+// result is drained after the next unit's first P, which the tensor core has meanwhile been given the scores of.
 template <int D>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(FCfg<D>::kThreads, 1)
     fwd_kernel(const __grid_constant__ CUtensorMap tQ, const __grid_constant__ CUtensorMap tK,
                const __grid_constant__ CUtensorMap tV, const FwdArgs args) {
     using C = FCfg<D>;
-    constexpr int ND = D / 64;
+    constexpr int ND = D / 64, NB = C::kBufs;
     constexpr int kVC = kBlk / C::kVRows;  // V chunks of a tile
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
     uint8_t* ring = smem + C::kRingOff;
     uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + C::kBarOff);
+    const UnitQueue queue{reinterpret_cast<uint4*>(full_bar), full_bar + 8, full_bar + 12,
+                          reinterpret_cast<volatile int*>(full_bar + 16)};
+    volatile int* abort_flag = queue.abort;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(full_bar + 16) + 1;
+    full_bar += 17;
     uint64_t* empty_bar = full_bar + C::kStages;
     uint64_t* q_full = empty_bar + C::kStages;  // [2]
     uint64_t* q_empty = q_full + 2;             // [2]
-    uint64_t* s_full = q_empty + 2;             // [2]
-    uint64_t* p_full = s_full + 2;              // [2]
-    uint64_t* o_full = p_full + 2;              // [2]
-    uint64_t* o_empty = o_full + 2;             // [2]
-    uint64_t* pv_done = o_empty + 2;            // [2]
-    uint64_t* part_bar = pv_done + 2;           // [2][4]: both halves' maxima of a tile's lane quarter written
-    uint64_t* max_bar = part_bar + 8;           // [2][4]: its reference written, and the one before it read
-    uint64_t* fin_bar = max_bar + 8;            // [2][4]: the four warps of a lane quarter wrote a unit's sums
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(fin_bar + 8);
-    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    uint64_t* s_full = q_empty + 2;             // [NB]
+    uint64_t* p_full = s_full + NB;             // [NB][2]: the first and second 64 keys' P written
+    uint64_t* pv_done = p_full + 2 * NB;        // [NB]
+    uint64_t* o_full = pv_done + NB;
+    uint64_t* o_empty = o_full + 1;
+    uint64_t* max_bar = o_empty + 1;            // [NB][4]: a tile's reference written, by lane quarter
+    uint64_t* fin_bar = max_bar + 4 * NB;       // [2][4]: the unit's sums written, by lane quarter
     float* ref_m = reinterpret_cast<float*>(smem + C::kMaxOff);
-    float* part = reinterpret_cast<float*>(smem + C::kPartOff);
     float2* fin = reinterpret_cast<float2*>(smem + C::kFinOff);
 
     const int warp = __shfl_sync(0xFFFFFFFFu, threadIdx.x >> 5, 0);
     const int lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
+        queue.init(3 + 4 * NB);
         for (int s = 0; s < C::kStages; ++s) {
             mbar_init(&full_bar[s], 1);
             mbar_init(&empty_bar[s], 1);
@@ -192,17 +227,17 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int b = 0; b < 2; ++b) {
             mbar_init(&q_full[b], 2);
             mbar_init(&q_empty[b], 1);
+        }
+        for (int b = 0; b < NB; ++b) {
             mbar_init(&s_full[b], 1);
-            mbar_init(&p_full[b], kSoftWarps / 2);
-            mbar_init(&o_full[b], 1);
-            mbar_init(&o_empty[b], kSoftWarps);
+            mbar_init(&p_full[2 * b], 4);
+            mbar_init(&p_full[2 * b + 1], 4);
             mbar_init(&pv_done[b], 1);
         }
-        for (int b = 0; b < 8; ++b) {
-            mbar_init(&part_bar[b], 2);
-            mbar_init(&max_bar[b], 2);
-            mbar_init(&fin_bar[b], 4);
-        }
+        mbar_init(o_full, 1);
+        mbar_init(o_empty, 4 * NB);
+        for (int b = 0; b < 4 * NB; ++b) mbar_init(&max_bar[b], 1);
+        for (int b = 0; b < 8; ++b) mbar_init(&fin_bar[b], NB);
         *abort_flag = 0;
         fence_mbar_init();
     }
@@ -219,37 +254,40 @@ __global__ void __launch_bounds__(kThreads, 1)
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = __shfl_sync(0xFFFFFFFFu, *tmem_slot, 0);
-    const int G = gridDim.x, c = blockIdx.x;
+    const uint32_t o_base = tmem + (uint32_t)(NB * kBlk);
 
-    if (warp < 4) {
-        set_max_regs_dec<kCtrlRegs>();
-        if (warp == 0 || warp == 3) {
-            // --------------------------------------------------------- TMA producers: every other chunk each
-            const uint32_t lead = elect_one();
-            const int p = warp == 3;
-            int stage = p, lt = 0;
-            uint32_t phase = 0;
-            bool ok = true;
-            for (int t = 0; ok && t * G < args.units; ++t) {
-                const int u = unit_of(t, c, G);
-                if (u >= args.units) continue;
-                const Unit un = unit_geom(args.blocks, args.Hq, u);
-                const int shift = kBlk - un.n, kvh = un.h / args.grp;
-                const int seq0 = un.tok0 - un.i * kBlk;
-                const int qs = lt % C::kQStages;
-                if (!warp_wait(&q_empty[qs], (uint32_t)((lt / C::kQStages) & 1) ^ 1u, abort_flag)) break;
-                if (lead) {
-                    mbar_expect_tx(&q_full[qs], C::kQBytes / 2);
-                    for (int s = p; s < ND; s += 2)
-                        tma_load_3d(smem + qs * C::kQBytes + s * kChunk, &tQ, &q_full[qs], un.h * args.q_head + 64 * s, -shift,
-                                    un.tok0);
-                }
-                auto load = [&](bool v, int j) {
-                    const int tok = seq0 + j * kBlk, r0 = j == un.i ? -shift : 0;
+    if (warp == 0 || warp == 3) {
+        // ------------------------------------------------------------- TMA producers: every other chunk each
+        const uint32_t lead = elect_one();
+        const int p = warp == 3;
+        int stage = p;
+        uint32_t phase = 0;
+        bool ok = true;
+        for (int u = blockIdx.x, lt = 0; ok && u >= 0; u = ok ? queue.next(lt) : -1, ++lt) {
+            const Unit un = unit_geom(args.blocks, args.Hq, u);
+            const int shift = kBlk - un.n, kvh = un.h / args.grp;
+            const int seq0 = un.tok0 - un.i * kBlk;
+            const int qs = lt % C::kQStages;
+            if (!(ok = warp_wait(&q_empty[qs], (uint32_t)((lt / C::kQStages) & 1) ^ 1u, abort_flag))) break;
+            if (lead) {
+                mbar_expect_tx(&q_full[qs], C::kQBytes / 2);
+                for (int s = p; s < ND; s += 2)
+                    tma_load_3d(smem + qs * C::kQBytes + s * kChunk, &tQ, &q_full[qs], un.h * args.q_head + 64 * s, -shift,
+                                un.tok0);
+            }
+            // K of a tile NB - 1 ahead of V
+#pragma unroll 1
+            for (int j = 1 - NB; j <= un.i && ok; ++j) {
+                if (p && j == un.i && !(ok = queue.ask(lt, lead))) break;
+#pragma unroll
+                for (int v = 0; v < 2; ++v) {
+                    const int tile = v ? j : j + NB - 1;
+                    if (tile < 0 || tile > un.i) continue;
+                    const int tok = seq0 + tile * kBlk, r0 = tile == un.i ? -shift : 0;
                     const int x = kvh * (v ? args.v_head : args.k_head);
 #pragma unroll
                     for (int ch = p; ch < (v ? kVC : ND); ch += 2) {
-                        if (!(ok = ok && warp_wait(&empty_bar[stage], phase ^ 1u, abort_flag))) return;
+                        if (!(ok = ok && warp_wait(&empty_bar[stage], phase ^ 1u, abort_flag))) break;
                         if (lead) {
                             uint8_t* st = ring + stage * kChunk;
                             mbar_expect_tx(&full_bar[stage], kChunk);
@@ -267,206 +305,235 @@ __global__ void __launch_bounds__(kThreads, 1)
                             phase ^= 1u;
                         }
                     }
-                };
-                load(false, 0);
-                for (int j = 0; j <= un.i && ok; ++j) {
-                    if (j < un.i) load(false, j + 1);
-                    load(true, j);
                 }
-                ++lt;
             }
-        } else if (warp == 1) {
-            const uint32_t lead = elect_one();
-            // --------------------------------------------------------- MMA issuer
-            constexpr uint32_t idesc_s = make_idesc_bf16(kBlk, kBlk, 0, 0);
-            constexpr uint32_t idesc_o = make_idesc_bf16(kBlk, D, 0, 1);
-            const uint32_t k_lo = sdesc_lo(smem_u32(ring), 16), v_lo = sdesc_lo(smem_u32(ring), C::kVRows * 128);
-            int stage = 0, lt = 0, g = 0;  // g: tiles whose S has been issued
-            uint32_t phase = 0;
-            bool ok = true;
-            auto next = [&]() {
-                umma_commit_by(lead, &empty_bar[stage]);
-                if (++stage == C::kStages) {
-                    stage = 0;
-                    phase ^= 1u;
-                }
-            };
-            for (int t = 0; ok && t * G < args.units; ++t) {
-                const int u = unit_of(t, c, G);
-                if (u >= args.units) continue;
-                const int nt = unit_geom(args.blocks, args.Hq, u).i + 1;
-                const int qs = lt % C::kQStages, ob = lt % C::kORing;
-                if (!warp_wait(&q_full[qs], (uint32_t)((lt / C::kQStages) & 1), abort_flag)) break;
-                tc_fence_after();
-                const uint32_t q_lo = sdesc_lo(smem_u32(smem), 16) + (uint32_t)(qs * (C::kQBytes >> 4));
-                const uint32_t o_tmem = tmem + 256u + (uint32_t)(ob * 128);
-                // S into buffer g & 1, whose last P the tensor core has taken: P V of two tiles back is before it in
-                // the issue order
-                auto issue_s = [&](bool last) {
+        }
+    } else if (warp == 1) {
+        // ------------------------------------------------------------- MMA issuer
+        const uint32_t lead = elect_one();
+        constexpr uint32_t idesc_s = make_idesc_bf16(kBlk, kBlk, 0, 0);
+        constexpr uint32_t idesc_o = make_idesc_bf16(kBlk, D, 0, 1);
+        const uint32_t k_lo = sdesc_lo(smem_u32(ring), 16), v_lo = sdesc_lo(smem_u32(ring), C::kVRows * 128);
+        int stage = 0, sb = 0, pb = 0;  // sb, pb: the next S's and the next P's buffer
+        uint32_t phase = 0, p_phase = 0;
+        bool ok = true;
+        auto next = [&]() {
+            umma_commit_by(lead, &empty_bar[stage]);
+            if (++stage == C::kStages) {
+                stage = 0;
+                phase ^= 1u;
+            }
+        };
+        for (int u = blockIdx.x, lt = 0; ok && u >= 0; u = ok ? queue.next(lt) : -1, ++lt) {
+            const int nt = unit_geom(args.blocks, args.Hq, u).i + 1;
+            const int qs = lt % C::kQStages;
+            if (!(ok = warp_wait(&q_full[qs], (uint32_t)((lt / C::kQStages) & 1), abort_flag))) break;
+            tc_fence_after();
+            const uint32_t q_lo = sdesc_lo(smem_u32(smem), 16) + (uint32_t)(qs * (C::kQBytes >> 4));
+#pragma unroll 1
+            for (int j = 1 - NB; j < nt && ok; ++j) {
+                const int js = j + NB - 1;
+                if (js < nt) {
+                    // S into the buffer whose last P V is already before it in the issue order
+#pragma unroll
                     for (int kb = 0; kb < ND; ++kb) {
-                        if (!(ok = ok && warp_wait(&full_bar[stage], phase, abort_flag))) return;
+                        if (!(ok = ok && warp_wait(&full_bar[stage], phase, abort_flag))) break;
                         tc_fence_after();
                         const uint32_t a = q_lo + (uint32_t)(kb * kChunkLo), b = k_lo + (uint32_t)(stage * kChunkLo);
 #pragma unroll
                         for (int kk = 0; kk < 4; ++kk)
-                            umma_f16_by(lead, tmem + (uint32_t)((g & 1) * kBlk), sdesc(a + kk * 2, kDescHi),
+                            umma_f16_by(lead, tmem + (uint32_t)(sb * kBlk), sdesc(a + kk * 2, kDescHi),
                                         sdesc(b + kk * 2, kDescHi), idesc_s, (kb > 0 || kk > 0) ? 1u : 0u);
                         next();
                     }
-                    umma_commit_by(lead, &s_full[g & 1]);
-                    if (last) umma_commit_by(lead, &q_empty[qs]);
-                    ++g;
-                };
-                const int g0 = g;
-                issue_s(nt == 1);
-                for (int j = 0; j < nt && ok; ++j) {
-                    if (j + 1 < nt) issue_s(j + 2 == nt);
                     if (!ok) break;
-                    const int gj = g0 + j, b = gj & 1;
-                    if (!(ok = warp_wait(&p_full[b], (uint32_t)((gj >> 1) & 1), abort_flag))) break;
-                    if (j == 0 &&
-                        !(ok = warp_wait(&o_empty[ob], (uint32_t)((lt / C::kORing) & 1) ^ 1u, abort_flag)))
-                        break;
-                    tc_fence_after();
-                    for (int ch = 0; ch < kVC; ++ch) {
-                        if (!(ok = warp_wait(&full_bar[stage], phase, abort_flag))) break;
-                        tc_fence_after();
-                        const uint32_t v = v_lo + (uint32_t)(stage * kChunkLo);
+                    umma_commit_by(lead, &s_full[sb]);
+                    if (js + 1 == nt) umma_commit_by(lead, &q_empty[qs]);
+                    if (++sb == NB) sb = 0;
+                }
+                if (j < 0) continue;
+                if (j == 0 && !(ok = warp_wait(o_empty, (uint32_t)(lt & 1) ^ 1u, abort_flag))) break;
 #pragma unroll
-                        for (int kk = 0; kk < C::kVRows / 16; ++kk)
-                            umma_f16_ts_by(lead, o_tmem, tmem + (uint32_t)(b * kBlk + half_col(ch * (C::kVRows / 16) + kk)),
-                                           sdesc(v + kk * 128, kDescHi), idesc_o,
-                                           (j > 0 || ch > 0 || kk > 0) ? 1u : 0u);
-                        next();
-                    }
-                    if (!ok) break;
-                    umma_commit_by(lead, &pv_done[b]);
+                for (int ch = 0; ch < kVC; ++ch) {
+                    if (ch % (kVC / 2) == 0) ok = ok && warp_wait(&p_full[2 * pb + ch / (kVC / 2)], p_phase, abort_flag);
+                    if (!(ok = ok && warp_wait(&full_bar[stage], phase, abort_flag))) break;
+                    tc_fence_after();
+                    const uint32_t v = v_lo + (uint32_t)(stage * kChunkLo);
+#pragma unroll
+                    for (int kk = 0; kk < C::kVRows / 16; ++kk)
+                        umma_f16_ts_by(lead, o_base, tmem + (uint32_t)(pb * kBlk + (ch * C::kVRows + kk * 16) / 2),
+                                       sdesc(v + kk * 128, kDescHi), idesc_o, (j > 0 || ch > 0 || kk > 0) ? 1u : 0u);
+                    next();
                 }
                 if (!ok) break;
-                umma_commit_by(lead, &o_full[ob]);
-                ++lt;
+                umma_commit_by(lead, &pv_done[pb]);
+                if (++pb == NB) {
+                    pb = 0;
+                    p_phase ^= 1u;
+                }
             }
+            if (!ok) break;
+            umma_commit_by(lead, o_full);
         }
-    } else {
+    } else if (warp >= 4) {
         // ------------------------------------------------------------- softmax
-        set_max_regs_inc<kSoftRegs>();
-        const int q = warp & 3, wg = (warp - 4) >> 2, w = wg >> 1, hf = wg & 1;  // tile parity, column half
+        const int q = warp & 3, w = (warp - 4) >> 2;
         const int row = q * 32 + lane;
         const uint32_t lane_off = (uint32_t)(q * 32) << 16;
-        const uint32_t s_tmem = tmem + lane_off + (uint32_t)(w * kBlk + hf * 64);
-        int g0 = 0, lt = 0;
+        const uint32_t s_tmem = tmem + lane_off + (uint32_t)(w * kBlk), o_tmem = o_base + lane_off;
+        const int prev = w == 0 ? NB - 1 : w - 1;  // the buffer of the tile before
+        int turn = w;                              // tiles until this warpgroup's next
+        uint32_t phase = 0;                        // of this buffer's barriers
         bool ok = true;
-        for (int t = 0; ok && t * G < args.units; ++t) {
-            const int u = unit_of(t, c, G);
-            if (u >= args.units) continue;
-            const Unit un = unit_geom(args.blocks, args.Hq, u);
-            const int shift = kBlk - un.n, nt = un.i + 1, ob = lt % C::kORing;
-            const uint32_t o_tmem = tmem + lane_off + 256u + (uint32_t)(ob * 128);
-            float m = 0.0f, l = 0.0f;  // the reference of this warpgroup's last tile, its columns' sum relative to it
-            for (int j = (g0 + w) & 1; j < nt; j += 2) {
-                const int g = g0 + j;
-                if (!(ok = warp_wait(&s_full[w], (uint32_t)((g >> 1) & 1), abort_flag))) break;
-                tc_fence_after();
-                float x[64];
+        // the unit whose result is still in TMEM: its number and geometry, the buffer of its last tile
+        int d_lt = -1, d_last = 0, d_nt = 0, d_h = 0, d_shift = 0;
+        int64_t d_tok = 0;
+        auto drain = [&]() -> bool {
+            const float2* sums = fin + (d_lt & 1) * (NB * 128);
+            if (!warp_wait(&fin_bar[(d_lt & 1) * 4 + q], (uint32_t)((d_lt >> 1) & 1), abort_flag)) return false;
+            // the row's sums, moved to the last tile's reference, the last tile's buffer first (which buffer that is
+            // differs with the units a CTA has had before, the order of the sum does not)
+            const float m = sums[d_last * 128 + row].x;
+            float sum = 0.0f;
 #pragma unroll
-                for (int cc = 0; cc < 2; ++cc)
-                    tmem_ld32(s_tmem + (uint32_t)(cc * 32), *reinterpret_cast<uint32_t(*)[32]>(&x[cc * 32]));
-                tmem_ld_wait();
-                if (args.sign != 1.0f) {
-#pragma unroll
-                    for (int e = 0; e < 64; ++e) x[e] *= args.sign;
-                }
-                if (j == un.i) {
-#pragma unroll
-                    for (int e = 0; e < 64; ++e)
-                        if (hf * 64 + e > row || hf * 64 + e < shift) x[e] = -INFINITY;
-                }
-                // a NaN score makes the maximum NaN, and with it the row
-                float mx[4] = {x[0], x[1], x[2], x[3]};
-#pragma unroll
-                for (int e = 4; e < 64; ++e) mx[e & 3] = max_nan(mx[e & 3], x[e]);
-                float top = max_nan(max_nan(mx[0], mx[1]), max_nan(mx[2], mx[3])) * args.sl2;
-                part[(w * 2 + hf) * 128 + row] = top;
+            for (int back = 0, b = d_last; back < NB; ++back) {
+                // a buffer that had no tile of the unit holds nothing of it
+                const float2 s = sums[b * 128 + row];
+                if (back < d_nt) sum = back == 0 ? s.y : fmaf(s.y, ex2_ftz(s.x - m), sum);
+                b = b == 0 ? NB - 1 : b - 1;
+            }
+            if (!warp_wait(o_full, (uint32_t)(d_lt & 1), abort_flag)) return false;
+            tc_fence_after();
+            if (w == 0 && row >= d_shift) args.lse[d_h * args.ld_lse + d_tok] = fmaf(m, kLn2, logf(sum));
+            const float inv = 1.0f / sum;
+            __nv_bfloat16* op = args.o + d_tok * args.o_tok + d_h * args.o_head;
+#pragma unroll 1
+            for (int cc = w; cc < D / 32; cc += NB) {
+                uint32_t r[32];
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&part_bar[w * 4 + q]);
-                if (!(ok = warp_wait(&part_bar[w * 4 + q], (uint32_t)((g >> 1) & 1), abort_flag))) break;
-                top = max_nan(top, part[(w * 2 + (hf ^ 1)) * 128 + row]);
+                tmem_ld32(o_tmem + (uint32_t)(cc * 32), r);
+                tmem_ld_wait();
+                if (row >= d_shift) store_row32(op + cc * 32, r, inv);
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(o_empty);
+            d_lt = -1;
+            return true;
+        };
+        for (int u = blockIdx.x, lt = 0; ok && u >= 0; u = ok ? queue.next(lt) : -1, ++lt) {
+            const Unit un = unit_geom(args.blocks, args.Hq, u);
+            const int shift = kBlk - un.n, nt = un.i + 1;
+            float m = 0.0f, l = 0.0f;  // the reference of this warpgroup's last tile, its tiles' sum relative to it
+            int j = turn;
+            for (; j < nt; j += NB) {
+                if (!(ok = warp_wait(&s_full[w], phase, abort_flag))) break;
+                tc_fence_after();
+                const bool diag = j == un.i;
+                float mx[2] = {-INFINITY, -INFINITY};
+#pragma unroll 1
+                for (int cc = 0; cc < 4; ++cc) {
+                    float x[32];
+                    tmem_ld32(s_tmem + (uint32_t)(cc * 32), *reinterpret_cast<uint32_t(*)[32]>(&x[0]));
+                    tmem_ld_wait();
+                    if (args.sign != 1.0f) {
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) x[e] *= args.sign;
+                    }
+                    if (diag) {
+#pragma unroll
+                        for (int e = 0; e < 32; ++e)
+                            if (cc * 32 + e > row || cc * 32 + e < shift) x[e] = -INFINITY;
+                    }
+                    // a NaN score makes the maximum NaN, and with it the row
+#pragma unroll
+                    for (int e = 0; e < 32; e += 4) {
+                        mx[0] = max3_nan(mx[0], x[e], x[e + 1]);
+                        mx[1] = max3_nan(mx[1], x[e + 2], x[e + 3]);
+                    }
+                }
+                const float top = max3_nan(mx[0], mx[1], mx[1]) * args.sl2;
                 float mn;
                 if (j == 0) {
                     mn = top == -INFINITY ? 0.0f : top;  // a row of nothing visible (or of -inf scores) sums to 0
                 } else {
-                    if (!(ok = warp_wait(&max_bar[(w ^ 1) * 4 + q], (uint32_t)(((g - 1) >> 1) & 1), abort_flag))) break;
-                    const float mp = ref_m[(w ^ 1) * 128 + row];
+                    // the last unit's result before any wait on this unit's tiles: their first P V waits for its drain
+                    if (d_lt >= 0 && !(ok = drain())) break;
+                    // the tile before this one is of the same turn of the buffers, or (buffer 0) of the last
+                    if (!(ok = warp_wait(&max_bar[prev * 4 + q], w == 0 ? phase ^ 1u : phase, abort_flag))) break;
+                    const float mp = ref_m[prev * 128 + row];
                     mn = top <= mp + kLazy ? mp : top;
                     if (__any_sync(0xFFFFFFFFu, mn != mp)) {
-                        // O still holds sums relative to mp: wait for the last P V, then move this thread's half to mn
-                        if (!(ok = warp_wait(&pv_done[(g - 1) & 1], (uint32_t)(((g - 1) >> 1) & 1), abort_flag))) break;
+                        // O still holds sums relative to mp: wait for the last P V, then move it to mn
+                        if (!(ok = warp_wait(&pv_done[prev], w == 0 ? phase ^ 1u : phase, abort_flag))) break;
                         tc_fence_after();
                         const float f = ex2_ftz(mp - mn);
 #pragma unroll 1
                         for (int cc = 0; cc < D / 32; ++cc) {
-                            uint32_t r[16];
-                            tmem_ld16(o_tmem + (uint32_t)(hf * (D / 2) + cc * 16), r);
+                            uint32_t r[32];
+                            tmem_ld32(o_tmem + (uint32_t)(cc * 32), r);
                             tmem_ld_wait();
 #pragma unroll
-                            for (int e = 0; e < 16; ++e) r[e] = __float_as_uint(__uint_as_float(r[e]) * f);
-                            tmem_st16(o_tmem + (uint32_t)(hf * (D / 2) + cc * 16), r);
+                            for (int e = 0; e < 32; ++e) r[e] = __float_as_uint(__uint_as_float(r[e]) * f);
+                            tmem_st32(o_tmem + (uint32_t)(cc * 32), r);
                         }
                     }
                 }
-                if (hf == 0) ref_m[w * 128 + row] = mn;
+                ref_m[w * 128 + row] = mn;
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&max_bar[w * 4 + q]);
-                if (j >= 2) l *= ex2_ftz(m - mn);
+                if (j >= NB) l *= ex2_ftz(m - mn);
                 m = mn;
                 float2 s[2] = {both(0.0f), both(0.0f)};
-                uint32_t pk[32];
-                const float2 sl2 = both(args.sl2), off = both(-m);
+                const float2 sl2 = both(args.sl2 * args.sign), off = both(-m);
+#pragma unroll 1
+                for (int cc = 0; cc < 4; ++cc) {
+                    float x[32];
+                    uint32_t pk[16];
+                    tmem_ld32(s_tmem + (uint32_t)(cc * 32), *reinterpret_cast<uint32_t(*)[32]>(&x[0]));
+                    tmem_ld_wait();
 #pragma unroll
-                for (int e = 0; e < 32; ++e) {
-                    const float2 y = fma2(make_float2(x[2 * e], x[2 * e + 1]), sl2, off);
-                    const float2 p2 = make_float2(ex2_ftz(y.x), ex2_ftz(y.y));
-                    s[e & 1] = add2(s[e & 1], p2);
-                    pk[e] = pack_bf16(p2.x, p2.y);
+                    for (int e = 0; e < 16; ++e) {
+                        const float2 y = fma2(make_float2(x[2 * e], x[2 * e + 1]), sl2, off);
+                        x[2 * e] = ex2_ftz(y.x);
+                        x[2 * e + 1] = ex2_ftz(y.y);
+                    }
+                    if (diag) {
+#pragma unroll
+                        for (int e = 0; e < 32; ++e)
+                            if (cc * 32 + e > row || cc * 32 + e < shift) x[e] = 0.0f;
+                    }
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        s[e & 1] = add2(s[e & 1], make_float2(x[2 * e], x[2 * e + 1]));
+                        pk[e] = pack_bf16(x[2 * e], x[2 * e + 1]);
+                    }
+                    // over columns this thread has read: 32 scores become 16 columns
+                    tmem_st16(s_tmem + (uint32_t)(cc * 16), pk);
+                    if (cc & 1) {
+                        tmem_st_wait();
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(&p_full[2 * w + (cc >> 1)]);
+                    }
                 }
-                tmem_st32(s_tmem, pk);
-                tmem_st_wait();
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&p_full[w]);
                 l += (s[0].x + s[0].y) + (s[1].x + s[1].y);
+                phase ^= 1u;
+                if (d_lt >= 0 && !(ok = drain())) break;
             }
             if (!ok) break;
-            // the row's four sums, moved to the last tile's reference
-            float2* mine = fin + (lt & 1) * 512;
-            mine[wg * 128 + row] = make_float2(m, l);
+            turn = j - nt;
+            if (d_lt >= 0 && !(ok = drain())) break;  // a unit without a tile of this warpgroup
+            fin[(lt & 1) * (NB * 128) + w * 128 + row] = make_float2(m, l);
             __syncwarp();
             if (lane == 0) mbar_arrive(&fin_bar[(lt & 1) * 4 + q]);
-            if (!(ok = warp_wait(&fin_bar[(lt & 1) * 4 + q], (uint32_t)((lt >> 1) & 1), abort_flag))) break;
-            const int wl = (g0 + nt - 1) & 1;  // the last tile's parity
-            const float2 last = mine[wl * 256 + row], other = mine[(wl ^ 1) * 256 + row];
-            float sum = last.y + mine[wl * 256 + 128 + row].y;
-            if (nt > 1) sum = fmaf(other.y + mine[(wl ^ 1) * 256 + 128 + row].y, ex2_ftz(other.x - last.x), sum);
-            if (!(ok = warp_wait(&o_full[ob], (uint32_t)((lt / C::kORing) & 1), abort_flag))) break;
-            tc_fence_after();
-            const int64_t tok = un.tok0 + row - shift;
-            if (wg == 0 && row >= shift) args.lse[un.h * args.ld_lse + tok] = fmaf(last.x, kLn2, logf(sum));
-            const float inv = 1.0f / sum;
-            __nv_bfloat16* op = args.o + tok * args.o_tok + un.h * args.o_head + wg * (D / 4);
-#pragma unroll 1
-            for (int cc = 0; cc < D / 128; ++cc) {
-                uint32_t r[32];
-                __syncwarp();
-                tmem_ld32(o_tmem + (uint32_t)(wg * (D / 4) + cc * 32), r);
-                tmem_ld_wait();
-                if (row >= shift) store_row32(op + cc * 32, r, inv);
-            }
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&o_empty[ob]);
-            g0 += nt;
-            ++lt;
+            d_lt = lt, d_nt = nt, d_h = un.h, d_shift = shift;
+            d_tok = (int64_t)un.tok0 + row - shift;
+            // the last tile's buffer: this warpgroup's next tile is `turn` tiles into the next unit
+            d_last = w - turn - 1;
+            if (d_last < 0) d_last += NB;
         }
+        if (ok && d_lt >= 0) ok = drain();
         if (!ok) *abort_flag = 1;
     }
 
@@ -491,12 +558,12 @@ int launch_fwd(const R97bPacked& p, const R97bAttnPackedFwd& a, cudaStream_t st)
     r.o = reinterpret_cast<__nv_bfloat16*>(a.o.ptr);
     r.lse = a.lse;
     r.o_tok = a.o.tok, r.o_head = a.o.head, r.ld_lse = a.ld_lse;
-    r.Hq = a.Hq, r.grp = a.Hq / a.Hkv, r.units = p.n_blocks * a.Hq;
+    r.Hq = a.Hq, r.grp = a.Hq / a.Hkv;
     r.q_head = (int32_t)a.q.head, r.k_head = (int32_t)a.k.head, r.v_head = (int32_t)a.v.head;
     r.sl2 = a.scale == 0.0f ? 1.0f : fabsf(a.scale) * kLog2e;
     r.sign = a.scale == 0.0f ? 0.0f : (a.scale < 0.0f ? -1.0f : 1.0f);
     if (!smem_opt_in(fwd_kernel<D>, C::kSmemBytes)) return R97B_ELAUNCH;
-    fwd_kernel<D><<<min(num_sms(), r.units), kThreads, C::kSmemBytes, st>>>(q, k, v, r);
+    fwd_kernel<D><<<p.n_blocks * a.Hq, C::kThreads, C::kSmemBytes, st>>>(q, k, v, r);
     return launch_status();
 }
 
@@ -518,6 +585,11 @@ int launch_fwd(const R97bPacked& p, const R97bAttnPackedFwd& a, cudaStream_t st)
 // beside them, and only dS (a product and a rounding) stands between dP and the products that read it.
 enum Kind { kDQ = 0, kDKV = 1, kDV = 2, kDK = 3 };
 
+constexpr int kThreads = 640;  // warps 0, 3: TMA, warp 1: MMA, warp 2: the columns' statistics; four warpgroups after
+constexpr int kSoftWarps = 16;
+constexpr int kCtrlRegs = 64, kSoftRegs = 104;  // 128 x 64 + 512 x 104 = 640 x 96, what the launch holds
+static_assert(128 * kCtrlRegs + 512 * kSoftRegs <= 640 * 96, "register split");
+
 template <int D, int KIND>
 struct BCfg {
     static constexpr bool kDP = KIND != kDV;          // needs dP (a second resident operand, delta)
@@ -526,7 +598,7 @@ struct BCfg {
     static constexpr int kStages = D == 256 && kDP ? 6 : 9;
     static constexpr int kRingOff = (kDP ? 2 : 1) * kABytes;
     static constexpr int kBarOff = kRingOff + kStages * kChunk;
-    static constexpr int kStatOff = kBarOff + 512;    // kKeys: float [2 (stage)][-lse log2 e, -delta][128]
+    static constexpr int kStatOff = kBarOff + 640;    // kKeys: float [2 (stage)][-lse log2 e, -delta][128]
     static constexpr int kSmemBytes = kStatOff + (kKeys ? 2048 : 0);
     static constexpr int kVRows = kChunk / (D * 2);
 };
@@ -539,7 +611,7 @@ struct BwdArgs {
     __nv_bfloat16 *out0, *out1;        // kDQ: dq; kDKV: dv, dk; kDV: dv; kDK: dk
     int64_t tok0, head0, tok1, head1;
     int32_t a0_head, a1_head, b0_head, b1_head, c0_head, c1_head;
-    int32_t heads, grp, units;         // the rows' heads (query heads for kDQ, key/value heads else)
+    int32_t heads, grp;                // the rows' heads (query heads for kDQ, key/value heads else)
     float sl2, scale;
 };
 
@@ -574,9 +646,15 @@ __global__ void __launch_bounds__(kThreads, 1)
     using C = BCfg<D, KIND>;
     constexpr int ND = D / 64;
     constexpr int kVC = kBlk / C::kVRows;
+    constexpr int kUnrollChunks = D == 128 ? 2 : 1, kUnrollStreams = D == 128 ? 4 : 1;
     extern __shared__ __align__(1024) uint8_t smem[];
     uint8_t* ring = smem + C::kRingOff;
     uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + C::kBarOff);
+    const UnitQueue queue{reinterpret_cast<uint4*>(full_bar), full_bar + 8, full_bar + 12,
+                          reinterpret_cast<volatile int*>(full_bar + 16)};
+    volatile int* abort_flag = queue.abort;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(full_bar + 16) + 1;
+    full_bar += 17;
     uint64_t* empty_bar = full_bar + C::kStages;
     uint64_t* a_full = empty_bar + C::kStages;   // [2]
     uint64_t* a_empty = a_full + 2;              // [2]
@@ -589,8 +667,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint64_t* acc_empty = acc_full + 1;
     uint64_t* stat_full = acc_empty + 1;         // [2]
     uint64_t* stat_empty = stat_full + 2;        // [2]
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(stat_empty + 2);
-    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
     float* stats = reinterpret_cast<float*>(smem + C::kStatOff);
 
     const int warp = __shfl_sync(0xFFFFFFFFu, threadIdx.x >> 5, 0);
@@ -600,6 +676,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         return;
     }
     if (threadIdx.x == 0) {
+        queue.init((C::kKeys ? 4 : 3) + kSoftWarps);
         for (int s = 0; s < C::kStages; ++s) {
             mbar_init(&full_bar[s], 1);
             mbar_init(&empty_bar[s], 1);
@@ -639,7 +716,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     tc_fence_after();
     const uint32_t tmem = __shfl_sync(0xFFFFFFFFu, *tmem_slot, 0);
     const uint32_t acc0 = tmem + 256u, acc1 = tmem + 384u;  // acc1: kDKV's dK
-    const int G = gridDim.x, c = blockIdx.x;
 
     if (warp < 4) {
         set_max_regs_dec<kCtrlRegs>();
@@ -647,12 +723,10 @@ __global__ void __launch_bounds__(kThreads, 1)
             // --------------------------------------------------------- TMA producers: every other chunk each
             const uint32_t lead = elect_one();
             const int p = warp == 3;
-            int stage = p, lt = 0;
+            int stage = p;
             uint32_t phase = 0;
             bool ok = true;
-            for (int t = 0; ok && t * G < args.units; ++t) {
-                const int u = unit_of(t, c, G);
-                if (u >= args.units) continue;
+            for (int u = blockIdx.x, lt = 0; ok && u >= 0; u = ok ? queue.next(lt) : -1, ++lt) {
                 const Walk<KIND> wk(args, u);
                 if (p == 0 || C::kDP) {  // a resident operand each
                     if (!(ok = warp_wait(&a_empty[p], (uint32_t)(lt & 1) ^ 1u, abort_flag))) break;
@@ -663,48 +737,51 @@ __global__ void __launch_bounds__(kThreads, 1)
                                         wk.h * (p ? args.a1_head : args.a0_head) + 64 * s, -wk.shift(), wk.tok0);
                     }
                 }
-                // a column block K-major (the score products), or MN-major (the accumulating ones)
-                auto load = [&](const CUtensorMap* map, bool mn, int head_stride, int tile) {
-                    const int blk = wk.block(tile), x = wk.head(tile) * head_stride;
-                    const int r0 = -wk.shift_of(blk), tok = wk.seq0 + blk * kBlk;
+                // a step's streams, in the order the products take them: the next tile's column block for S (K-major), this
+                // tile's for the accumulating products (MN-major), the next tile's for dP. Rolled at D = 256: the warps
+                // share an instruction cache that unrolled copies do not fit in beside the softmax.
+#pragma unroll 1
+                for (int j = -1; j < wk.tiles && ok; ++j) {
+                    if (p && j + 1 == wk.tiles && !(ok = queue.ask(lt, lead))) break;
+#pragma unroll kUnrollStreams
+                    for (int s = 0; s < 4 && ok; ++s) {
+                        const bool mn = s == 1 || s == 2;
+                        const int tile = mn ? j : j + 1;
+                        if (tile < 0 || tile >= wk.tiles || (s == 2 && KIND != kDKV) || (s == 3 && !C::kDP)) continue;
+                        const CUtensorMap* map = s == 0 ? &tB0 : (s == 1 ? &tC0 : (s == 2 ? &tC1 : &tB1));
+                        const int head_stride =
+                            s == 0 ? args.b0_head : (s == 1 ? args.c0_head : (s == 2 ? args.c1_head : args.b1_head));
+                        const int blk = wk.block(tile), x = wk.head(tile) * head_stride;
+                        const int r0 = -wk.shift_of(blk), tok = wk.seq0 + blk * kBlk;
+#pragma unroll kUnrollChunks
+                        for (int ch = p; ch < (mn ? kVC : ND); ch += 2) {
+                            if (!(ok = warp_wait(&empty_bar[stage], phase ^ 1u, abort_flag))) break;
+                            if (lead) {
+                                uint8_t* st = ring + stage * kChunk;
+                                mbar_expect_tx(&full_bar[stage], kChunk);
+                                if (mn) {
 #pragma unroll
-                    for (int ch = p; ch < (mn ? kVC : ND); ch += 2) {
-                        if (!(ok = ok && warp_wait(&empty_bar[stage], phase ^ 1u, abort_flag))) return;
-                        if (lead) {
-                            uint8_t* st = ring + stage * kChunk;
-                            mbar_expect_tx(&full_bar[stage], kChunk);
-                            if (mn) {
-#pragma unroll
-                                for (int n = 0; n < ND; ++n)
-                                    tma_load_3d(st + n * (C::kVRows * 128), map, &full_bar[stage], x + 64 * n,
-                                                ch * C::kVRows + r0, tok);
-                            } else {
-                                tma_load_3d(st, map, &full_bar[stage], x + 64 * ch, r0, tok);
+                                    for (int n = 0; n < ND; ++n)
+                                        tma_load_3d(st + n * (C::kVRows * 128), map, &full_bar[stage], x + 64 * n,
+                                                    ch * C::kVRows + r0, tok);
+                                } else {
+                                    tma_load_3d(st, map, &full_bar[stage], x + 64 * ch, r0, tok);
+                                }
+                            }
+                            if ((stage += 2) >= C::kStages) {
+                                stage -= C::kStages;
+                                phase ^= 1u;
                             }
                         }
-                        if ((stage += 2) >= C::kStages) {
-                            stage -= C::kStages;
-                            phase ^= 1u;
-                        }
                     }
-                };
-                load(&tB0, false, args.b0_head, 0);
-                if (C::kDP) load(&tB1, false, args.b1_head, 0);
-                for (int j = 0; j < wk.tiles && ok; ++j) {
-                    const bool more = j + 1 < wk.tiles;
-                    if (more) load(&tB0, false, args.b0_head, j + 1);
-                    load(&tC0, true, args.c0_head, j);
-                    if (KIND == kDKV) load(&tC1, true, args.c1_head, j);
-                    if (more && C::kDP) load(&tB1, false, args.b1_head, j + 1);
                 }
-                ++lt;
             }
         } else if (warp == 1) {
             const uint32_t lead = elect_one();
             // --------------------------------------------------------- MMA issuer
             constexpr uint32_t idesc_s = make_idesc_bf16(kBlk, kBlk, 0, 0);
             constexpr uint32_t idesc_c = make_idesc_bf16(kBlk, D, 0, 1);
-            int stage = 0, lt = 0, g = 0;  // g: the current unit's first tile
+            int stage = 0, g = 0;  // g: the current unit's first tile
             uint32_t phase = 0;
             bool ok = true;
             const uint32_t a_lo = sdesc_lo(smem_u32(smem), 16);
@@ -722,6 +799,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
             };
             auto score = [&](int resident, uint32_t d) {
+#pragma unroll kUnrollChunks
                 for (int kb = 0; kb < ND; ++kb) {
                     if (!chunk()) return;
                     const uint32_t a = a_lo + (uint32_t)(resident * (C::kABytes >> 4) + kb * kChunkLo);
@@ -734,6 +812,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
             };
             auto accumulate = [&](uint32_t a, uint32_t d, bool first) {
+#pragma unroll kUnrollChunks
                 for (int ch = 0; ch < kVC; ++ch) {
                     if (!chunk()) return;
                     const uint32_t b = c_lo + (uint32_t)(stage * kChunkLo);
@@ -749,9 +828,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 ok = ok && warp_wait(bar, (uint32_t)(n & 1), abort_flag);
                 tc_fence_after();
             };
-            for (int t = 0; ok && t * G < args.units; ++t) {
-                const int u = unit_of(t, c, G);
-                if (u >= args.units) continue;
+            for (int u = blockIdx.x, lt = 0; ok && u >= 0; u = ok ? queue.next(lt) : -1, ++lt) {
                 const Walk<KIND> wk(args, u);
                 const int n = wk.tiles;
                 auto issue_s = [&](int j) {
@@ -770,35 +847,32 @@ __global__ void __launch_bounds__(kThreads, 1)
                     umma_commit_by(lead, dp_full);
                     if (j + 1 == n) umma_commit_by(lead, &a_empty[1]);
                 };
-                issue_s(0);
-                if (C::kDP) issue_dp(0);
-                for (int j = 0; j < n && ok; ++j) {
-                    const int gj = g + j;
+#pragma unroll 1
+                for (int j = -1; j < n && ok; ++j) {
+                    const int gj = g + j, b = KIND == kDV ? (gj & 1) : 0;
                     const bool more = j + 1 < n;
                     if (more) issue_s(j + 1);
-                    const int b = KIND == kDV ? (gj & 1) : 0;
-                    if (KIND == kDV)
-                        wait(&p_full[b], gj >> 1);
-                    else
-                        wait(ds_full, gj);
-                    if (j == 0) wait(acc_empty, lt + 1);
-                    if (!ok) break;
-                    accumulate(tmem + (uint32_t)(KIND == kDV ? b * kBlk : kBlk), acc0, j == 0);
-                    if (KIND == kDKV) accumulate(tmem + (uint32_t)(kBlk + 16), acc1, j == 0);
+                    if (j >= 0) {
+                        if (KIND == kDV)
+                            wait(&p_full[b], gj >> 1);
+                        else
+                            wait(ds_full, gj);
+                        if (j == 0) wait(acc_empty, lt + 1);
+                        if (!ok) break;
+                        accumulate(tmem + (uint32_t)(KIND == kDV ? b * kBlk : kBlk), acc0, j == 0);
+                        if (KIND == kDKV) accumulate(tmem + (uint32_t)(kBlk + 16), acc1, j == 0);
+                    }
                     if (more && C::kDP) issue_dp(j + 1);
                 }
                 if (!ok) break;
                 umma_commit_by(lead, acc_full);
                 g += n;
-                ++lt;
             }
         } else if (C::kKeys && warp == 2) {
             // --------------------------------------------------------- the columns' lse and delta, a tile ahead
             int g = 0;
             bool ok = true;
-            for (int t = 0; ok && t * G < args.units; ++t) {
-                const int u = unit_of(t, c, G);
-                if (u >= args.units) continue;
+            for (int u = blockIdx.x, lt = 0; ok && u >= 0; u = ok ? queue.next(lt) : -1, ++lt) {
                 const Walk<KIND> wk(args, u);
                 for (int j = 0; j < wk.tiles; ++j, ++g) {
                     const int blk = wk.block(j), shift = wk.shift_of(blk), h = wk.head(j), st = g & 1;
@@ -827,11 +901,37 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int row = q * 32 + lane;
         const uint32_t lane_off = (uint32_t)(q * 32) << 16;
         const uint32_t mine = tmem + lane_off + (uint32_t)(w * 32);  // this thread's columns of S (and, 128 on, of dP)
-        int g = 0, lt = 0;
+        int g = 0;
         bool ok = true;
-        for (int t = 0; ok && t * G < args.units; ++t) {
-            const int u = unit_of(t, c, G);
-            if (u >= args.units) continue;
+        // the unit whose result is still in TMEM: its number, head, first valid row, and this row's token
+        int d_lt = -1, d_h = 0, d_shift = 0;
+        int64_t d_tok = 0;
+        auto drain = [&]() -> bool {
+            if (!warp_wait(acc_full, (uint32_t)(d_lt & 1), abort_flag)) return false;
+            tc_fence_after();
+#pragma unroll
+            for (int r = 0; r < (KIND == kDKV ? 2 : 1); ++r) {
+                // dV takes no scale; dS is kept unscaled in bf16, so dQ and dK take it here
+                const float f = (KIND == kDV || (KIND == kDKV && r == 0)) ? 1.0f : args.scale;
+                __nv_bfloat16* op = r ? args.out1 + d_tok * args.tok1 + d_h * args.head1
+                                      : args.out0 + d_tok * args.tok0 + d_h * args.head0;
+                const uint32_t src = (r ? acc1 : acc0) + lane_off + (uint32_t)(w * (D / 4));
+#pragma unroll 1
+                for (int cc = 0; cc < D / 128; ++cc) {
+                    uint32_t v[32];
+                    __syncwarp();
+                    tmem_ld32(src + (uint32_t)(cc * 32), v);
+                    tmem_ld_wait();
+                    if (row >= d_shift) store_row32(op + w * (D / 4) + cc * 32, v, f);
+                }
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(acc_empty);
+            d_lt = -1;
+            return true;
+        };
+        for (int u = blockIdx.x, lt = 0; ok && u >= 0; u = ok ? queue.next(lt) : -1, ++lt) {
             const Walk<KIND> wk(args, u);
             const int shift = wk.shift();
             const int64_t tok = (int64_t)wk.tok0 + row - shift;
@@ -908,31 +1008,13 @@ __global__ void __launch_bounds__(kThreads, 1)
                     if (lane == 0) mbar_arrive(ds_full);
                 }
                 if (C::kKeys && lane == 0) mbar_arrive(&stat_empty[g & 1]);
+                // the last unit's result, now that the tensor core has this unit's first products to go on with
+                if (d_lt >= 0 && !(ok = drain())) break;
             }
             if (!ok) break;
-            if (!(ok = warp_wait(acc_full, (uint32_t)(lt & 1), abort_flag))) break;
-            tc_fence_after();
-#pragma unroll
-            for (int r = 0; r < (KIND == kDKV ? 2 : 1); ++r) {
-                // dV takes no scale; dS is kept unscaled in bf16, so dQ and dK take it here
-                const float f = (KIND == kDV || (KIND == kDKV && r == 0)) ? 1.0f : args.scale;
-                __nv_bfloat16* op = r ? args.out1 + tok * args.tok1 + wk.h * args.head1
-                                      : args.out0 + tok * args.tok0 + wk.h * args.head0;
-                const uint32_t src = (r ? acc1 : acc0) + lane_off + (uint32_t)(w * (D / 4));
-#pragma unroll 1
-                for (int cc = 0; cc < D / 128; ++cc) {
-                    uint32_t v[32];
-                    __syncwarp();
-                    tmem_ld32(src + (uint32_t)(cc * 32), v);
-                    tmem_ld_wait();
-                    if (row >= shift) store_row32(op + w * (D / 4) + cc * 32, v, f);
-                }
-            }
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(acc_empty);
-            ++lt;
+            d_lt = lt, d_h = wk.h, d_shift = shift, d_tok = tok;
         }
+        if (ok && d_lt >= 0) ok = drain();
         if (!ok) *abort_flag = 1;
     }
 
@@ -1002,10 +1084,10 @@ int launch_bwd(const R97bPacked& p, const R97bAttnPackedBwd& a, const float* del
     r.out1 = reinterpret_cast<__nv_bfloat16*>(o1.ptr), r.tok1 = o1.tok, r.head1 = o1.head;
     r.a0_head = (int32_t)a0.head, r.a1_head = (int32_t)a1.head, r.b0_head = (int32_t)b0.head, r.b1_head = (int32_t)b1.head;
     r.c0_head = (int32_t)c0.head, r.c1_head = (int32_t)c1.head;
-    r.heads = ha, r.grp = a.Hq / a.Hkv, r.units = p.n_blocks * ha;
+    r.heads = ha, r.grp = a.Hq / a.Hkv;
     r.sl2 = a.scale * kLog2e, r.scale = a.scale;
     if (!smem_opt_in(bwd_kernel<D, KIND>, C::kSmemBytes)) return R97B_ELAUNCH;
-    bwd_kernel<D, KIND><<<min(num_sms(), r.units), kThreads, C::kSmemBytes, st>>>(m[0], m[1], m[2], m[3], m[4], m[5], r);
+    bwd_kernel<D, KIND><<<p.n_blocks * ha, kThreads, C::kSmemBytes, st>>>(m[0], m[1], m[2], m[3], m[4], m[5], r);
     return launch_status();
 }
 

@@ -164,6 +164,36 @@ __device__ __forceinline__ void tma_load_2d_pair(void* dst, const CUtensorMap* m
         : "memory");
 }
 
+// ------------------------------------------------------------------------------------ launch control
+
+// Asks the launch for a CTA of this grid that has not started (cancelling it); the 16-byte answer arrives in `slot`,
+// completing `bar`'s transaction bytes.
+__device__ __forceinline__ void launch_cancel(uint4* slot, uint64_t* bar) {
+    asm volatile(
+        "clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(
+            smem_u32(slot)),
+        "r"(smem_u32(bar))
+        : "memory");
+}
+
+// The x index of the CTA an arrived answer cancelled, or -1 when none was left.
+__device__ __forceinline__ int launch_cancelled(const uint4* slot) {
+    int x;
+    asm volatile(
+        "{\n .reg .pred p;\n .reg .b128 h;\n ld.shared.b128 h, [%1];\n"
+        " clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, h;\n mov.b32 %0, -1;\n"
+        " @p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %0, h;\n}\n"
+        : "=r"(x)
+        : "r"(smem_u32(slot))
+        : "memory");
+    return x;
+}
+
+// Orders this thread's generic accesses of shared memory before later asynchronous ones.
+__device__ __forceinline__ void fence_proxy_async_smem() {
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+}
+
 // ------------------------------------------------------------------------------------ tcgen05
 
 __device__ __forceinline__ void tmem_alloc(uint32_t* dst_smem, uint32_t ncols) {
