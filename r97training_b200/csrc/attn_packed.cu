@@ -55,29 +55,6 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volati
     return true;
 }
 
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
-    float2 d;
-    asm("{\n .reg .b64 x, y, z;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n mov.b64 z, {%6, %7};\n"
-        " fma.rn.f32x2 x, x, y, z;\n mov.b64 {%0, %1}, x;\n}\n"
-        : "=f"(d.x), "=f"(d.y)
-        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
-    return d;
-}
-__device__ __forceinline__ float2 add2(float2 a, float2 b) {
-    float2 d;
-    asm("{\n .reg .b64 x, y;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n add.rn.f32x2 x, x, y;\n mov.b64 {%0, %1}, x;\n}\n"
-        : "=f"(d.x), "=f"(d.y)
-        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
-    return d;
-}
-__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
-    float2 d;
-    asm("{\n .reg .b64 x, y;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n mul.rn.f32x2 x, x, y;\n mov.b64 {%0, %1}, x;\n}\n"
-        : "=f"(d.x), "=f"(d.y)
-        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
-    return d;
-}
-__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
     const __nv_bfloat162 b = __floats2bfloat162_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&b);
@@ -633,8 +610,15 @@ struct Walk {
         tiles = KIND == kDQ ? m : m * a.grp;
     }
     __device__ int shift() const { return kBlk - n; }
-    __device__ int block(int t) const { return KIND == kDQ ? t : i + t % m; }           // the tile's column block
-    __device__ int head(int t) const { return KIND == kDQ ? h / grp : h * grp + t / m; }  // and its head
+    // the first tile's column block and head, and the step to the next one's
+    __device__ int first_block() const { return KIND == kDQ ? 0 : i; }
+    __device__ int first_head() const { return KIND == kDQ ? h / grp : h * grp; }
+    __device__ void step(int& blk, int& head) const {
+        if (++blk == i + m && KIND != kDQ) {
+            blk = i;
+            ++head;
+        }
+    }
     __device__ int shift_of(int blk) const { return kBlk - min(kBlk, len - blk * kBlk); }
 };
 
@@ -740,6 +724,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 // a step's streams, in the order the products take them: the next tile's column block for S (K-major), this
                 // tile's for the accumulating products (MN-major), the next tile's for dP. Rolled at D = 256: the warps
                 // share an instruction cache that unrolled copies do not fit in beside the softmax.
+                int blk0 = 0, head0 = 0, blk1 = wk.first_block(), head1 = wk.first_head();  // of tiles j and j + 1
 #pragma unroll 1
                 for (int j = -1; j < wk.tiles && ok; ++j) {
                     if (p && j + 1 == wk.tiles && !(ok = queue.ask(lt, lead))) break;
@@ -751,7 +736,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                         const CUtensorMap* map = s == 0 ? &tB0 : (s == 1 ? &tC0 : (s == 2 ? &tC1 : &tB1));
                         const int head_stride =
                             s == 0 ? args.b0_head : (s == 1 ? args.c0_head : (s == 2 ? args.c1_head : args.b1_head));
-                        const int blk = wk.block(tile), x = wk.head(tile) * head_stride;
+                        const int blk = mn ? blk0 : blk1, x = (mn ? head0 : head1) * head_stride;
                         const int r0 = -wk.shift_of(blk), tok = wk.seq0 + blk * kBlk;
 #pragma unroll kUnrollChunks
                         for (int ch = p; ch < (mn ? kVC : ND); ch += 2) {
@@ -774,6 +759,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                             }
                         }
                     }
+                    blk0 = blk1, head0 = head1;
+                    wk.step(blk1, head1);
                 }
             }
         } else if (warp == 1) {
@@ -847,21 +834,20 @@ __global__ void __launch_bounds__(kThreads, 1)
                     umma_commit_by(lead, dp_full);
                     if (j + 1 == n) umma_commit_by(lead, &a_empty[1]);
                 };
-#pragma unroll 1
-                for (int j = -1; j < n && ok; ++j) {
+                issue_s(0);
+                if (C::kDP) issue_dp(0);
+                for (int j = 0; j < n && ok; ++j) {
                     const int gj = g + j, b = KIND == kDV ? (gj & 1) : 0;
                     const bool more = j + 1 < n;
                     if (more) issue_s(j + 1);
-                    if (j >= 0) {
-                        if (KIND == kDV)
-                            wait(&p_full[b], gj >> 1);
-                        else
-                            wait(ds_full, gj);
-                        if (j == 0) wait(acc_empty, lt + 1);
-                        if (!ok) break;
-                        accumulate(tmem + (uint32_t)(KIND == kDV ? b * kBlk : kBlk), acc0, j == 0);
-                        if (KIND == kDKV) accumulate(tmem + (uint32_t)(kBlk + 16), acc1, j == 0);
-                    }
+                    if (KIND == kDV)
+                        wait(&p_full[b], gj >> 1);
+                    else
+                        wait(ds_full, gj);
+                    if (j == 0) wait(acc_empty, lt + 1);
+                    if (!ok) break;
+                    accumulate(tmem + (uint32_t)(KIND == kDV ? b * kBlk : kBlk), acc0, j == 0);
+                    if (KIND == kDKV) accumulate(tmem + (uint32_t)(kBlk + 16), acc1, j == 0);
                     if (more && C::kDP) issue_dp(j + 1);
                 }
                 if (!ok) break;
@@ -874,8 +860,9 @@ __global__ void __launch_bounds__(kThreads, 1)
             bool ok = true;
             for (int u = blockIdx.x, lt = 0; ok && u >= 0; u = ok ? queue.next(lt) : -1, ++lt) {
                 const Walk<KIND> wk(args, u);
-                for (int j = 0; j < wk.tiles; ++j, ++g) {
-                    const int blk = wk.block(j), shift = wk.shift_of(blk), h = wk.head(j), st = g & 1;
+                int blk = wk.first_block(), h = wk.first_head();
+                for (int j = 0; j < wk.tiles; ++j, ++g, wk.step(blk, h)) {
+                    const int shift = wk.shift_of(blk), st = g & 1;
                     const int64_t tok = (int64_t)wk.seq0 + blk * kBlk - shift;
                     float v[8];
 #pragma unroll

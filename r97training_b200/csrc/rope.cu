@@ -6,11 +6,14 @@
 //   R rotates pair i < rot / 2 of the head, (i, i + rot / 2) or (2 i, 2 i + 1), by pos * inv_i
 //   adjoint: d = R(-pos) dy (the tables' amplitude included), dx = rstd w d - x rstd^3 mean(w d x)
 //
-// Bound by HBM: each row is read once and written once (the adjoint reads x and dy). A warp owns one token and
-// up to kBatch head rows of it at a time, 16 bytes a lane, so the token's cos and sin values are fetched once per
-// batch into registers and all the batch's row loads are in flight together; queries and keys share one launch.
+// Bound by HBM: each row is read once and written once (the adjoint reads x and dy). A lane holds 16 values of a row as
+// two 16-byte chunks that rotate with one another -- in the half layout chunk k and the one rot / 2 after it -- so the
+// rotation needs no exchange between lanes and D / 16 lanes sum the norm. A warp takes kWarpRows rows a lane of one token,
+// queries and keys alike, with the token's cos and sin in registers; what hides the loads is the number of warps, so the
+// gain is read again (from L1) for every row rather than held.
 #include "sm100.cuh"
 #include "r97b_internal.h"
+#include "fastmath.cuh"
 
 #include <cuda_bf16.h>
 #include <math.h>
@@ -21,7 +24,13 @@ R97B_ERROR_READER(rope_error_word)
 
 namespace {
 
-constexpr int kBatch = 4;  // row loads a lane has in flight (two a row in the adjoint)
+constexpr int kBlockThreads = 128;
+// Rows a lane takes in turn, and the blocks an SM holds (what their registers, 70 and 80 a thread, then may be): measured at
+// 8192 tokens of 16 + 4 heads of 256 (forward / adjoint) and the adjoint of 32749 tokens, 16 + 4 heads of 128, rotated
+// whole: 5 rows at 7 / 6 blocks 39.7 / 54.8 / 101 us; 10 rows at 8 / 6 41.8 / 56.8 / 102; 4 rows at 8 / 6 44.4 / 60.4 / 121;
+// 10 / 8 blocks (spills) 70 / 82 / 141. The copy-rate times of the same bytes are 25.9 / 38.7 / 79.6 us.
+constexpr int kWarpRows = 5;
+constexpr int kFwdBlocks = 7, kBwdBlocks = 6;
 
 struct RopeArgs {
     R97bRopePart part[2];
@@ -33,154 +42,138 @@ struct RopeArgs {
     float eps;
 };
 
-__device__ __forceinline__ uint4 ld_row(const R97bHeadRows& r, int64_t t, int h, int e) {
-    return *reinterpret_cast<const uint4*>(reinterpret_cast<const __nv_bfloat16*>(r.ptr) + t * r.tok + h * r.head + e);
+struct Row16 {  // a lane's two chunks of a row
+    uint4 a, b;
+};
+__device__ __forceinline__ Row16 ld_row(const R97bHeadRows& r, int64_t t, int h, int ea, int eb) {
+    const __nv_bfloat16* p = reinterpret_cast<const __nv_bfloat16*>(r.ptr) + t * r.tok + h * r.head;
+    return Row16{*reinterpret_cast<const uint4*>(p + ea), *reinterpret_cast<const uint4*>(p + eb)};
 }
-__device__ __forceinline__ void unpack8(const uint4& u, float (&v)[8]) {
+__device__ __forceinline__ void unpack8(const uint4& u, float2* v) {
     const __nv_bfloat162* p = reinterpret_cast<const __nv_bfloat162*>(&u);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const float2 f = __bfloat1622float2(p[i]);
-        v[2 * i] = f.x;
-        v[2 * i + 1] = f.y;
-    }
+    for (int i = 0; i < 4; ++i) v[i] = __bfloat1622float2(p[i]);
 }
-__device__ __forceinline__ void st_row(const R97bHeadRows& r, int64_t t, int h, int e, const float (&v)[8]) {
+__device__ __forceinline__ uint4 pack8(const float2* v) {
     uint4 u;
     __nv_bfloat162* p = reinterpret_cast<__nv_bfloat162*>(&u);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) p[i] = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
-    *reinterpret_cast<uint4*>(reinterpret_cast<__nv_bfloat16*>(r.ptr) + t * r.tok + h * r.head + e) = u;
+    for (int i = 0; i < 4; ++i) p[i] = __floats2bfloat162_rn(v[i].x, v[i].y);
+    return u;
 }
-
-// Rotates the lane's 8 values by the pairs' (cos, sin); sign -1 is the inverse rotation. `src` is the lane that
-// holds the partners of a half-layout lane, `lead` whether this lane holds the pairs' first members.
-template <bool INTER>
-__device__ __forceinline__ void rotate8(float (&v)[8], const float (&cs)[8], const float (&sn)[8], bool in_rot, bool lead,
-                                        int src, float sign) {
-    if (INTER) {
-        if (in_rot) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float a = v[2 * i], b = v[2 * i + 1], s = sign * sn[i];
-                v[2 * i] = a * cs[i] - b * s;
-                v[2 * i + 1] = b * cs[i] + a * s;
-            }
-        }
-    } else {
-        const float sg = lead ? -sign : sign;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const float o = __shfl_sync(0xFFFFFFFFu, v[i], src);  // every lane joins
-            if (in_rot) v[i] = v[i] * cs[i] + sg * o * sn[i];
-        }
-    }
+__device__ __forceinline__ void ld8f(const float* p, float2* v) {
+    const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
+    v[0] = make_float2(a.x, a.y), v[1] = make_float2(a.z, a.w), v[2] = make_float2(b.x, b.y), v[3] = make_float2(b.z, b.w);
 }
 
 template <int D, bool INTER, bool BACK>
-__global__ void __launch_bounds__(256) qk_rope_kernel(const __grid_constant__ RopeArgs a) {
-    constexpr int kLanes = D / 8;          // lanes of one row
+__global__ void __launch_bounds__(kBlockThreads, BACK ? kBwdBlocks : kFwdBlocks) qk_rope_kernel(const __grid_constant__ RopeArgs a) {
+    constexpr int kLanes = D / 16;         // lanes of one row
     constexpr int kRows = 32 / kLanes;     // rows a warp covers at once
     const int64_t unit = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) >> 5;
     if (unit >= a.units) return;
     const int64_t t = a.chunks == 1 ? unit : unit / a.chunks;
-    const int h0 = (int)(unit - t * a.chunks) * (kBatch * kRows);
-    const int lane = threadIdx.x & 31, l = lane & (kLanes - 1), e = 8 * l;
+    const int lane = threadIdx.x & 31, l = lane & (kLanes - 1);
     const int heads0 = (int)a.part[0].heads;
-
-    int head[kBatch];
-    bool live[kBatch], second[kBatch];
-    uint4 rx[kBatch], rd[kBatch];
-#pragma unroll
-    for (int b = 0; b < kBatch; ++b) {
-        const int hh = h0 + b * kRows + lane / kLanes;
-        live[b] = hh < a.heads;
-        second[b] = hh >= heads0;
-        head[b] = second[b] ? hh - heads0 : hh;
-        rx[b] = rd[b] = make_uint4(0, 0, 0, 0);
-        if (live[b]) {
-            const R97bRopePart& p = a.part[second[b]];
-            if (!BACK || p.w) rx[b] = ld_row(p.x, t, head[b], e);
-            if (BACK) rd[b] = ld_row(p.y, t, head[b], e);
-        }
-    }
-
-    // this lane's rotary values: 8 pairs of one member each (half layout) or 4 whole pairs
-    const int half = a.rot / 2;
-    const bool in_rot = e < a.rot, lead = e < half;
-    const int src = in_rot ? (lane & ~(kLanes - 1)) + (lead ? l + half / 8 : l - half / 8) : lane;
+    int hh = (int)(unit - t * a.chunks) * (kWarpRows * kRows) + lane / kLanes;
     const int32_t pos = a.pos[t];
+
+    // the lane's chunks: the l-th pair of the rotated part, or two neighbours of the rest
+    const int half = a.rot / 2, pairs = half / 8;
+    const bool in_rot = l < pairs;
+    const int ea = in_rot ? (INTER ? 16 * l : 8 * l) : a.rot + 16 * (l - pairs);
+    const int eb = in_rot && !INTER ? ea + half : ea + 8;
+
     const bool known = pos >= 0 && pos < a.n_pos;
     if (!known && lane == 0) atomicOr(&g_device_error, kErrArgs);
-    float cs[8], sn[8];
+    float2 cs[4], sn[4];  // the chunks' 8 pairs
 #pragma unroll
-    for (int i = 0; i < 8; ++i) cs[i] = sn[i] = 0.0f;
+    for (int i = 0; i < 4; ++i) cs[i] = both(1.0f), sn[i] = both(0.0f);
     if (in_rot && known) {
-        const int64_t at = (int64_t)pos * half + (INTER ? e / 2 : (lead ? e : e - half));
+        ld8f(a.cos_tab + (int64_t)pos * half + 8 * l, cs);
+        ld8f(a.sin_tab + (int64_t)pos * half + 8 * l, sn);
+        if (BACK) {
 #pragma unroll
-        for (int i = 0; i < (INTER ? 1 : 2); ++i) {
-            const float4 c = *reinterpret_cast<const float4*>(a.cos_tab + at + 4 * i);
-            const float4 s = *reinterpret_cast<const float4*>(a.sin_tab + at + 4 * i);
-            cs[4 * i] = c.x, cs[4 * i + 1] = c.y, cs[4 * i + 2] = c.z, cs[4 * i + 3] = c.w;
-            sn[4 * i] = s.x, sn[4 * i + 1] = s.y, sn[4 * i + 2] = s.z, sn[4 * i + 3] = s.w;
+            for (int i = 0; i < 4; ++i) sn[i] = make_float2(-sn[i].x, -sn[i].y);
         }
     }
 
-#pragma unroll
-    for (int b = 0; b < kBatch; ++b) {
-        const R97bRopePart& p = a.part[second[b] && live[b]];
+#pragma unroll 1
+    for (int n = 0; n < kWarpRows; ++n, hh += kRows) {
+        const bool live = hh < a.heads;
+        if (!__any_sync(0xFFFFFFFFu, live)) break;
+        const int i = live && hh >= heads0, h = i ? hh - heads0 : hh;
+        const R97bRopePart& p = a.part[i];
         const bool norm = p.w != nullptr;
-        float x[8], d[8], w[8];
-        unpack8(rx[b], x);
-        if (BACK) unpack8(rd[b], d);
+        float2 x[8], v[8];  // (lanes past the last row compute on zeros and store nothing)
+        Row16 rx{}, rd{};
+        if (live && (!BACK || norm)) rx = ld_row(p.x, t, h, ea, eb);
+        if (BACK && live) rd = ld_row(p.y, t, h, ea, eb);
+        float2 w[8];
         if (norm) {
-            const float4 w0 = *reinterpret_cast<const float4*>(p.w + e), w1 = *reinterpret_cast<const float4*>(p.w + e + 4);
-            w[0] = w0.x, w[1] = w0.y, w[2] = w0.z, w[3] = w0.w, w[4] = w1.x, w[5] = w1.y, w[6] = w1.z, w[7] = w1.w;
+            ld8f(p.w + ea, w);
+            ld8f(p.w + eb, w + 4);
+        }
+        unpack8(rx.a, x);
+        unpack8(rx.b, x + 4);
+        float2 ss = both(0.0f), dot = both(0.0f);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) ss = fma2(x[k], x[k], ss);
+        float s = ss.x + ss.y, r = 1.0f;
+        if (BACK) {
+            unpack8(rd.a, v);
+            unpack8(rd.b, v + 4);
+        } else {
+#pragma unroll
+            for (int o = kLanes / 2; o > 0; o >>= 1) s += __shfl_xor_sync(0xFFFFFFFFu, s, o);
+            if (norm) r = rsqrtf(s / (float)D + a.eps);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) v[k] = norm ? mul2(x[k], mul2(w[k], both(r))) : x[k];
+        }
+        if (INTER) {
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const float c = k & 1 ? cs[k / 2].y : cs[k / 2].x, z = k & 1 ? sn[k / 2].y : sn[k / 2].x;
+                v[k] = fma2(make_float2(v[k].y, v[k].x), make_float2(-z, z), mul2(v[k], both(c)));
+            }
+        } else {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const float2 c0 = v[k], c1 = v[k + 4];
+                v[k] = fma2(c1, make_float2(-sn[k].x, -sn[k].y), mul2(c0, cs[k]));
+                v[k + 4] = fma2(c0, sn[k], mul2(c1, cs[k]));
+            }
+        }
+        if (BACK && norm) {
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                v[k] = mul2(v[k], w[k]);
+                dot = fma2(v[k], x[k], dot);
+            }
         }
         if (BACK) {
-            rotate8<INTER>(d, cs, sn, in_rot, lead, src, -1.0f);
-            float ss = 0.0f, dot = 0.0f;
-            if (norm) {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    d[i] *= w[i];
-                    ss = fmaf(x[i], x[i], ss);
-                    dot = fmaf(d[i], x[i], dot);
-                }
-            }
+            float d = dot.x + dot.y;
 #pragma unroll
             for (int o = kLanes / 2; o > 0; o >>= 1) {
-                ss += __shfl_xor_sync(0xFFFFFFFFu, ss, o);
-                dot += __shfl_xor_sync(0xFFFFFFFFu, dot, o);
+                s += __shfl_xor_sync(0xFFFFFFFFu, s, o);
+                d += __shfl_xor_sync(0xFFFFFFFFu, d, o);
             }
             if (norm) {
-                const float r = rsqrtf(ss / (float)D + a.eps);
-                const float k = r * r * r * (dot / (float)D);
+                r = rsqrtf(s / (float)D + a.eps);
+                const float k3 = -r * r * r * (d / (float)D);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) d[i] = r * d[i] - k * x[i];
+                for (int k = 0; k < 8; ++k) v[k] = fma2(x[k], both(k3), mul2(v[k], both(r)));
             }
-            if (!known) {
+        }
+        if (!known) {
 #pragma unroll
-                for (int i = 0; i < 8; ++i) d[i] = 0.0f;
-            }
-            if (live[b]) st_row(p.dx, t, head[b], e, d);
-        } else {
-            float ss = 0.0f;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) ss = fmaf(x[i], x[i], ss);
-#pragma unroll
-            for (int o = kLanes / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xFFFFFFFFu, ss, o);
-            if (norm) {
-                const float r = rsqrtf(ss / (float)D + a.eps);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) x[i] *= r * w[i];
-            }
-            rotate8<INTER>(x, cs, sn, in_rot, lead, src, 1.0f);
-            if (!known) {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) x[i] = 0.0f;
-            }
-            if (live[b]) st_row(p.y, t, head[b], e, x);
+            for (int k = 0; k < 8; ++k) v[k] = both(0.0f);
+        }
+        if (live) {
+            const R97bHeadRows& o = BACK ? p.dx : p.y;
+            __nv_bfloat16* q = reinterpret_cast<__nv_bfloat16*>(o.ptr) + t * o.tok + h * o.head;
+            *reinterpret_cast<uint4*>(q + ea) = pack8(v);
+            *reinterpret_cast<uint4*>(q + eb) = pack8(v + 4);
         }
     }
 }
@@ -244,19 +237,19 @@ int rope_run(const R97bRope* a, void* stream) {
     r.n_pos = a->n_pos;
     r.rot = a->rot;
     r.eps = a->eps;
-    const int per = kBatch * 256 / a->D;  // head rows a warp takes: kBatch x (32 lanes x 8 / D)
+    const int per = kWarpRows * (512 / a->D);  // rows a warp takes
     r.chunks = (r.heads + per - 1) / per;
     r.units = a->T * r.chunks;
-    const int64_t grid = (r.units + 7) / 8;
+    const int64_t grid = (r.units + kBlockThreads / 32 - 1) / (kBlockThreads / 32);
     if (grid > 0x7FFFFFFF) return R97B_EINVAL;
     cudaStream_t st = as_stream(stream);
     const bool inter = a->interleaved != 0;
 #define R97B_ROPE_D(DD)                                                                    \
     if (a->D == DD) {                                                                      \
         if (inter)                                                                         \
-            qk_rope_kernel<DD, true, BACK><<<(unsigned)grid, 256, 0, st>>>(r);             \
+            qk_rope_kernel<DD, true, BACK><<<(unsigned)grid, kBlockThreads, 0, st>>>(r);             \
         else                                                                               \
-            qk_rope_kernel<DD, false, BACK><<<(unsigned)grid, 256, 0, st>>>(r);            \
+            qk_rope_kernel<DD, false, BACK><<<(unsigned)grid, kBlockThreads, 0, st>>>(r);            \
     }
     R97B_ROPE_D(64)
     R97B_ROPE_D(128)
