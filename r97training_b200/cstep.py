@@ -74,6 +74,8 @@ class CStep:
 
     def __init__(self, model, head_chunk: int = 2048):
         c = model.cfg
+        if c.rope_interleaved:
+            raise ValueError("the C++ step takes the fixed frame, whose rotary pairs are not interleaved")
         self.model = model
         cfg = R97hostStepConfig(c.hidden, c.layers, c.gdn_per_attn, c.gdn_heads, c.gdn_qk_heads, c.head_k,
                                 c.attn_heads, c.attn_kv_heads, c.attn_head_dim, c.rotary_dim, c.ffn, c.vocab, c.rank,

@@ -17,7 +17,8 @@ saved position resumes identically on either.
 
 ``step_rows`` lays one sub-batch into the fixed ``[rows, seq]`` frame ``TrainStep.run`` takes: a sequence a
 row, padded, with next-token targets where the sequence scores the token (``TokenSeq.score``, include/r97/
-batch.h: ``score[i] == 1`` when token i is a target predicted at position i - 1) and -1 elsewhere."""
+batch.h: ``score[i] == 1`` when token i is a target predicted at position i - 1) and -1 elsewhere.
+``step_packed`` lays it end to end instead, with the cu_seqlens of a ``model.PackedBatch``."""
 from __future__ import annotations
 
 import ctypes
@@ -275,3 +276,26 @@ def step_rows(batch, rows: int, seq: int, pad_id: int = 0):
             sc = np.asarray(s.score[1:], dtype=np.uint8) != 0
             tgt[r, :n - 1] = np.where(sc, ids[r, 1:n], -1)
     return ids, tgt.reshape(-1), int((tgt >= 0).sum())
+
+
+def step_packed(batch):
+    """One sub-batch laid end to end without padding, for ``TrainStep.run(..., batch=PackedBatch(model, cu))``: (ids
+    int32 [T], targets int32 [T], cu_seqlens int32 [n + 1], scored). Position p of a sequence targets its token p + 1
+    when the sequence scores it, else -1, as in ``step_rows``; empty sequences take no tokens."""
+    cu = np.zeros(len(batch) + 1, dtype=np.int32)
+    ids, tgt = [], []
+    for r, s in enumerate(batch):
+        n = len(s.ids)
+        if len(s.score) != n:
+            raise ValueError("step_packed: score and ids differ in length")
+        cu[r + 1] = cu[r] + n
+        row = np.asarray(s.ids, dtype=np.int32)
+        t = np.full(n, -1, dtype=np.int32)
+        if n > 1:
+            sc = np.asarray(s.score[1:], dtype=np.uint8) != 0
+            t[:-1] = np.where(sc, row[1:], -1)
+        ids.append(row)
+        tgt.append(t)
+    cat = lambda a: np.concatenate(a) if a else np.zeros(0, np.int32)  # noqa: E731
+    tgt = cat(tgt)
+    return cat(ids), tgt, cu, int((tgt >= 0).sum())

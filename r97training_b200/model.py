@@ -30,6 +30,7 @@ import torch
 from . import iqr as IQ
 from . import ops
 from .gdn import GdnPlan
+from .packed import PackedPlan
 
 
 @dataclass
@@ -55,6 +56,11 @@ class HybridConfig:
     lr: float = 1e-4
     seed: int = 1234
     lora_mlp: bool = True      # adapters on the MLP projections too (config 4 names only the mixers')
+    # rotary positions of packed batches: the longest sequence (0: seq), the scaling of far positions
+    # (ops.rope_tables) and the pairing (the fixed frame takes neighbouring halves, unscaled)
+    max_pos: int = 0
+    rope_scaling: dict | None = None
+    rope_interleaved: bool = False
 
     @property
     def kinds(self):
@@ -168,6 +174,10 @@ class HybridModel:
         self.w_final = (1.0 + 0.1 * torch.randn(cfg.hidden, generator=gen, device=device)).float()
         self.head = IQ.synth_weight(cfg.vocab, cfg.hidden, seed + 1, device=device,
                                     scale_std=1.0 / (37.0 * math.sqrt(cfg.hidden)))
+        if cfg.max_pos or cfg.rope_scaling:
+            self.rope_cos, self.rope_sin = ops.rope_tables(max(cfg.max_pos, cfg.seq), cfg.rotary_dim, cfg.rope_theta,
+                                                           scaling=cfg.rope_scaling, device=device)
+            return
         half = cfg.rotary_dim // 2
         inv = 1.0 / (cfg.rope_theta ** (np.arange(half, dtype=np.float64) * 2.0 / cfg.rotary_dim))
         ang = np.arange(cfg.seq, dtype=np.float64)[:, None] * inv[None, :]
@@ -309,6 +319,29 @@ class Adapter:
 
 # ============================================================================================ the step
 
+class PackedBatch:
+    """The geometry of one packed batch for a model on its device: ragged sequences laid end to end, their cu_seqlens
+    (host ints, from 0; empty sequences allowed) turned into what the conv, gate and GDN kernels, the rotary positions
+    and the attention core take. Sequences up to the model's rotary table (cfg.max_pos, or cfg.seq)."""
+
+    def __init__(self, model: HybridModel, cu_seqlens):
+        cfg = model.cfg
+        self.plan = PackedPlan(cu_seqlens, model.device)
+        self.T = self.plan.T
+        if self.T == 0:
+            raise ops.R97bError("a packed batch needs a token")
+        if self.plan.max_len > model.rope_cos.shape[0]:
+            raise ops.R97bError(f"a sequence of {self.plan.max_len} tokens for {model.rope_cos.shape[0]} positions")
+        cu = self.plan.cu
+        self.cu_dev = torch.from_numpy(cu).to(model.device)
+        self.gdn = GdnPlan(cu, cfg.gdn_heads, cfg.gdn_qk_heads, model.device)
+        # next-token targets, a sequence's last position unscored, for a run without explicit ones
+        nxt = np.arange(1, self.T + 1, dtype=np.int64)
+        nxt[cu[1:][self.plan.lens > 0] - 1] = -1
+        self.next = torch.from_numpy(nxt).to(model.device)
+        self.n_next = int((nxt >= 0).sum())
+
+
 class Workspace:
     """Decoded-weight scratch (one block's projections at a time) and the head's logits chunk."""
 
@@ -361,6 +394,7 @@ class TrainStep:
         # the side stream the GDN layers' out-projection adapter gradients run on (None: all on one stream)
         self.side = torch.cuda.Stream(device=model.device) if model.device.type == "cuda" else None
         self.attn_ws = None  # the attention backward's P / dS tiles, allocated at the first attention layer
+        self.packed = None   # the PackedBatch of the run in hand (None: the fixed frame)
 
     # ------------------------------------------------------------------ decoded base weights
     def _w_fwd(self, li, g: Group) -> torch.Tensor:
@@ -536,13 +570,46 @@ class TrainStep:
 
     def _attn_fwd(self, li, blk, x, sv):
         cfg, T, S = self.cfg, self.T, self.cfg.seq
-        Hq, Hkv, Dh, B = cfg.attn_heads, cfg.attn_kv_heads, cfg.attn_head_dim, cfg.micro_batch
+        Hq, Hkv, Dh = cfg.attn_heads, cfg.attn_kv_heads, cfg.attn_head_dim
         g_qkv, g_o = blk["groups"][0], blk["groups"][1]
         n1 = ops.rmsnorm_fwd(x, blk["w_in"], eps=cfg.eps)
         W = self._w_fwd(li, g_qkv)
         y = torch.empty((T, g_qkv.n), dtype=torch.bfloat16, device=x.device)
         t_qkv = self._lin_fwd(li, g_qkv, n1, W, y)
         qn = 2 * Hq * Dh
+        if self.packed is not None:
+            # queries and keys rotated token-major, the values read in place; a frame of length 1 a token is how the
+            # output gate's kernel addresses token-major heads
+            q, k, v = self._qkv_views(y)
+            qr, kr = ops.qk_rope_fwd([(q, blk["q_norm"]), (k, blk["k_norm"])], self.model.rope_cos, self.model.rope_sin,
+                                     self.packed.plan.pos, interleaved=cfg.rope_interleaved, eps=cfg.eps)
+            fa = ops.attn_packed_fwd(qr, kr, v, self.packed.plan, 1.0 / math.sqrt(Dh))
+            attn, vt, S = fa[0], None, 1
+        else:
+            qr, kr, vt, attn, fa = self._attn_frame_fwd(blk, y, qn)
+        ga = torch.empty((T, Hq * Dh), dtype=torch.bfloat16, device=x.device)
+        ops.gate_mul_fwd(attn, y[:, Dh:], 2 * Dh, Hq, Dh, S, ga)
+        W = self._w_fwd(li, g_o)
+        h1 = torch.empty_like(x)
+        t_o = self._lin_fwd(li, g_o, ga, W, h1, addend=x)
+        sv.update(n1=n1, y=y, t_qkv=t_qkv, qkv=(qr, kr, vt), fa=fa, attn=attn, ga=ga, t_o=t_o)
+        return h1
+
+    def _qkv_views(self, y):
+        """The query, key and value heads inside the fused projection's rows (each query head beside its gate)."""
+        cfg = self.cfg
+        Hq, Hkv, Dh = cfg.attn_heads, cfg.attn_kv_heads, cfg.attn_head_dim
+        qn, kn = 2 * Hq * Dh, Hkv * Dh
+        return (y[:, :qn].view(-1, Hq, 2 * Dh)[:, :, :Dh], y[:, qn:qn + kn].view(-1, Hkv, Dh),
+                y[:, qn + kn:qn + 2 * kn].view(-1, Hkv, Dh))
+
+    def _attn_frame_fwd(self, blk, y, qn):
+        """The fixed frame's q/k norm and rotation and the attention core: (q, k, v, output, (output, lse))."""
+        cfg, S = self.cfg, self.cfg.seq
+        Hq, Hkv, Dh, B = cfg.attn_heads, cfg.attn_kv_heads, cfg.attn_head_dim, cfg.micro_batch
+        x = y
+        if cfg.rope_interleaved:
+            raise ops.R97bError("interleaved rotary pairs are for packed batches")
         qr = torch.empty((B, Hq, S, Dh), dtype=torch.bfloat16, device=x.device)
         kr = torch.empty((B, Hkv, S, Dh), dtype=torch.bfloat16, device=x.device)
         vt = torch.empty((B, Hkv, S, Dh), dtype=torch.bfloat16, device=x.device)
@@ -554,43 +621,53 @@ class TrainStep:
         # the attention core on this package's tcgen05 kernel (csrc/attn_fwd.cu); its output and per-row
         # log-sum-exp feed the matching backward below
         attn, lse = ops.attn_fwd(qr, kr, vt, 1.0 / math.sqrt(Dh))
-        fa = (attn, lse)
-        ga = torch.empty((T, Hq * Dh), dtype=torch.bfloat16, device=x.device)
-        ops.gate_mul_fwd(attn, y[:, Dh:], 2 * Dh, Hq, Dh, S, ga)
-        W = self._w_fwd(li, g_o)
-        h1 = torch.empty_like(x)
-        t_o = self._lin_fwd(li, g_o, ga, W, h1, addend=x)
-        sv.update(n1=n1, y=y, t_qkv=t_qkv, qkv=(qr, kr, vt), fa=fa, attn=attn, ga=ga, t_o=t_o)
-        return h1
+        return qr, kr, vt, attn, (attn, lse)
 
     def _attn_bwd(self, li, blk, x, sv, dh1):
-        cfg, T, S = self.cfg, self.T, self.cfg.seq
-        Hq, Hkv, Dh, B = cfg.attn_heads, cfg.attn_kv_heads, cfg.attn_head_dim, cfg.micro_batch
+        cfg, T = self.cfg, self.T
+        Hq, Dh = cfg.attn_heads, cfg.attn_head_dim
         g_qkv, g_o = blk["groups"][0], blk["groups"][1]
-        qn = 2 * Hq * Dh
         W = self._w_bwd(li, g_o)
         dga = torch.empty((T, Hq * Dh), dtype=torch.bfloat16, device=x.device)
         self._lin_bwd(li, g_o, sv["ga"], sv["t_o"], W, dh1, dga)
         y = sv["y"]
         dy = torch.empty_like(y)
-        dattn = torch.empty((B, Hq, S, Dh), dtype=torch.bfloat16, device=x.device)
+        if self.packed is not None:
+            plan = self.packed.plan
+            dattn = torch.empty((T, Hq, Dh), dtype=torch.bfloat16, device=x.device)
+            ops.gate_mul_bwd(sv["attn"], y[:, Dh:], 2 * Dh, Hq, Dh, 1, dga, dattn, dy[:, Dh:])
+            q, k, v = self._qkv_views(y)
+            dqv, dkv, dvv = self._qkv_views(dy)
+            qr, kr, _ = sv["qkv"]
+            dq, dk, _ = ops.attn_packed_bwd(qr, kr, v, sv["fa"][0], dattn, sv["fa"][1], plan, 1.0 / math.sqrt(Dh), dv=dvv)
+            ops.qk_rope_bwd([(q, blk["q_norm"], dq, dqv), (k, blk["k_norm"], dk, dkv)], self.model.rope_cos,
+                            self.model.rope_sin, plan.pos, interleaved=cfg.rope_interleaved, eps=cfg.eps)
+        else:
+            self._attn_frame_bwd(blk, y, dy, dga, sv)
+        W = self._w_bwd(li, g_qkv)
+        dn1 = torch.empty_like(x)
+        self._lin_bwd(li, g_qkv, sv["n1"], sv["t_qkv"], W, dy, dn1)
+        return ops.rmsnorm_bwd(x, blk["w_in"], dn1, addend=dh1, eps=cfg.eps)
+
+    def _attn_frame_bwd(self, blk, y, dy, dga, sv):
+        """The fixed frame's gate, attention core and q/k norm and rotation adjoints, into dy."""
+        cfg, S = self.cfg, self.cfg.seq
+        Hq, Hkv, Dh, B = cfg.attn_heads, cfg.attn_kv_heads, cfg.attn_head_dim, cfg.micro_batch
+        qn = 2 * Hq * Dh
+        dattn = torch.empty((B, Hq, S, Dh), dtype=torch.bfloat16, device=y.device)
         ops.gate_mul_bwd(sv["attn"], y[:, Dh:], 2 * Dh, Hq, Dh, S, dga, dattn, dy[:, Dh:])
         qg, kg, vg = sv["qkv"]
         fa = sv["fa"]
         # the attention core's adjoint on this package's tensor-core passes (csrc/attn.cu), from the
         # forward's output and log-sum-exp
         if self.attn_ws is None:
-            self.attn_ws = ops.attn_bwd_workspace(B, Hq, S, x.device)
+            self.attn_ws = ops.attn_bwd_workspace(B, Hq, S, y.device)
         dq, dk, dv = ops.attn_bwd(qg, kg, vg, fa[0], dattn, fa[1], 1.0 / math.sqrt(Dh), self.attn_ws)
         ops.qk_norm_rope_bwd(y, 2 * Dh, Hq, Dh, blk["q_norm"], self.model.rope_cos, self.model.rope_sin,
                              cfg.rotary_dim, S, cfg.eps, dq, dy)
         ops.qk_norm_rope_bwd(y[:, qn:], Dh, Hkv, Dh, blk["k_norm"], self.model.rope_cos, self.model.rope_sin,
                              cfg.rotary_dim, S, cfg.eps, dk, dy[:, qn:])
         ops.to_bhsd(dy[:, qn + Hkv * Dh:], Dh, Hkv, Dh, S, dv, reverse=True)
-        W = self._w_bwd(li, g_qkv)
-        dn1 = torch.empty_like(x)
-        self._lin_bwd(li, g_qkv, sv["n1"], sv["t_qkv"], W, dy, dn1)
-        return ops.rmsnorm_bwd(x, blk["w_in"], dn1, addend=dh1, eps=cfg.eps)
 
     def _mlp_fwd(self, li, blk, h1, sv):
         cfg, T = self.cfg, self.T
@@ -618,15 +695,36 @@ class TrainStep:
         return ops.rmsnorm_bwd(h1, blk["w_post"], dn2, addend=dxn, eps=cfg.eps)
 
     # ------------------------------------------------------------------ the whole step
-    def run(self, ids: torch.Tensor, targets: torch.Tensor | None = None, n_scored: int | None = None):
+    def run(self, ids: torch.Tensor, targets: torch.Tensor | None = None, n_scored: int | None = None,
+            batch: PackedBatch | None = None):
         """ids: int32 [micro_batch, seq] (device). targets: int32 [micro_batch * seq] with -1 where a row
         is not scored; default: next-token targets, the last position of each sequence unscored.
         n_scored: how many rows targets scores, when the caller knows it (default targets: from the shape;
         explicit targets without it: counted on the device, which synchronises the host once).
+        batch: a PackedBatch whose ragged sequences ids (and targets) hold end to end, [batch.T]: no frame, no
+        padding; any number of tokens up to what the device holds.
         Returns the mean CE over scored rows (device f32 scalar)."""
+        if batch is None:
+            if self.packed is not None:
+                raise ops.R97bError("the step is in a packed run")
+            return self._run(ids, targets, n_scored)
+        if ids.numel() != batch.T or (targets is not None and targets.numel() != batch.T):
+            raise ops.R97bError(f"a packed batch of {batch.T} tokens, {ids.numel()} ids")
+        keep = self.T, self.cu_dev, self.plan
+        self.T, self.cu_dev, self.plan, self.packed = batch.T, batch.cu_dev, batch.gdn, batch
+        try:
+            return self._run(ids, targets, n_scored)
+        finally:
+            (self.T, self.cu_dev, self.plan), self.packed = keep, None
+
+    def _run(self, ids, targets, n_scored):
         cfg, model, T = self.cfg, self.model, self.T
         ids = ids.reshape(-1).to(torch.int32).contiguous()
-        if targets is None:
+        if targets is None and self.packed is not None:
+            nxt = self.packed.next
+            n_scored = self.packed.n_next
+            targets = torch.where(nxt >= 0, ids[nxt.clamp(min=0)], -1).to(torch.int32)
+        elif targets is None:
             n_scored = int(cfg.micro_batch * (cfg.seq - 1))
             targets = torch.empty_like(ids)
             tv = targets.view(cfg.micro_batch, cfg.seq)

@@ -213,3 +213,19 @@ def test_rope_form_against_differences(interleaved, norm):
     loss = lambda: float((ref.rope_fwd(x, w, cos, sin, interleaved, 1e-6) * do).sum())  # noqa: E731
     got = ref.rope_bwd(x, w, do, cos, sin, interleaved, 1e-6)
     assert torch.allclose(got, _central(loss, x), rtol=0, atol=1e-8)
+
+
+# ------------------------------------------------------------------------------------------ batches
+
+def test_step_packed_lays_sequences_end_to_end():
+    from r97training_b200.data import TokenSeq, step_packed, step_rows
+    batch = [TokenSeq([5, 6, 7], [0, 1, 0]), TokenSeq([], []), TokenSeq([9], [1]), TokenSeq([1, 2, 3, 4], [0, 0, 1, 1])]
+    ids, tgt, cu, scored = step_packed(batch)
+    assert ids.tolist() == [5, 6, 7, 9, 1, 2, 3, 4] and cu.tolist() == [0, 3, 3, 4, 8]
+    assert tgt.tolist() == [6, -1, -1, -1, -1, 3, 4, -1] and scored == 3
+    _, frame, n = step_rows(batch, 4, 4)
+    assert n == scored and frame.reshape(4, 4)[3].tolist() == tgt[4:].tolist()
+    ids, tgt, cu, scored = step_packed([])
+    assert len(ids) == len(tgt) == scored == 0 and cu.tolist() == [0]
+    with pytest.raises(ValueError):
+        step_packed([TokenSeq([1, 2], [1])])
