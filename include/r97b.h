@@ -602,12 +602,14 @@ int r97b_gemm_i8g_gated(const int8_t* a, int64_t lda, const float* a_scale, int6
 /* A packed batch: sequence s holds tokens [cu[s], cu[s + 1]) of T = cu[n_seq]; cu[0] = 0, empty sequences
  * allowed. q_blocks and k_blocks are device tables of n_blocks int32[4] rows {first token of the sequence,
  * its length, block index in the sequence, 0}, one per 128-token block, filled by r97b_packed_blocks on the
- * host: q_blocks with the most keys to visit first, k_blocks with the most queries first. */
+ * host: q_blocks with the most keys to visit first, k_blocks with the most queries first; k_blocks_host is the
+ * latter's host array, read during a call (the backward balances its key blocks by it). */
 typedef struct R97bPacked {
     int32_t n_seq, n_blocks;
     int64_t T;
     const int32_t* q_blocks;
     const int32_t* k_blocks;
+    const int32_t* k_blocks_host;
 } R97bPacked;
 
 /* Fills both block tables (host arrays of int32[4] rows, either may be null) and returns the block count, or

@@ -64,7 +64,8 @@ class R97bQLinearLoraBwd(ctypes.Structure):
 
 
 class R97bPacked(ctypes.Structure):
-    _fields_ = [("n_seq", c_i32), ("n_blocks", c_i32), ("T", c_i64), ("q_blocks", c_vp), ("k_blocks", c_vp)]
+    _fields_ = [("n_seq", c_i32), ("n_blocks", c_i32), ("T", c_i64), ("q_blocks", c_vp), ("k_blocks", c_vp),
+                ("k_blocks_host", c_vp)]
 
 
 class R97bHeadRows(ctypes.Structure):

@@ -589,30 +589,50 @@ struct BwdArgs {
     int64_t tok0, head0, tok1, head1;
     int32_t a0_head, a1_head, b0_head, b1_head, c0_head, c1_head;
     int32_t heads, grp;                // the rows' heads (query heads for kDQ, key/value heads else)
+    // keys: the first split_blocks blocks' query heads go to `parts` units each, launched behind the first_blocks
+    // blocks after them (whose whole units are longer)
+    int32_t split_blocks, parts, first_blocks;
+    float *part0, *part1;              // and their sums, f32 [split block][head][part][128][D], here
     float sl2, scale;
 };
 
 // A unit's tiles: kDQ walks the key blocks up to its own; the others every query block from their own on, head by head.
 template <int KIND>
 struct Walk {
-    int h, i, n, seq0, tok0, len, m, tiles, grp;
+    int h, i, n, seq0, tok0, len, m, tiles, head0;
+    int slot;  // the unit's partial sums, or -1 when it writes its rows' results
     __device__ Walk(const BwdArgs& a, int u) {
-        const int b = u / a.heads;
+        int b, part = 0, heads = KIND == kDQ ? 1 : a.grp;  // the tiles' query heads
+        slot = -1;
+        if (KIND != kDQ) u -= a.first_blocks * a.heads;
+        if (KIND != kDQ && u >= 0 && u < a.split_blocks * a.heads * a.parts) {
+            slot = u;
+            b = u / (a.heads * a.parts);
+            h = (u - b * a.heads * a.parts) / a.parts;
+            part = u % a.parts;
+            heads /= a.parts;
+        } else {
+            if (KIND != kDQ) {  // before the split ones, or behind them
+                u += a.first_blocks * a.heads;
+                u += u < a.first_blocks * a.heads ? a.split_blocks * a.heads : -a.split_blocks * a.heads * (a.parts - 1);
+            }
+            b = u / a.heads;
+            h = u - b * a.heads;
+        }
         const int4 e = a.blocks[b];
-        h = u - b * a.heads;
+        head0 = KIND == kDQ ? h / a.grp : h * a.grp + part * heads;
         i = e.z;
         seq0 = e.x;
         len = e.y;
         tok0 = seq0 + i * kBlk;
         n = min(kBlk, len - i * kBlk);
-        grp = a.grp;
         m = KIND == kDQ ? i + 1 : (len + kBlk - 1) / kBlk - i;
-        tiles = KIND == kDQ ? m : m * a.grp;
+        tiles = m * heads;
     }
     __device__ int shift() const { return kBlk - n; }
     // the first tile's column block and head, and the step to the next one's
     __device__ int first_block() const { return KIND == kDQ ? 0 : i; }
-    __device__ int first_head() const { return KIND == kDQ ? h / grp : h * grp; }
+    __device__ int first_head() const { return head0; }
     __device__ void step(int& blk, int& head) const {
         if (++blk == i + m && KIND != kDQ) {
             blk = i;
@@ -890,8 +910,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         const uint32_t mine = tmem + lane_off + (uint32_t)(w * 32);  // this thread's columns of S (and, 128 on, of dP)
         int g = 0;
         bool ok = true;
-        // the unit whose result is still in TMEM: its number, head, first valid row, and this row's token
-        int d_lt = -1, d_h = 0, d_shift = 0;
+        // the unit whose result is still in TMEM: its number, head, first valid row, partial slot, and this row's token
+        int d_lt = -1, d_h = 0, d_shift = 0, d_slot = -1;
         int64_t d_tok = 0;
         auto drain = [&]() -> bool {
             if (!warp_wait(acc_full, (uint32_t)(d_lt & 1), abort_flag)) return false;
@@ -909,7 +929,17 @@ __global__ void __launch_bounds__(kThreads, 1)
                     __syncwarp();
                     tmem_ld32(src + (uint32_t)(cc * 32), v);
                     tmem_ld_wait();
-                    if (row >= d_shift) store_row32(op + w * (D / 4) + cc * 32, v, f);
+                    if (row < d_shift) continue;
+                    if (C::kKeys && d_slot >= 0) {
+                        float4* pp = reinterpret_cast<float4*>((r ? args.part1 : args.part0) +
+                                                               ((int64_t)d_slot * kBlk + row) * D + w * (D / 4) + cc * 32);
+#pragma unroll
+                        for (int k = 0; k < 8; ++k)
+                            pp[k] = make_float4(__uint_as_float(v[4 * k]), __uint_as_float(v[4 * k + 1]),
+                                                __uint_as_float(v[4 * k + 2]), __uint_as_float(v[4 * k + 3]));
+                    } else {
+                        store_row32(op + w * (D / 4) + cc * 32, v, f);
+                    }
                 }
             }
             tc_fence_before();
@@ -999,7 +1029,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (d_lt >= 0 && !(ok = drain())) break;
             }
             if (!ok) break;
-            d_lt = lt, d_h = wk.h, d_shift = shift, d_tok = tok;
+            d_lt = lt, d_h = wk.h, d_shift = shift, d_slot = wk.slot, d_tok = tok;
         }
         if (ok && d_lt >= 0) ok = drain();
         if (!ok) *abort_flag = 1;
@@ -1049,8 +1079,72 @@ __global__ void __launch_bounds__(256) delta_kernel(const DeltaArgs a) {
 
 int64_t delta_ld(int64_t T) { return (T + 63) / 64 * 64; }
 
+// dk, dv rows of the split blocks: their parts summed in order. One warp a row and tensor, 16 bytes of bf16 a lane.
+struct SumArgs {
+    const int4* blocks;
+    const float *dv_parts, *dk_parts;
+    R97bHeadRows dv, dk;
+    float scale;
+    int32_t heads, parts;
+};
+template <int D>
+__global__ void __launch_bounds__(256) sum_parts_kernel(const SumArgs a) {
+    const int r = (int)((blockIdx.x * 256 + threadIdx.x) >> 5) % (2 * kBlk);
+    const int unit = (int)((blockIdx.x * 256 + threadIdx.x) >> 5) / (2 * kBlk), lane = threadIdx.x & 31;
+    const int row = r >> 1, is_dk = r & 1;
+    const int b = unit / a.heads, h = unit - b * a.heads;
+    const int4 e = a.blocks[b];
+    const int shift = kBlk - min(kBlk, e.y - e.z * kBlk);
+    if (row < shift || lane * 8 >= D) return;
+    const float* p = (is_dk ? a.dk_parts : a.dv_parts) + ((int64_t)unit * a.parts * kBlk + row) * D + lane * 8;
+    float v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = 0.0f;
+    for (int k = 0; k < a.parts; ++k, p += kBlk * D) {
+        const float4 x = *reinterpret_cast<const float4*>(p), y = *reinterpret_cast<const float4*>(p + 4);
+        v[0] += x.x, v[1] += x.y, v[2] += x.z, v[3] += x.w, v[4] += y.x, v[5] += y.y, v[6] += y.z, v[7] += y.w;
+    }
+    const float f = is_dk ? a.scale : 1.0f;
+    const R97bHeadRows& o = is_dk ? a.dk : a.dv;
+    const int64_t tok = (int64_t)e.x + e.z * kBlk + row - shift;
+    *reinterpret_cast<uint4*>(reinterpret_cast<__nv_bfloat16*>(o.ptr) + tok * o.tok + h * o.head + lane * 8) =
+        make_uint4(pack_bf16(v[0] * f, v[1] * f), pack_bf16(v[2] * f, v[3] * f), pack_bf16(v[4] * f, v[5] * f),
+                   pack_bf16(v[6] * f, v[7] * f));
+}
+
+// How the key blocks' units are split over their query heads: a block takes as many tiles as its query blocks times the
+// group's heads, and the longest unit bounds the pass where the SMs' average share is less. The blocks (a prefix of the
+// longest-first table) whose units are above 1.25 of that share go to `parts` units each, with their f32 sums in the
+// workspace and one more launch to add them. Measured, dK and dV with the sums: a chat batch of 8192 tokens, 16/4 heads of
+// 256: 186 us at 1.25, 187 at 1, 206 at 1.5, 222 at 0.75, 230 unsplit; 2 x 4096 tokens, whose longest unit is 1.12 of the
+// share: 511 us unsplit, 523 split (power, not the longest unit, bounds it).
+struct Split {
+    int blocks, parts, first;
+};
+Split split_of(const R97bPacked& p, int Hq, int Hkv) {
+    const int grp = Hq / Hkv;
+    if (grp == 1 || p.T == 0) return Split{0, 1, 0};
+    auto queries = [&](int b) {
+        const int32_t* e = p.k_blocks_host + 4 * (int64_t)b;
+        return ((int64_t)e[1] + kBlk - 1) / kBlk - e[2];
+    };
+    int64_t tiles = 0;
+    for (int b = 0; b < p.n_blocks; ++b) tiles += queries(b);
+    const double limit = 1.25 * (double)(tiles * Hq) / num_sms();
+    const double longest = (double)(queries(0) * grp);
+    if (longest <= limit) return Split{0, 1, 0};
+    Split s{0, grp, 0};
+    for (int d = grp - 1; d > 1; --d)
+        if (grp % d == 0 && longest / d <= limit) s.parts = d;
+    while (s.blocks < p.n_blocks && (double)(queries(s.blocks) * grp) > limit) ++s.blocks;
+    while (s.blocks + s.first < p.n_blocks && queries(s.blocks + s.first) * s.parts > queries(0)) ++s.first;
+    return s;
+}
+int64_t part_floats(const Split& s, int Hkv, int D) { return (int64_t)s.blocks * s.parts * Hkv * kBlk * D; }
+
 template <int D, int KIND>
-int launch_bwd(const R97bPacked& p, const R97bAttnPackedBwd& a, const float* delta, cudaStream_t st) {
+int launch_bwd(const R97bPacked& p, const R97bAttnPackedBwd& a, const float* delta, const Split& split, float* dv_parts,
+               float* dk_parts, cudaStream_t st) {
     using C = BCfg<D, KIND>;
     static_assert(C::kSmemBytes <= 232448, "shared memory");
     const bool dq = KIND == kDQ;
@@ -1072,9 +1166,12 @@ int launch_bwd(const R97bPacked& p, const R97bAttnPackedBwd& a, const float* del
     r.a0_head = (int32_t)a0.head, r.a1_head = (int32_t)a1.head, r.b0_head = (int32_t)b0.head, r.b1_head = (int32_t)b1.head;
     r.c0_head = (int32_t)c0.head, r.c1_head = (int32_t)c1.head;
     r.heads = ha, r.grp = a.Hq / a.Hkv;
+    r.split_blocks = dq ? 0 : split.blocks, r.parts = split.parts, r.first_blocks = dq ? 0 : split.first;
+    r.part0 = KIND == kDK ? dk_parts : dv_parts, r.part1 = dk_parts;
     r.sl2 = a.scale * kLog2e, r.scale = a.scale;
+    const int units = (p.n_blocks + (dq ? 0 : split.blocks * (split.parts - 1))) * ha;
     if (!smem_opt_in(bwd_kernel<D, KIND>, C::kSmemBytes)) return R97B_ELAUNCH;
-    bwd_kernel<D, KIND><<<p.n_blocks * ha, kThreads, C::kSmemBytes, st>>>(m[0], m[1], m[2], m[3], m[4], m[5], r);
+    bwd_kernel<D, KIND><<<units, kThreads, C::kSmemBytes, st>>>(m[0], m[1], m[2], m[3], m[4], m[5], r);
     return launch_status();
 }
 
@@ -1086,25 +1183,30 @@ int run_bwd(const R97bPacked& p, const R97bAttnPackedBwd& a, cudaStream_t st) {
     if (grid > 0x7FFFFFFF) return R97B_EINVAL;
     delta_kernel<D><<<(unsigned)grid, 256, 0, st>>>(d);
     int rc = launch_status();
-    if (D == 256) {
-        if (rc == R97B_OK) rc = launch_bwd<D, D == 256 ? kDV : kDKV>(p, a, delta, st);
-        if (rc == R97B_OK) rc = launch_bwd<D, D == 256 ? kDK : kDKV>(p, a, delta, st);
-    } else {
-        if (rc == R97B_OK) rc = launch_bwd<D, D == 256 ? kDV : kDKV>(p, a, delta, st);
+    const Split split = split_of(p, a.Hq, a.Hkv);
+    float* dv_parts = delta + a.Hq * delta_ld(p.T);
+    float* dk_parts = dv_parts + part_floats(split, a.Hkv, D);
+    if (rc == R97B_OK) rc = launch_bwd<D, D == 256 ? kDV : kDKV>(p, a, delta, split, dv_parts, dk_parts, st);
+    if (D == 256 && rc == R97B_OK) rc = launch_bwd<D, D == 256 ? kDK : kDKV>(p, a, delta, split, dv_parts, dk_parts, st);
+    if (split.blocks > 0 && rc == R97B_OK) {
+        const SumArgs s{reinterpret_cast<const int4*>(p.k_blocks), dv_parts, dk_parts, a.dv, a.dk, a.scale, a.Hkv,
+                        split.parts};
+        sum_parts_kernel<D><<<split.blocks * a.Hkv * (2 * kBlk / 8), 256, 0, st>>>(s);
+        rc = launch_status();
     }
-    return rc == R97B_OK ? launch_bwd<D, kDQ>(p, a, delta, st) : rc;
+    return rc == R97B_OK ? launch_bwd<D, kDQ>(p, a, delta, split, dv_parts, dk_parts, st) : rc;
 }
 
 bool plan_ok(const R97bPacked* p) {
     if (!p || p->n_seq < 0 || p->n_blocks < 0 || p->T < 0 || p->T > 0x7FFFFF00) return false;
     if (p->T == 0) return p->n_blocks == 0;
-    return p->n_blocks >= (p->T + 127) / 128 && p->n_blocks <= p->T && p->q_blocks && p->k_blocks &&
+    return p->n_blocks >= (p->T + 127) / 128 && p->n_blocks <= p->T && p->q_blocks && p->k_blocks && p->k_blocks_host &&
            !(reinterpret_cast<uintptr_t>(p->q_blocks) & 15) && !(reinterpret_cast<uintptr_t>(p->k_blocks) & 15);
 }
 bool heads_ok(int32_t Hq, int32_t Hkv, int32_t D) {
     return Hq > 0 && Hkv > 0 && Hq % Hkv == 0 && Hq <= 65535 && (D == 128 || D == 256);
 }
-bool units_ok(const R97bPacked* p, int32_t H) { return (int64_t)p->n_blocks * H <= 0x3FFFFFFF; }
+bool units_ok(const R97bPacked* p, int32_t H) { return (int64_t)p->n_blocks * H <= 0x3FFFFF; }
 bool lse_ok(const float* lse, int64_t ld, int64_t T) { return lse && !(reinterpret_cast<uintptr_t>(lse) & 3) && ld >= T; }
 
 }  // namespace
@@ -1154,7 +1256,8 @@ extern "C" int r97b_attn_packed_fwd(const R97bPacked* p, const R97bAttnPackedFwd
 
 extern "C" int64_t r97b_attn_packed_bwd_workspace_bytes(const R97bPacked* p, int32_t Hq, int32_t Hkv, int32_t D) {
     if (!r97b::plan_ok(p) || !r97b::heads_ok(Hq, Hkv, D)) return -1;
-    return (int64_t)Hq * r97b::delta_ld(p->T) * 4;
+    const r97b::Split s = r97b::split_of(*p, Hq, Hkv);
+    return ((int64_t)Hq * r97b::delta_ld(p->T) + 2 * r97b::part_floats(s, Hkv, D)) * 4;
 }
 
 extern "C" int r97b_attn_packed_bwd(const R97bPacked* p, const R97bAttnPackedBwd* a, void* stream) {

@@ -37,5 +37,6 @@ class PackedPlan:
         self.device = self.buf.device
         self.pos = self.buf[8 * n:]
         base = self.buf.data_ptr()
-        self.desc = R97bPacked(self.n_seq, n, self.T, base, base + 16 * n)
+        self._k_host = host[4 * n:8 * n].copy()
+        self.desc = R97bPacked(self.n_seq, n, self.T, base, base + 16 * n, self._k_host.ctypes.data)
         self.ref = ctypes.byref(self.desc)

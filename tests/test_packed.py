@@ -55,6 +55,13 @@ def test_plan_positions_and_limits():
     assert L.lib().r97b_packed_blocks(None, 1, None, None) == -1
 
 
+HOST = np.array([[0, 300, 0, 0], [0, 300, 1, 0], [0, 300, 2, 0]], np.int32)  # 300 tokens, longest first
+
+
+def _plan():
+    return L.R97bPacked(1, 3, 300, FAKE, FAKE, HOST.ctypes.data)
+
+
 def _rows(ptr=FAKE, tok=2048, head=256):
     return L.R97bHeadRows(ptr, tok, head)
 
@@ -82,11 +89,11 @@ BAD_COMMON = [dict(Hq=0), dict(Hkv=0), dict(Hq=7), dict(D=192), dict(D=64), dict
 
 @pytest.mark.parametrize("bad", BAD_COMMON + [dict(p=dict(T=-1)), dict(p=dict(n_blocks=2)), dict(p=dict(q_blocks=None)),
                                               dict(p=dict(k_blocks=FAKE + 4)), dict(p=dict(T=0)),
-                                              dict(p=dict(n_blocks=301))])
+                                              dict(p=dict(n_blocks=301)), dict(p=dict(k_blocks_host=None))])
 def test_attention_refusals(bad):
     h = L.lib()
     bad = dict(bad)
-    plan = L.R97bPacked(1, 3, 300, FAKE, FAKE)
+    plan = _plan()
     for n, v in bad.pop("p", {}).items():
         setattr(plan, n, v)
     assert h.r97b_attn_packed_fwd(ctypes.byref(plan), ctypes.byref(_fwd_args(**bad)), None) == 1
@@ -95,7 +102,7 @@ def test_attention_refusals(bad):
 
 def test_attention_refusals_of_one_direction():
     h = L.lib()
-    plan = L.R97bPacked(1, 3, 300, FAKE, FAKE)
+    plan = _plan()
     ref_ = ctypes.byref(plan)
     assert h.r97b_attn_packed_fwd(None, ctypes.byref(_fwd_args()), None) == 1
     assert h.r97b_attn_packed_fwd(ref_, None, None) == 1
@@ -115,7 +122,7 @@ def test_attention_refusals_of_one_direction():
 def test_nothing_to_do_is_ok():
     """A batch of empty sequences launches nothing."""
     h = L.lib()
-    plan = L.R97bPacked(2, 0, 0, None, None)
+    plan = L.R97bPacked(2, 0, 0, None, None, None)
     assert h.r97b_attn_packed_fwd(ctypes.byref(plan), ctypes.byref(_fwd_args()), None) == 0
     assert h.r97b_attn_packed_bwd(ctypes.byref(plan), ctypes.byref(_bwd_args()), None) == 0
     assert h.r97b_qk_rope_fwd(ctypes.byref(_rope_args(T=0)), None) == 0
