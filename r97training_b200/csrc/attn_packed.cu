@@ -1153,10 +1153,13 @@ int launch_bwd(const R97bPacked& p, const R97bAttnPackedBwd& a, const float* del
     const R97bHeadRows &c0 = dq ? a.k : (KIND == kDK ? a.q : a.dout), &c1 = a.q;
     const int ha = dq ? a.Hq : a.Hkv, hb = dq ? a.Hkv : a.Hq;
     CUtensorMap m[6];
-    if (!make_rows_map(&m[0], a0, ha, D, p.T, kBlk) || !make_rows_map(&m[1], a1, ha, D, p.T, kBlk) ||
-        !make_rows_map(&m[2], b0, hb, D, p.T, kBlk) || !make_rows_map(&m[3], b1, hb, D, p.T, kBlk) ||
-        !make_rows_map(&m[4], c0, hb, D, p.T, C::kVRows) || !make_rows_map(&m[5], c1, a.Hq, D, p.T, C::kVRows))
+    if (!make_rows_map(&m[0], a0, ha, D, p.T, kBlk) || !make_rows_map(&m[2], b0, hb, D, p.T, kBlk) ||
+        !make_rows_map(&m[4], c0, hb, D, p.T, C::kVRows))
         return R97B_EINVAL;
+    m[1] = m[0], m[3] = m[2], m[5] = m[4];  // where the kind has no such stream
+    if (C::kDP && (!make_rows_map(&m[1], a1, ha, D, p.T, kBlk) || !make_rows_map(&m[3], b1, hb, D, p.T, kBlk)))
+        return R97B_EINVAL;
+    if (KIND == kDKV && !make_rows_map(&m[5], c1, a.Hq, D, p.T, C::kVRows)) return R97B_EINVAL;
     BwdArgs r{};
     r.blocks = reinterpret_cast<const int4*>(dq ? p.q_blocks : p.k_blocks);
     r.lse = a.lse, r.ld_lse = a.ld_lse, r.delta = delta, r.ld_delta = delta_ld(p.T);

@@ -7,11 +7,12 @@ raises R97bError on a non-zero status. Nothing here computes on the CPU.
 from __future__ import annotations
 
 import ctypes
+import struct
 
 import torch
 
 from ._lib import (R97bAttnBwd, R97bAttnFwd, R97bAttnPackedBwd, R97bAttnPackedFwd, R97bCastSeg, R97bError, R97bGemm,
-                   R97bHeadRows, R97bMat, R97bQLinearLora, R97bQLinearLoraBwd, R97bRope, check, lib)
+                   R97bMat, R97bQLinearLora, R97bQLinearLoraBwd, R97bRope, check, lib)
 
 EPI_STORE_BF16, EPI_STORE_F32, EPI_ATOMIC_F32, EPI_ATOMIC_F32T, EPI_SPLIT_BF16 = 0, 1, 2, 3, 4
 EPI_SWIGLU, EPI_SWIGLU_BWD = 5, 6
@@ -438,42 +439,59 @@ def attn_bwd(q, k, v, o, dout, lse, scale, ws, dq=None, dk=None, dv=None, stream
 
 # ------------------------------------------------------------------------------------------ packed sequences
 
-def _here(dev, what: str):
-    """A launch goes to the current device: tensors of another one are refused."""
-    if dev.index != torch.cuda.current_device():
+# The descriptions these calls pass are packed as bytes in the C structs' layout (R97bAttnPackedFwd and its kin in
+# _lib.py): filling nested ctypes structures field by field costs more than a short batch's kernels.
+_FWD = struct.Struct("@3if" + "3q" * 4 + "Pq")
+_BWD = struct.Struct("@3if" + "3q" * 5 + "Pq" + "3q" * 3 + "Pq")
+_ROPE = struct.Struct("@4i2qfi3P" + "qP9q" * 2)
+for _s, _c in ((_FWD, R97bAttnPackedFwd), (_BWD, R97bAttnPackedBwd), (_ROPE, R97bRope)):
+    assert _s.size == ctypes.sizeof(_c)
+_BF16, _F32 = torch.bfloat16, torch.float32
+
+
+def _packed_stream(stream, dev, what: str) -> int:
+    """The stream of a call on tensors of `dev`: a launch goes to the current device, and tensors or a stream of another
+    one are refused."""
+    if not dev.type == "cuda":
+        raise R97bError(f"{what}: tensors must be on a CUDA device, got {dev}")
+    if dev.index != torch.cuda.current_device() or (stream is not None and stream.device_index != dev.index):
         raise R97bError(f"{what}: tensors are on {dev}, the current device is cuda:{torch.cuda.current_device()}")
+    return torch._C._cuda_getCurrentRawStream(dev.index) if stream is None else stream.cuda_stream
 
 
-def _head_rows(t, name: str, heads: int, D: int, rows: int, device) -> R97bHeadRows:
-    """A token-major bf16 view [>= rows, heads, D]: unit inner stride, tokens and heads at any stride of a multiple
-    of 8 elements that keeps a token's heads apart."""
-    _need(t, torch.bfloat16, name)
-    if t.dim() != 3 or t.shape[1] != heads or t.shape[2] != D or t.shape[0] < rows or t.device != device:
-        raise R97bError(f"{name} must be [>= {rows}, {heads}, {D}] on {device}, got {tuple(t.shape)} on {t.device}")
+def _head_rows(t, name: str, heads: int, D: int, rows: int, dev):
+    """(pointer, token stride, head stride) of a token-major bf16 view [>= rows, heads, D]: unit inner stride, tokens and
+    heads at any stride of a multiple of 8 elements that keeps a token's heads apart."""
+    if t.dtype is not _BF16 or t.dim() != 3 or t.device != dev:
+        raise R97bError(f"{name} must be a 3-D bf16 tensor on {dev}, got {t.dim()}-D {t.dtype} on {t.device}")
+    n, h, d = t.shape
+    if h != heads or d != D or n < rows:
+        raise R97bError(f"{name} must be [>= {rows}, {heads}, {D}], got {tuple(t.shape)}")
     tok, head, inner = t.stride()
-    head = head if heads > 1 else D
-    tok = tok if t.shape[0] > 1 else (heads - 1) * head + D
-    if inner != 1 or head < D or head % 8 or tok % 8 or tok < (heads - 1) * head + D:
+    if heads == 1:
+        head = D
+    least = (heads - 1) * head + D
+    if n == 1:
+        tok = least
+    if inner != 1 or head < D or head % 8 or tok % 8 or tok < least:
         raise R97bError(f"{name}: strides {t.stride()} are not token-major head rows")
-    return R97bHeadRows(t.data_ptr(), tok, head)
+    return t.data_ptr(), tok, head
 
 
-def _lse_ld(lse, heads: int, T: int, device) -> int:
-    _need(lse, torch.float32, "lse")
-    if lse.dim() != 2 or lse.shape[0] != heads or lse.shape[1] < T or lse.device != device or \
+def _lse_ld(lse, heads: int, T: int, dev) -> int:
+    if lse.dtype is not _F32 or lse.dim() != 2 or lse.device != dev or lse.shape[0] != heads or lse.shape[1] < T or \
             (lse.shape[1] > 1 and lse.stride(1) != 1):
-        raise R97bError(f"lse must be a row-major [{heads}, >= {T}] f32 tensor on {device}")
+        raise R97bError(f"lse must be a row-major [{heads}, >= {T}] f32 tensor on {dev}")
     return lse.stride(0) if heads > 1 else max(T, 1)
 
 
 def _packed_dims(q, k, plan):
     if q.dim() != 3 or k.dim() != 3:
         raise R97bError("q and k must be [T, heads, D]")
-    _need(q, torch.bfloat16, "q")
     if plan.device != q.device:
         raise R97bError(f"the plan is on {plan.device}, q on {q.device}")
-    _here(q.device, "attn_packed")
-    return q.shape[1], k.shape[1], q.shape[2]
+    T, Hq, D = q.shape
+    return max(T, plan.T), Hq, k.shape[1], D, q.device
 
 
 def attn_packed_fwd(q, k, v, plan, scale, o=None, lse=None, stream=None):
@@ -481,17 +499,17 @@ def attn_packed_fwd(q, k, v, plan, scale, o=None, lse=None, stream=None):
     [T, Hkv, D] bf16 token-major views (any token and head strides of a multiple of 8), D 128 or 256, `plan` a
     packed.PackedPlan of at most T tokens. Returns (o [T, Hq, D] bf16, lse [Hq, T] f32); rows behind the plan's last
     token are left as they were."""
-    Hq, Hkv, D = _packed_dims(q, k, plan)
-    rows = max(plan.T, q.shape[0])
-    o = torch.empty((rows, Hq, D), dtype=torch.bfloat16, device=q.device) if o is None else o
-    lse = torch.empty((Hq, rows), dtype=torch.float32, device=q.device) if lse is None else lse
-    if plan.T == 0:
+    rows, Hq, Hkv, D, dev = _packed_dims(q, k, plan)
+    st = _packed_stream(stream, dev, "attn_packed_fwd")
+    o = torch.empty((rows, Hq, D), dtype=_BF16, device=dev) if o is None else o
+    lse = torch.empty((Hq, rows), dtype=_F32, device=dev) if lse is None else lse
+    T = plan.T
+    if T == 0:
         return o, lse
-    dev = q.device
-    a = R97bAttnPackedFwd(Hq, Hkv, D, float(scale), _head_rows(q, "q", Hq, D, plan.T, dev),
-                          _head_rows(k, "k", Hkv, D, plan.T, dev), _head_rows(v, "v", Hkv, D, plan.T, dev),
-                          _head_rows(o, "o", Hq, D, plan.T, dev), _ptr(lse), _lse_ld(lse, Hq, plan.T, dev))
-    check(lib().r97b_attn_packed_fwd(plan.ref, ctypes.byref(a), _stream(stream)), "r97b_attn_packed_fwd")
+    a = _FWD.pack(Hq, Hkv, D, scale, *_head_rows(q, "q", Hq, D, T, dev), *_head_rows(k, "k", Hkv, D, T, dev),
+                  *_head_rows(v, "v", Hkv, D, T, dev), *_head_rows(o, "o", Hq, D, T, dev), lse.data_ptr(),
+                  _lse_ld(lse, Hq, T, dev))
+    check(lib().r97b_attn_packed_fwd(plan.ref, a, st), "r97b_attn_packed_fwd")
     return o, lse
 
 
@@ -508,23 +526,23 @@ def attn_packed_bwd(q, k, v, o, dout, lse, plan, scale, ws=None, dq=None, dk=Non
     the probabilities): every operand a token-major view as there. `ws` is attn_packed_bwd_workspace's buffer (calls
     that share one must not overlap on the GPU); without it one is allocated. Rows behind the plan's last token
     are left as they were."""
-    Hq, Hkv, D = _packed_dims(q, k, plan)
-    dev, T = q.device, plan.T
-    rows = max(T, q.shape[0])
-    need = lambda h: torch.empty((rows, h, D), dtype=torch.bfloat16, device=dev)  # noqa: E731
-    dq = need(Hq) if dq is None else dq
-    dk = need(Hkv) if dk is None else dk
-    dv = need(Hkv) if dv is None else dv
+    rows, Hq, Hkv, D, dev = _packed_dims(q, k, plan)
+    st = _packed_stream(stream, dev, "attn_packed_bwd")
+    dq = torch.empty((rows, Hq, D), dtype=_BF16, device=dev) if dq is None else dq
+    dk = torch.empty((rows, Hkv, D), dtype=_BF16, device=dev) if dk is None else dk
+    dv = torch.empty((rows, Hkv, D), dtype=_BF16, device=dev) if dv is None else dv
+    T = plan.T
     if T == 0:
         return dq, dk, dv
     ws = attn_packed_bwd_workspace(plan, Hq, Hkv, D) if ws is None else ws
     if ws.device != dev or not ws.is_contiguous():
         raise R97bError(f"ws must be a contiguous buffer on {dev}")
-    r = lambda t, name, h: _head_rows(t, name, h, D, T, dev)  # noqa: E731
-    a = R97bAttnPackedBwd(Hq, Hkv, D, float(scale), r(q, "q", Hq), r(k, "k", Hkv), r(v, "v", Hkv), r(o, "o", Hq),
-                          r(dout, "dout", Hq), _ptr(lse), _lse_ld(lse, Hq, T, dev), r(dq, "dq", Hq), r(dk, "dk", Hkv),
-                          r(dv, "dv", Hkv), _ptr(ws), ws.numel() * ws.element_size())
-    check(lib().r97b_attn_packed_bwd(plan.ref, ctypes.byref(a), _stream(stream)), "r97b_attn_packed_bwd")
+    a = _BWD.pack(Hq, Hkv, D, scale, *_head_rows(q, "q", Hq, D, T, dev), *_head_rows(k, "k", Hkv, D, T, dev),
+                  *_head_rows(v, "v", Hkv, D, T, dev), *_head_rows(o, "o", Hq, D, T, dev),
+                  *_head_rows(dout, "dout", Hq, D, T, dev), lse.data_ptr(), _lse_ld(lse, Hq, T, dev),
+                  *_head_rows(dq, "dq", Hq, D, T, dev), *_head_rows(dk, "dk", Hkv, D, T, dev),
+                  *_head_rows(dv, "dv", Hkv, D, T, dev), ws.data_ptr(), ws.numel() * ws.element_size())
+    check(lib().r97b_attn_packed_bwd(plan.ref, a, st), "r97b_attn_packed_bwd")
     return dq, dk, dv
 
 
@@ -548,51 +566,49 @@ def rope_tables(n_pos: int, rot: int, theta: float, scaling=None, device="cuda",
     device = torch.device(device)
     if device.index is None:
         device = torch.device("cuda", torch.cuda.current_device())
-    _here(device, "rope_tables")
+    st = _packed_stream(stream, device, "rope_tables")
     cos = torch.empty((n_pos, rot // 2), dtype=torch.float32, device=device)
     sin = torch.empty_like(cos)
     v = {**args, **sc}
     check(lib().r97b_rope_tables(_ptr(cos), _ptr(sin), n_pos, rot, float(theta), ROPE_SCALINGS[kind],
                                  float(v.get("factor", 1.0)), float(v.get("original", 0.0)),
-                                 float(v.get("beta_fast", 0.0)), float(v.get("beta_slow", 0.0)), _stream(stream)),
+                                 float(v.get("beta_fast", 0.0)), float(v.get("beta_slow", 0.0)), st),
           "r97b_rope_tables")
     return cos, sin
 
 
-def _rope_call(tensors, cos, sin, pos, interleaved, eps):
-    """The R97bRope description of [(x, w, y, dx)] tensors (x None where it is not read, dx None in the forward)."""
+_NO_ROWS = (0, 0, 0)
+
+
+def _rope_call(tensors, cos, sin, pos, interleaved, eps, stream, what):
+    """(the R97bRope description, stream) of [(x, w, y, dx)] tensors (x None where it is not read, dx None in the
+    forward)."""
     if not 1 <= len(tensors) <= 2:
         raise R97bError("qk_rope takes one or two tensors")
     lead = tensors[0][2]
     dev, T = lead.device, pos.numel()
-    _need(pos, torch.int32, "pos")
-    for t, name in ((cos, "cos"), (sin, "sin")):
-        _need(t, torch.float32, name)
-        if t.dim() != 2 or not t.is_contiguous() or t.shape != cos.shape or t.device != dev:
-            raise R97bError(f"{name} must be a contiguous [n_pos, rot / 2] table on {dev}")
-    if pos.dim() != 1 or not pos.is_contiguous() or pos.device != dev:
-        raise R97bError(f"pos must be a contiguous 1-D tensor on {dev}")
-    _here(dev, "qk_rope")
-    a = R97bRope()
-    a.D, a.rot, a.interleaved, a.n_parts = lead.shape[-1], 2 * cos.shape[1], int(interleaved), len(tensors)
-    a.T, a.n_pos, a.eps = T, cos.shape[0], eps
-    a.cos_tab, a.sin_tab, a.pos = cos.data_ptr(), sin.data_ptr(), pos.data_ptr()
-    for i, (x, w, y, dx) in enumerate(tensors):
+    st = _packed_stream(stream, dev, what)
+    if cos.dtype is not _F32 or sin.dtype is not _F32 or cos.dim() != 2 or cos.shape != sin.shape or \
+            cos.device != dev or sin.device != dev or not cos.is_contiguous() or not sin.is_contiguous():
+        raise R97bError(f"cos and sin must be contiguous [n_pos, rot / 2] f32 tables on {dev}")
+    if pos.dtype is not torch.int32 or pos.dim() != 1 or not pos.is_contiguous() or pos.device != dev:
+        raise R97bError(f"pos must be a contiguous 1-D i32 tensor on {dev}")
+    D = lead.shape[-1]
+    parts = []
+    for x, w, y, dx in tensors:
         if y.dim() != 3:
             raise R97bError("qk_rope tensors are [T, heads, D]")
-        p, heads = a.part[i], y.shape[1]
-        p.heads = heads
-        if w is not None:
-            _need(w, torch.float32, "w")
-            if tuple(w.shape) != (a.D,) or not w.is_contiguous() or w.device != dev:
-                raise R97bError(f"w must be a contiguous [{a.D}] f32 gain on {dev}")
-            p.w = w.data_ptr()
-        p.y = _head_rows(y, "y", heads, a.D, T, dev)
-        if x is not None:
-            p.x = _head_rows(x, "x", heads, a.D, T, dev)
-        if dx is not None:
-            p.dx = _head_rows(dx, "dx", heads, a.D, T, dev)
-    return a
+        heads = y.shape[1]
+        if w is not None and (w.dtype is not _F32 or w.dim() != 1 or w.shape[0] != D or not w.is_contiguous() or
+                              w.device != dev):
+            raise R97bError(f"w must be a contiguous [{D}] f32 gain on {dev}")
+        parts += (heads, 0 if w is None else w.data_ptr(),
+                  *(_NO_ROWS if x is None else _head_rows(x, "x", heads, D, T, dev)), *_head_rows(y, "y", heads, D, T, dev),
+                  *(_NO_ROWS if dx is None else _head_rows(dx, "dx", heads, D, T, dev)))
+    if len(tensors) == 1:
+        parts += (0,) * 11
+    return _ROPE.pack(D, 2 * cos.shape[1], 1 if interleaved else 0, len(tensors), T, cos.shape[0], eps, 0, cos.data_ptr(),
+                      sin.data_ptr(), pos.data_ptr(), *parts), st
 
 
 def qk_rope_fwd(parts, cos, sin, pos, *, interleaved=False, eps=1e-6, outs=None, stream=None):
@@ -601,13 +617,14 @@ def qk_rope_fwd(parts, cos, sin, pos, *, interleaved=False, eps=1e-6, outs=None,
     or None for none; cos, sin [n_pos, rot / 2] (rope_tables; rot a multiple of 16 up to D), pos i32 [T]. Pairs
     (i, i + rot / 2), or (2 i, 2 i + 1) when interleaved. Returns one [rows, heads, D] tensor a part (`outs`, when
     given); rows behind T are left as they were."""
-    outs = [torch.empty((x.shape), dtype=torch.bfloat16, device=x.device) for x, _ in parts] if outs is None else outs
+    outs = [torch.empty(x.shape, dtype=_BF16, device=x.device) for x, _ in parts] if outs is None else outs
     if len(outs) != len(parts):
         raise R97bError("qk_rope_fwd: one output a part")
     if pos.numel() == 0:
         return outs
-    a = _rope_call([(x, w, y, None) for (x, w), y in zip(parts, outs)], cos, sin, pos, interleaved, eps)
-    check(lib().r97b_qk_rope_fwd(ctypes.byref(a), _stream(stream)), "r97b_qk_rope_fwd")
+    a, st = _rope_call([(x, w, y, None) for (x, w), y in zip(parts, outs)], cos, sin, pos, interleaved, eps, stream,
+                       "qk_rope_fwd")
+    check(lib().r97b_qk_rope_fwd(a, st), "r97b_qk_rope_fwd")
     return outs
 
 
@@ -618,9 +635,9 @@ def qk_rope_bwd(parts, cos, sin, pos, *, interleaved=False, eps=1e-6, stream=Non
         raise R97bError("qk_rope_bwd: a normalised part needs its x")
     if pos.numel() == 0:
         return
-    a = _rope_call([(x if w is not None else None, w, dout, dx) for x, w, dout, dx in parts], cos, sin, pos, interleaved,
-                   eps)
-    check(lib().r97b_qk_rope_bwd(ctypes.byref(a), _stream(stream)), "r97b_qk_rope_bwd")
+    a, st = _rope_call([(x if w is not None else None, w, dout, dx) for x, w, dout, dx in parts], cos, sin, pos,
+                       interleaved, eps, stream, "qk_rope_bwd")
+    check(lib().r97b_qk_rope_bwd(a, st), "r97b_qk_rope_bwd")
 
 
 def embed(table, ids, out, stream=None):
