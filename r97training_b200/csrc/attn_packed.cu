@@ -160,7 +160,7 @@ __device__ __forceinline__ Unit unit_geom(const int4* blocks, int heads, int u) 
 // One pass over the keys. A unit is one 128-query block of one head; key tile j of it: S_j = Q K_j^T into one of kBufs
 // TMEM buffers, P_j = 2^(S_j c - m) as bf16 over the same buffer's columns, O += P_j V_j in TMEM. Each buffer has a
 // softmax warpgroup, a thread a row, so the tiles' exponentials overlap one another and the products: S is issued kBufs - 1
-// tiles ahead of P V, and P V starts on the first half of the keys while the second half's P is formed. The reference m a
+// tiles ahead of P V, and P V starts on one half of the keys while the other's P is formed. The reference m a
 // row's exponentials use is handed from tile to tile; it is moved (and O rescaled, by the threads that own the rows) only
 // when the row's maximum has outgrown it by 2^8, which f32 sums and bf16 probabilities carry without loss. A unit's
 // result is drained after the next unit's first P, which the tensor core has meanwhile been given the scores of.
@@ -184,7 +184,7 @@ __global__ void __launch_bounds__(FCfg<D>::kThreads, 1)
     uint64_t* q_full = empty_bar + C::kStages;  // [2]
     uint64_t* q_empty = q_full + 2;             // [2]
     uint64_t* s_full = q_empty + 2;             // [NB]
-    uint64_t* p_full = s_full + NB;             // [NB][2]: the first and second 64 keys' P written
+    uint64_t* p_full = s_full + NB;             // [NB][2]: P of keys 64 to 127, of 0 to 63 written
     uint64_t* pv_done = p_full + 2 * NB;        // [NB]
     uint64_t* o_full = pv_done + NB;
     uint64_t* o_empty = o_full + 1;
@@ -272,7 +272,7 @@ __global__ void __launch_bounds__(FCfg<D>::kThreads, 1)
 #pragma unroll
                                 for (int n = 0; n < ND; ++n)
                                     tma_load_3d(st + n * (C::kVRows * 128), &tV, &full_bar[stage], x + 64 * n,
-                                                r0 + ch * C::kVRows, tok);
+                                                r0 + (ch + kVC / 2) % kVC * C::kVRows, tok);  // keys 64 on first
                             } else {
                                 tma_load_3d(st, &tK, &full_bar[stage], x + 64 * ch, r0, tok);
                             }
@@ -338,7 +338,7 @@ __global__ void __launch_bounds__(FCfg<D>::kThreads, 1)
                     const uint32_t v = v_lo + (uint32_t)(stage * kChunkLo);
 #pragma unroll
                     for (int kk = 0; kk < C::kVRows / 16; ++kk)
-                        umma_f16_ts_by(lead, o_base, tmem + (uint32_t)(pb * kBlk + (ch * C::kVRows + kk * 16) / 2),
+                        umma_f16_ts_by(lead, o_base, tmem + (uint32_t)(pb * kBlk + 64 + (ch * C::kVRows + kk * 16) / 2),
                                        sdesc(v + kk * 128, kDescHi), idesc_o, (j > 0 || ch > 0 || kk > 0) ? 1u : 0u);
                     next();
                 }
@@ -408,11 +408,13 @@ __global__ void __launch_bounds__(FCfg<D>::kThreads, 1)
                 tc_fence_after();
                 const bool diag = j == un.i;
                 float mx[2] = {-INFINITY, -INFINITY};
-#pragma unroll 1
-                for (int cc = 0; cc < 4; ++cc) {
-                    float x[32];
+                float xa[32], xb[32];
+                auto load = [&](float(&x)[32], int cc) {
                     tmem_ld32(s_tmem + (uint32_t)(cc * 32), *reinterpret_cast<uint32_t(*)[32]>(&x[0]));
-                    tmem_ld_wait();
+                };
+                // a chunk's part of the row maximum, its scores left signed and masked; a NaN score makes the maximum
+                // NaN, and with it the row
+                auto maximum = [&](float(&x)[32], int cc) {
                     if (args.sign != 1.0f) {
 #pragma unroll
                         for (int e = 0; e < 32; ++e) x[e] *= args.sign;
@@ -422,12 +424,23 @@ __global__ void __launch_bounds__(FCfg<D>::kThreads, 1)
                         for (int e = 0; e < 32; ++e)
                             if (cc * 32 + e > row || cc * 32 + e < shift) x[e] = -INFINITY;
                     }
-                    // a NaN score makes the maximum NaN, and with it the row
 #pragma unroll
                     for (int e = 0; e < 32; e += 4) {
                         mx[0] = max3_nan(mx[0], x[e], x[e + 1]);
                         mx[1] = max3_nan(mx[1], x[e + 2], x[e + 3]);
                     }
+                };
+                // each chunk on its way while the one before is worked on; the last two stay for the exponentials
+                load(xa, 0);
+                tmem_ld_wait();
+#pragma unroll 1
+                for (int h = 0; h < 2; ++h) {
+                    load(xb, 2 * h + 1);
+                    maximum(xa, 2 * h);
+                    tmem_ld_wait();
+                    if (h == 0) load(xa, 2);
+                    maximum(xb, 2 * h + 1);
+                    tmem_ld_wait();
                 }
                 const float top = max3_nan(mx[0], mx[1], mx[1]) * args.sl2;
                 float mn;
@@ -462,37 +475,38 @@ __global__ void __launch_bounds__(FCfg<D>::kThreads, 1)
                 if (j >= NB) l *= ex2_ftz(m - mn);
                 m = mn;
                 float2 s[2] = {both(0.0f), both(0.0f)};
-                const float2 sl2 = both(args.sl2 * args.sign), off = both(-m);
-#pragma unroll 1
-                for (int cc = 0; cc < 4; ++cc) {
-                    float x[32];
+                const float2 sl2 = both(args.sl2), off = both(-m);
+                // a chunk's P, as the at-th 16 of the buffer's last 64 columns: the scores there are read by then
+                auto probability = [&](float(&x)[32], int at) {
                     uint32_t pk[16];
-                    tmem_ld32(s_tmem + (uint32_t)(cc * 32), *reinterpret_cast<uint32_t(*)[32]>(&x[0]));
-                    tmem_ld_wait();
 #pragma unroll
                     for (int e = 0; e < 16; ++e) {
                         const float2 y = fma2(make_float2(x[2 * e], x[2 * e + 1]), sl2, off);
-                        x[2 * e] = ex2_ftz(y.x);
-                        x[2 * e + 1] = ex2_ftz(y.y);
+                        const float2 p2 = make_float2(ex2_ftz(y.x), ex2_ftz(y.y));
+                        s[e & 1] = add2(s[e & 1], p2);
+                        pk[e] = pack_bf16(p2.x, p2.y);
                     }
-                    if (diag) {
-#pragma unroll
-                        for (int e = 0; e < 32; ++e)
-                            if (cc * 32 + e > row || cc * 32 + e < shift) x[e] = 0.0f;
+                    tmem_st16(s_tmem + (uint32_t)(64 + at * 16), pk);
+                };
+                // keys 64 to 127, whose scores are here, then the others read again (signed and masked again: the
+                // mask of a tile's first half only ever falls on the diagonal's)
+#pragma unroll 1
+                for (int h = 0; h < 2; ++h) {
+                    probability(xa, 2 * h);
+                    if (h == 0) load(xa, 0);
+                    probability(xb, 2 * h + 1);
+                    if (h == 0) {
+                        load(xb, 1);
+                        tmem_ld_wait();
+                        if (args.sign != 1.0f || diag) {
+                            maximum(xa, 0);
+                            maximum(xb, 1);
+                        }
                     }
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) {
-                        s[e & 1] = add2(s[e & 1], make_float2(x[2 * e], x[2 * e + 1]));
-                        pk[e] = pack_bf16(x[2 * e], x[2 * e + 1]);
-                    }
-                    // over columns this thread has read: 32 scores become 16 columns
-                    tmem_st16(s_tmem + (uint32_t)(cc * 16), pk);
-                    if (cc & 1) {
-                        tmem_st_wait();
-                        tc_fence_before();
-                        __syncwarp();
-                        if (lane == 0) mbar_arrive(&p_full[2 * w + (cc >> 1)]);
-                    }
+                    tmem_st_wait();
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&p_full[2 * w + h]);
                 }
                 l += (s[0].x + s[0].y) + (s[1].x + s[1].y);
                 phase ^= 1u;
