@@ -586,9 +586,13 @@ struct BCfg {
     static constexpr bool kDP = KIND != kDV;          // needs dP (a second resident operand, delta)
     static constexpr bool kKeys = KIND != kDQ;        // rows are keys: lse and delta run along the columns
     static constexpr int kABytes = kBlk * D * 2;
-    static constexpr int kStages = D == 256 && kDP ? 6 : 9;
+    // At D = 128 the ring holds whole column blocks of 32 KB, each read by both of its products (K-major for the scores,
+    // MN-major for the accumulating one); at 256 it holds 16 KB chunks, loaded once for either.
+    static constexpr bool kWhole = D == 128;
+    static constexpr int kSlot = kWhole ? kABytes : kChunk;
+    static constexpr int kStages = kWhole ? 5 : (kDP ? 6 : 9);
     static constexpr int kRingOff = (kDP ? 2 : 1) * kABytes;
-    static constexpr int kBarOff = kRingOff + kStages * kChunk;
+    static constexpr int kBarOff = kRingOff + kStages * kSlot;
     static constexpr int kStatOff = kBarOff + 640;    // kKeys: float [2 (stage)][-lse log2 e, -delta][128]
     static constexpr int kSmemBytes = kStatOff + (kKeys ? 2048 : 0);
     static constexpr int kVRows = kChunk / (D * 2);
@@ -601,7 +605,7 @@ struct BwdArgs {
     int64_t ld_lse, ld_delta;
     __nv_bfloat16 *out0, *out1;        // kDQ: dq; kDKV: dv, dk; kDV: dv; kDK: dk
     int64_t tok0, head0, tok1, head1;
-    int32_t a0_head, a1_head, b0_head, b1_head, c0_head, c1_head;
+    int32_t a0_head, a1_head, b0_head, b1_head, c0_head;
     int32_t heads, grp;                // the rows' heads (query heads for kDQ, key/value heads else)
     // keys: the first split_blocks blocks' query heads go to `parts` units each, launched behind the first_blocks
     // blocks after them (whose whole units are longer)
@@ -660,11 +664,10 @@ template <int D, int KIND>
 __global__ void __launch_bounds__(kThreads, 1)
     bwd_kernel(const __grid_constant__ CUtensorMap tA0, const __grid_constant__ CUtensorMap tA1,
                const __grid_constant__ CUtensorMap tB0, const __grid_constant__ CUtensorMap tB1,
-               const __grid_constant__ CUtensorMap tC0, const __grid_constant__ CUtensorMap tC1, const BwdArgs args) {
+               const __grid_constant__ CUtensorMap tC0, const BwdArgs args) {
     using C = BCfg<D, KIND>;
     constexpr int ND = D / 64;
     constexpr int kVC = kBlk / C::kVRows;
-    constexpr int kUnrollChunks = D == 128 ? 2 : 1, kUnrollStreams = D == 128 ? 4 : 1;
     extern __shared__ __align__(1024) uint8_t smem[];
     uint8_t* ring = smem + C::kRingOff;
     uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + C::kBarOff);
@@ -727,7 +730,6 @@ __global__ void __launch_bounds__(kThreads, 1)
             tma_prefetch(&tA1);
             tma_prefetch(&tB1);
         }
-        if (KIND == kDKV) tma_prefetch(&tC1);
     }
     tc_fence_before();
     __syncthreads();
@@ -755,46 +757,67 @@ __global__ void __launch_bounds__(kThreads, 1)
                                         wk.h * (p ? args.a1_head : args.a0_head) + 64 * s, -wk.shift(), wk.tok0);
                     }
                 }
-                // a step's streams, in the order the products take them: the next tile's column block for S (K-major), this
-                // tile's for the accumulating products (MN-major), the next tile's for dP. Rolled at D = 256: the warps
-                // share an instruction cache that unrolled copies do not fit in beside the softmax.
                 int blk0 = 0, head0 = 0, blk1 = wk.first_block(), head1 = wk.first_head();  // of tiles j and j + 1
-#pragma unroll 1
-                for (int j = -1; j < wk.tiles && ok; ++j) {
-                    if (p && j + 1 == wk.tiles && !(ok = queue.ask(lt, lead))) break;
-#pragma unroll kUnrollStreams
-                    for (int s = 0; s < 4 && ok; ++s) {
-                        const bool mn = s == 1 || s == 2;
-                        const int tile = mn ? j : j + 1;
-                        if (tile < 0 || tile >= wk.tiles || (s == 2 && KIND != kDKV) || (s == 3 && !C::kDP)) continue;
-                        const CUtensorMap* map = s == 0 ? &tB0 : (s == 1 ? &tC0 : (s == 2 ? &tC1 : &tB1));
-                        const int head_stride =
-                            s == 0 ? args.b0_head : (s == 1 ? args.c0_head : (s == 2 ? args.c1_head : args.b1_head));
-                        const int blk = mn ? blk0 : blk1, x = (mn ? head0 : head1) * head_stride;
-                        const int r0 = -wk.shift_of(blk), tok = wk.seq0 + blk * kBlk;
-#pragma unroll kUnrollChunks
-                        for (int ch = p; ch < (mn ? kVC : ND); ch += 2) {
-                            if (!(ok = warp_wait(&empty_bar[stage], phase ^ 1u, abort_flag))) break;
-                            if (lead) {
-                                uint8_t* st = ring + stage * kChunk;
-                                mbar_expect_tx(&full_bar[stage], kChunk);
-                                if (mn) {
+                if constexpr (C::kWhole) {
+                    // each of the two warps its operand's blocks, in slots taken in turn
+                    const CUtensorMap* map = p ? &tB1 : &tB0;
+                    const int head_stride = p ? args.b1_head : args.b0_head;
+                    for (int j = 0; j < wk.tiles && ok; ++j) {
+                        if (p && j + 1 == wk.tiles && !(ok = queue.ask(lt, lead))) break;
+                        if (!(ok = warp_wait(&empty_bar[stage], phase ^ 1u, abort_flag))) break;
+                        if (lead) {
+                            mbar_expect_tx(&full_bar[stage], C::kSlot);
 #pragma unroll
-                                    for (int n = 0; n < ND; ++n)
-                                        tma_load_3d(st + n * (C::kVRows * 128), map, &full_bar[stage], x + 64 * n,
-                                                    ch * C::kVRows + r0, tok);
-                                } else {
-                                    tma_load_3d(st, map, &full_bar[stage], x + 64 * ch, r0, tok);
+                            for (int ch = 0; ch < ND; ++ch)
+                                tma_load_3d(ring + stage * C::kSlot + ch * kChunk, map, &full_bar[stage],
+                                            head1 * head_stride + 64 * ch, -wk.shift_of(blk1), wk.seq0 + blk1 * kBlk);
+                        }
+                        if ((stage += 2) >= C::kStages) {
+                            stage -= C::kStages;
+                            phase ^= 1u;
+                        }
+                        wk.step(blk1, head1);
+                    }
+                } else {
+                    // a step's streams, in the order the products take them: the next tile's column block for S (K-major), this
+                    // tile's for the accumulating product (MN-major), the next tile's for dP. Rolled: the warps share an
+                    // instruction cache that unrolled copies do not fit in beside the softmax.
+#pragma unroll 1
+                    for (int j = -1; j < wk.tiles && ok; ++j) {
+                        if (p && j + 1 == wk.tiles && !(ok = queue.ask(lt, lead))) break;
+#pragma unroll 1
+                        for (int s = 0; s < 3 && ok; ++s) {
+                            const bool mn = s == 1;
+                            const int tile = mn ? j : j + 1;
+                            if (tile < 0 || tile >= wk.tiles || (s == 2 && !C::kDP)) continue;
+                            const CUtensorMap* map = s == 0 ? &tB0 : (s == 1 ? &tC0 : &tB1);
+                            const int head_stride = s == 0 ? args.b0_head : (s == 1 ? args.c0_head : args.b1_head);
+                            const int blk = mn ? blk0 : blk1, x = (mn ? head0 : head1) * head_stride;
+                            const int r0 = -wk.shift_of(blk), tok = wk.seq0 + blk * kBlk;
+#pragma unroll 1
+                            for (int ch = p; ch < (mn ? kVC : ND); ch += 2) {
+                                if (!(ok = warp_wait(&empty_bar[stage], phase ^ 1u, abort_flag))) break;
+                                if (lead) {
+                                    uint8_t* st = ring + stage * kChunk;
+                                    mbar_expect_tx(&full_bar[stage], kChunk);
+                                    if (mn) {
+#pragma unroll
+                                        for (int n = 0; n < ND; ++n)
+                                            tma_load_3d(st + n * (C::kVRows * 128), map, &full_bar[stage], x + 64 * n,
+                                                        ch * C::kVRows + r0, tok);
+                                    } else {
+                                        tma_load_3d(st, map, &full_bar[stage], x + 64 * ch, r0, tok);
+                                    }
+                                }
+                                if ((stage += 2) >= C::kStages) {
+                                    stage -= C::kStages;
+                                    phase ^= 1u;
                                 }
                             }
-                            if ((stage += 2) >= C::kStages) {
-                                stage -= C::kStages;
-                                phase ^= 1u;
-                            }
                         }
+                        blk0 = blk1, head0 = head1;
+                        wk.step(blk1, head1);
                     }
-                    blk0 = blk1, head0 = head1;
-                    wk.step(blk1, head1);
                 }
             }
         } else if (warp == 1) {
@@ -806,7 +829,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             uint32_t phase = 0;
             bool ok = true;
             const uint32_t a_lo = sdesc_lo(smem_u32(smem), 16);
-            const uint32_t b_lo = sdesc_lo(smem_u32(ring), 16), c_lo = sdesc_lo(smem_u32(ring), C::kVRows * 128);
+            const uint32_t b_lo = sdesc_lo(smem_u32(ring), 16);
+            const uint32_t c_lo = sdesc_lo(smem_u32(ring), C::kWhole ? kChunk : C::kVRows * 128);
             auto chunk = [&]() -> bool {  // the next ring chunk is there
                 ok = ok && warp_wait(&full_bar[stage], phase, abort_flag);
                 tc_fence_after();
@@ -819,30 +843,64 @@ __global__ void __launch_bounds__(kThreads, 1)
                     phase ^= 1u;
                 }
             };
+            // kWhole: the tile's operand `which` (0, 1) is in slot (2 tile + which) % kStages
             auto score = [&](int resident, uint32_t d) {
-#pragma unroll kUnrollChunks
-                for (int kb = 0; kb < ND; ++kb) {
-                    if (!chunk()) return;
-                    const uint32_t a = a_lo + (uint32_t)(resident * (C::kABytes >> 4) + kb * kChunkLo);
-                    const uint32_t b = b_lo + (uint32_t)(stage * kChunkLo);
+                if constexpr (C::kWhole) {
+                    ok = ok && warp_wait(&full_bar[stage], phase, abort_flag);
+                    tc_fence_after();
+                    if (!ok) return;
 #pragma unroll
-                    for (int kk = 0; kk < 4; ++kk)
-                        umma_f16_by(lead, d, sdesc(a + kk * 2, kDescHi), sdesc(b + kk * 2, kDescHi), idesc_s,
-                                    (kb > 0 || kk > 0) ? 1u : 0u);
-                    next();
+                    for (int kb = 0; kb < ND; ++kb) {
+                        const uint32_t a = a_lo + (uint32_t)(resident * (C::kABytes >> 4) + kb * kChunkLo);
+                        const uint32_t b = b_lo + (uint32_t)(stage * (C::kSlot >> 4) + kb * kChunkLo);
+#pragma unroll
+                        for (int kk = 0; kk < 4; ++kk)
+                            umma_f16_by(lead, d, sdesc(a + kk * 2, kDescHi), sdesc(b + kk * 2, kDescHi), idesc_s,
+                                        (kb > 0 || kk > 0) ? 1u : 0u);
+                    }
+                    if (KIND == kDQ && resident == 1) umma_commit_by(lead, &empty_bar[stage]);  // V is not read again
+                    if (++stage == C::kStages) {
+                        stage = 0;
+                        phase ^= 1u;
+                    }
+                } else {
+#pragma unroll 1
+                    for (int kb = 0; kb < ND; ++kb) {
+                        if (!chunk()) return;
+                        const uint32_t a = a_lo + (uint32_t)(resident * (C::kABytes >> 4) + kb * kChunkLo);
+                        const uint32_t b = b_lo + (uint32_t)(stage * kChunkLo);
+#pragma unroll
+                        for (int kk = 0; kk < 4; ++kk)
+                            umma_f16_by(lead, d, sdesc(a + kk * 2, kDescHi), sdesc(b + kk * 2, kDescHi), idesc_s,
+                                        (kb > 0 || kk > 0) ? 1u : 0u);
+                        next();
+                    }
                 }
             };
-            auto accumulate = [&](uint32_t a, uint32_t d, bool first) {
-#pragma unroll kUnrollChunks
-                for (int ch = 0; ch < kVC; ++ch) {
-                    if (!chunk()) return;
-                    const uint32_t b = c_lo + (uint32_t)(stage * kChunkLo);
+            // d (+)= a x the tile's operand `which`, MN-major
+            int held = 0;  // kWhole: the slot of the tile's operand 0
+            auto accumulate = [&](uint32_t a, uint32_t d, bool first, int which) {
+                if constexpr (C::kWhole) {
+                    int at = held + which;
+                    if (at >= C::kStages) at -= C::kStages;
+                    const uint32_t b = c_lo + (uint32_t)(at * (C::kSlot >> 4));
 #pragma unroll
-                    for (int kk = 0; kk < C::kVRows / 16; ++kk) {
-                        umma_f16_ts_by(lead, d, a + (uint32_t)quarter_col(ch * (C::kVRows / 16) + kk),
-                                       sdesc(b + kk * 128, kDescHi), idesc_c, (!first || ch > 0 || kk > 0) ? 1u : 0u);
+                    for (int k16 = 0; k16 < kBlk / 16; ++k16)
+                        umma_f16_ts_by(lead, d, a + (uint32_t)quarter_col(k16), sdesc(b + k16 * 128, kDescHi), idesc_c,
+                                       (!first || k16 > 0) ? 1u : 0u);
+                    umma_commit_by(lead, &empty_bar[at]);
+                } else {
+#pragma unroll 1
+                    for (int ch = 0; ch < kVC; ++ch) {
+                        if (!chunk()) return;
+                        const uint32_t b = c_lo + (uint32_t)(stage * kChunkLo);
+#pragma unroll
+                        for (int kk = 0; kk < C::kVRows / 16; ++kk) {
+                            umma_f16_ts_by(lead, d, a + (uint32_t)quarter_col(ch * (C::kVRows / 16) + kk),
+                                           sdesc(b + kk * 128, kDescHi), idesc_c, (!first || ch > 0 || kk > 0) ? 1u : 0u);
+                        }
+                        next();
                     }
-                    next();
                 }
             };
             auto wait = [&](uint64_t* bar, int n) {  // the bar's n-th completion
@@ -880,8 +938,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                         wait(ds_full, gj);
                     if (j == 0) wait(acc_empty, lt + 1);
                     if (!ok) break;
-                    accumulate(tmem + (uint32_t)(KIND == kDV ? b * kBlk : kBlk), acc0, j == 0);
-                    if (KIND == kDKV) accumulate(tmem + (uint32_t)(kBlk + 16), acc1, j == 0);
+                    accumulate(tmem + (uint32_t)(KIND == kDV ? b * kBlk : kBlk), acc0, j == 0, KIND == kDKV ? 1 : 0);
+                    if (KIND == kDKV) accumulate(tmem + (uint32_t)(kBlk + 16), acc1, j == 0, 0);
+                    if ((held += 2) >= C::kStages) held -= C::kStages;
                     if (more && C::kDP) issue_dp(j + 1);
                 }
                 if (!ok) break;
@@ -1164,16 +1223,14 @@ int launch_bwd(const R97bPacked& p, const R97bAttnPackedBwd& a, const float* del
     const bool dq = KIND == kDQ;
     // the rows' operands, the columns' and the accumulating products'
     const R97bHeadRows &a0 = dq ? a.q : a.k, &a1 = dq ? a.dout : a.v, &b0 = dq ? a.k : a.q, &b1 = dq ? a.v : a.dout;
-    const R97bHeadRows &c0 = dq ? a.k : (KIND == kDK ? a.q : a.dout), &c1 = a.q;
+    const R97bHeadRows& c0 = dq ? a.k : (KIND == kDK ? a.q : a.dout);  // (kWhole: the accumulating products reuse b0, b1)
     const int ha = dq ? a.Hq : a.Hkv, hb = dq ? a.Hkv : a.Hq;
-    CUtensorMap m[6];
-    if (!make_rows_map(&m[0], a0, ha, D, p.T, kBlk) || !make_rows_map(&m[2], b0, hb, D, p.T, kBlk) ||
-        !make_rows_map(&m[4], c0, hb, D, p.T, C::kVRows))
-        return R97B_EINVAL;
-    m[1] = m[0], m[3] = m[2], m[5] = m[4];  // where the kind has no such stream
+    CUtensorMap m[5];
+    if (!make_rows_map(&m[0], a0, ha, D, p.T, kBlk) || !make_rows_map(&m[2], b0, hb, D, p.T, kBlk)) return R97B_EINVAL;
+    m[1] = m[0], m[3] = m[2], m[4] = m[2];  // where the kind has no such stream
     if (C::kDP && (!make_rows_map(&m[1], a1, ha, D, p.T, kBlk) || !make_rows_map(&m[3], b1, hb, D, p.T, kBlk)))
         return R97B_EINVAL;
-    if (KIND == kDKV && !make_rows_map(&m[5], c1, a.Hq, D, p.T, C::kVRows)) return R97B_EINVAL;
+    if (!C::kWhole && !make_rows_map(&m[4], c0, hb, D, p.T, C::kVRows)) return R97B_EINVAL;
     BwdArgs r{};
     r.blocks = reinterpret_cast<const int4*>(dq ? p.q_blocks : p.k_blocks);
     r.lse = a.lse, r.ld_lse = a.ld_lse, r.delta = delta, r.ld_delta = delta_ld(p.T);
@@ -1181,14 +1238,14 @@ int launch_bwd(const R97bPacked& p, const R97bAttnPackedBwd& a, const float* del
     r.out0 = reinterpret_cast<__nv_bfloat16*>(o0.ptr), r.tok0 = o0.tok, r.head0 = o0.head;
     r.out1 = reinterpret_cast<__nv_bfloat16*>(o1.ptr), r.tok1 = o1.tok, r.head1 = o1.head;
     r.a0_head = (int32_t)a0.head, r.a1_head = (int32_t)a1.head, r.b0_head = (int32_t)b0.head, r.b1_head = (int32_t)b1.head;
-    r.c0_head = (int32_t)c0.head, r.c1_head = (int32_t)c1.head;
+    r.c0_head = (int32_t)c0.head;
     r.heads = ha, r.grp = a.Hq / a.Hkv;
     r.split_blocks = dq ? 0 : split.blocks, r.parts = split.parts, r.first_blocks = dq ? 0 : split.first;
     r.part0 = KIND == kDK ? dk_parts : dv_parts, r.part1 = dk_parts;
     r.sl2 = a.scale * kLog2e, r.scale = a.scale;
     const int units = (p.n_blocks + (dq ? 0 : split.blocks * (split.parts - 1))) * ha;
     if (!smem_opt_in(bwd_kernel<D, KIND>, C::kSmemBytes)) return R97B_ELAUNCH;
-    bwd_kernel<D, KIND><<<units, kThreads, C::kSmemBytes, st>>>(m[0], m[1], m[2], m[3], m[4], m[5], r);
+    bwd_kernel<D, KIND><<<units, kThreads, C::kSmemBytes, st>>>(m[0], m[1], m[2], m[3], m[4], r);
     return launch_status();
 }
 
