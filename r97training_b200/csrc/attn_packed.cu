@@ -233,6 +233,8 @@ __global__ void __launch_bounds__(FCfg<D>::kThreads, 1)
     const uint32_t tmem = __shfl_sync(0xFFFFFFFFu, *tmem_slot, 0);
     const uint32_t o_base = tmem + (uint32_t)(NB * kBlk);
 
+    // Producers and MMA issuer walk the CTA's tiles with two cursors: S of a tile (and its K) NB - 1 tiles ahead of P V
+    // (and its V), across the units' borders too, so that a unit's first softmax runs beside the last one's.
     if (warp == 0 || warp == 3) {
         // ------------------------------------------------------------- TMA producers: every other chunk each
         const uint32_t lead = elect_one();
@@ -240,49 +242,76 @@ __global__ void __launch_bounds__(FCfg<D>::kThreads, 1)
         int stage = p;
         uint32_t phase = 0;
         bool ok = true;
-        for (int u = blockIdx.x, lt = 0; ok && u >= 0; u = ok ? queue.next(lt) : -1, ++lt) {
-            const Unit un = unit_geom(args.blocks, args.Hq, u);
-            const int shift = kBlk - un.n, kvh = un.h / args.grp;
-            const int seq0 = un.tok0 - un.i * kBlk;
-            const int qs = lt % C::kQStages;
-            if (!(ok = warp_wait(&q_empty[qs], (uint32_t)((lt / C::kQStages) & 1) ^ 1u, abort_flag))) break;
-            if (lead) {
-                mbar_expect_tx(&q_full[qs], C::kQBytes / 2);
-                for (int s = p; s < ND; s += 2)
-                    tma_load_3d(smem + qs * C::kQBytes + s * kChunk, &tQ, &q_full[qs], un.h * args.q_head + 64 * s, -shift,
-                                un.tok0);
-            }
-            // K of a tile NB - 1 ahead of V
-#pragma unroll 1
-            for (int j = 1 - NB; j <= un.i && ok; ++j) {
-                if (p && j == un.i && !(ok = queue.ask(lt, lead))) break;
+        struct Cursor {
+            int x, seq0, i, shift, j;
+        };
+        Cursor ahead{}, behind{}, w0{}, w1{};  // w0, w1: the units between, oldest first
+        int waiting = 0, led = 0, lt = 0;
+        bool more = true, fresh = true;  // a unit for `ahead`; its Q not loaded yet
+        int u = blockIdx.x;
+        auto load = [&](bool v, const Cursor& c) {
+            const int tok = c.seq0 + c.j * kBlk, r0 = c.j == c.i ? -c.shift : 0;
+            const int x = c.x * (v ? args.v_head : args.k_head);
 #pragma unroll
-                for (int v = 0; v < 2; ++v) {
-                    const int tile = v ? j : j + NB - 1;
-                    if (tile < 0 || tile > un.i) continue;
-                    const int tok = seq0 + tile * kBlk, r0 = tile == un.i ? -shift : 0;
-                    const int x = kvh * (v ? args.v_head : args.k_head);
+            for (int ch = p; ch < (v ? kVC : ND); ch += 2) {
+                if (!(ok = ok && warp_wait(&empty_bar[stage], phase ^ 1u, abort_flag))) return;
+                if (lead) {
+                    uint8_t* st = ring + stage * kChunk;
+                    mbar_expect_tx(&full_bar[stage], kChunk);
+                    if (v) {
 #pragma unroll
-                    for (int ch = p; ch < (v ? kVC : ND); ch += 2) {
-                        if (!(ok = ok && warp_wait(&empty_bar[stage], phase ^ 1u, abort_flag))) break;
-                        if (lead) {
-                            uint8_t* st = ring + stage * kChunk;
-                            mbar_expect_tx(&full_bar[stage], kChunk);
-                            if (v) {
-#pragma unroll
-                                for (int n = 0; n < ND; ++n)
-                                    tma_load_3d(st + n * (C::kVRows * 128), &tV, &full_bar[stage], x + 64 * n,
-                                                r0 + (ch + kVC / 2) % kVC * C::kVRows, tok);  // keys 64 on first
-                            } else {
-                                tma_load_3d(st, &tK, &full_bar[stage], x + 64 * ch, r0, tok);
-                            }
-                        }
-                        if ((stage += 2) >= C::kStages) {
-                            stage -= C::kStages;
-                            phase ^= 1u;
-                        }
+                        for (int n = 0; n < ND; ++n)
+                            tma_load_3d(st + n * (C::kVRows * 128), &tV, &full_bar[stage], x + 64 * n,
+                                        r0 + (ch + kVC / 2) % kVC * C::kVRows, tok);  // keys 64 on first
+                    } else {
+                        tma_load_3d(st, &tK, &full_bar[stage], x + 64 * ch, r0, tok);
                     }
                 }
+                if ((stage += 2) >= C::kStages) {
+                    stage -= C::kStages;
+                    phase ^= 1u;
+                }
+            }
+        };
+        while (ok) {
+            if (fresh) {  // the next unit, or none
+                if (lt > 0) u = queue.next(lt - 1);
+                fresh = false;
+                more = u >= 0;
+                if (more) {
+                    const Unit un = unit_geom(args.blocks, args.Hq, u);
+                    ahead = Cursor{un.h / args.grp, un.tok0 - un.i * kBlk, un.i, kBlk - un.n, 0};
+                    const int qs = lt % C::kQStages;
+                    if (!(ok = warp_wait(&q_empty[qs], (uint32_t)((lt / C::kQStages) & 1) ^ 1u, abort_flag))) break;
+                    if (lead) {
+                        mbar_expect_tx(&q_full[qs], C::kQBytes / 2);
+                        for (int s = p; s < ND; s += 2)
+                            tma_load_3d(smem + qs * C::kQBytes + s * kChunk, &tQ, &q_full[qs], un.h * args.q_head + 64 * s,
+                                        -ahead.shift, un.tok0);
+                    }
+                    if (waiting == 0) {
+                        behind = ahead;
+                    } else if (waiting == 1) {
+                        w0 = ahead;
+                    } else {
+                        w1 = ahead;
+                    }
+                    ++waiting;
+                    ++lt;
+                }
+            }
+            if (more) {
+                if (p && ahead.j == ahead.i && !(ok = queue.ask(lt - 1, lead))) break;
+                load(false, ahead);
+                fresh = ++ahead.j > ahead.i;
+                if (++led < NB) continue;
+            }
+            if (led == 0) break;
+            load(true, behind);
+            --led;
+            if (++behind.j > behind.i) {
+                behind = w0, w0 = w1;
+                --waiting;
             }
         }
     } else if (warp == 1) {
@@ -301,56 +330,83 @@ __global__ void __launch_bounds__(FCfg<D>::kThreads, 1)
                 phase ^= 1u;
             }
         };
-        for (int u = blockIdx.x, lt = 0; ok && u >= 0; u = ok ? queue.next(lt) : -1, ++lt) {
-            const int nt = unit_geom(args.blocks, args.Hq, u).i + 1;
-            const int qs = lt % C::kQStages;
-            if (!(ok = warp_wait(&q_full[qs], (uint32_t)((lt / C::kQStages) & 1), abort_flag))) break;
-            tc_fence_after();
-            const uint32_t q_lo = sdesc_lo(smem_u32(smem), 16) + (uint32_t)(qs * (C::kQBytes >> 4));
-#pragma unroll 1
-            for (int j = 1 - NB; j < nt && ok; ++j) {
-                const int js = j + NB - 1;
-                if (js < nt) {
-                    // S into the buffer whose last P V is already before it in the issue order
-#pragma unroll
-                    for (int kb = 0; kb < ND; ++kb) {
-                        if (!(ok = ok && warp_wait(&full_bar[stage], phase, abort_flag))) break;
-                        tc_fence_after();
-                        const uint32_t a = q_lo + (uint32_t)(kb * kChunkLo), b = k_lo + (uint32_t)(stage * kChunkLo);
-#pragma unroll
-                        for (int kk = 0; kk < 4; ++kk)
-                            umma_f16_by(lead, tmem + (uint32_t)(sb * kBlk), sdesc(a + kk * 2, kDescHi),
-                                        sdesc(b + kk * 2, kDescHi), idesc_s, (kb > 0 || kk > 0) ? 1u : 0u);
-                        next();
+        int js = 0, ns = 0, jp = 0, np = 0, w0 = 0, w1 = 0;  // tile and tiles of the units at S and at P V; those between
+        int waiting = 0, led = 0, lt = 0, lt_p = 0;
+        uint32_t q_lo = 0;
+        bool more = true, fresh = true;
+        int u = blockIdx.x;
+        while (ok) {
+            if (fresh) {
+                if (lt > 0) u = queue.next(lt - 1);
+                fresh = false;
+                more = u >= 0;
+                if (more) {
+                    ns = unit_geom(args.blocks, args.Hq, u).i + 1;
+                    js = 0;
+                    const int qs = lt % C::kQStages;
+                    if (!(ok = warp_wait(&q_full[qs], (uint32_t)((lt / C::kQStages) & 1), abort_flag))) break;
+                    q_lo = sdesc_lo(smem_u32(smem), 16) + (uint32_t)(qs * (C::kQBytes >> 4));
+                    if (waiting == 0) {
+                        np = ns;
+                    } else if (waiting == 1) {
+                        w0 = ns;
+                    } else {
+                        w1 = ns;
                     }
-                    if (!ok) break;
-                    umma_commit_by(lead, &s_full[sb]);
-                    if (js + 1 == nt) umma_commit_by(lead, &q_empty[qs]);
-                    if (++sb == NB) sb = 0;
+                    ++waiting;
+                    ++lt;
                 }
-                if (j < 0) continue;
-                if (j == 0 && !(ok = warp_wait(o_empty, (uint32_t)(lt & 1) ^ 1u, abort_flag))) break;
+            }
+            if (more) {
+                // S into the buffer whose last P V is already before it in the issue order
 #pragma unroll
-                for (int ch = 0; ch < kVC; ++ch) {
-                    if (ch % (kVC / 2) == 0) ok = ok && warp_wait(&p_full[2 * pb + ch / (kVC / 2)], p_phase, abort_flag);
+                for (int kb = 0; kb < ND; ++kb) {
                     if (!(ok = ok && warp_wait(&full_bar[stage], phase, abort_flag))) break;
                     tc_fence_after();
-                    const uint32_t v = v_lo + (uint32_t)(stage * kChunkLo);
+                    const uint32_t a = q_lo + (uint32_t)(kb * kChunkLo), b = k_lo + (uint32_t)(stage * kChunkLo);
 #pragma unroll
-                    for (int kk = 0; kk < C::kVRows / 16; ++kk)
-                        umma_f16_ts_by(lead, o_base, tmem + (uint32_t)(pb * kBlk + 64 + (ch * C::kVRows + kk * 16) / 2),
-                                       sdesc(v + kk * 128, kDescHi), idesc_o, (j > 0 || ch > 0 || kk > 0) ? 1u : 0u);
+                    for (int kk = 0; kk < 4; ++kk)
+                        umma_f16_by(lead, tmem + (uint32_t)(sb * kBlk), sdesc(a + kk * 2, kDescHi),
+                                    sdesc(b + kk * 2, kDescHi), idesc_s, (kb > 0 || kk > 0) ? 1u : 0u);
                     next();
                 }
                 if (!ok) break;
-                umma_commit_by(lead, &pv_done[pb]);
-                if (++pb == NB) {
-                    pb = 0;
-                    p_phase ^= 1u;
+                umma_commit_by(lead, &s_full[sb]);
+                if (++sb == NB) sb = 0;
+                if (++js == ns) {
+                    umma_commit_by(lead, &q_empty[(lt - 1) % C::kQStages]);
+                    fresh = true;
                 }
+                if (++led < NB) continue;
+            }
+            if (led == 0) break;
+            if (jp == 0 && !(ok = warp_wait(o_empty, (uint32_t)(lt_p & 1) ^ 1u, abort_flag))) break;
+#pragma unroll
+            for (int ch = 0; ch < kVC; ++ch) {
+                if (ch % (kVC / 2) == 0) ok = ok && warp_wait(&p_full[2 * pb + ch / (kVC / 2)], p_phase, abort_flag);
+                if (!(ok = ok && warp_wait(&full_bar[stage], phase, abort_flag))) break;
+                tc_fence_after();
+                const uint32_t v = v_lo + (uint32_t)(stage * kChunkLo);
+#pragma unroll
+                for (int kk = 0; kk < C::kVRows / 16; ++kk)
+                    umma_f16_ts_by(lead, o_base, tmem + (uint32_t)(pb * kBlk + 64 + (ch * C::kVRows + kk * 16) / 2),
+                                   sdesc(v + kk * 128, kDescHi), idesc_o, (jp > 0 || ch > 0 || kk > 0) ? 1u : 0u);
+                next();
             }
             if (!ok) break;
-            umma_commit_by(lead, o_full);
+            umma_commit_by(lead, &pv_done[pb]);
+            if (++pb == NB) {
+                pb = 0;
+                p_phase ^= 1u;
+            }
+            --led;
+            if (++jp == np) {
+                umma_commit_by(lead, o_full);
+                ++lt_p;
+                jp = 0;
+                np = w0, w0 = w1;
+                --waiting;
+            }
         }
     } else if (warp >= 4) {
         // ------------------------------------------------------------- softmax
@@ -412,45 +468,53 @@ __global__ void __launch_bounds__(FCfg<D>::kThreads, 1)
                 auto load = [&](float(&x)[32], int cc) {
                     tmem_ld32(s_tmem + (uint32_t)(cc * 32), *reinterpret_cast<uint32_t(*)[32]>(&x[0]));
                 };
-                // a chunk's part of the row maximum, its scores left signed and masked; a NaN score makes the maximum
-                // NaN, and with it the row
-                auto maximum = [&](float(&x)[32], int cc) {
-                    if (args.sign != 1.0f) {
-#pragma unroll
-                        for (int e = 0; e < 32; ++e) x[e] *= args.sign;
-                    }
-                    if (diag) {
-#pragma unroll
-                        for (int e = 0; e < 32; ++e)
-                            if (cc * 32 + e > row || cc * 32 + e < shift) x[e] = -INFINITY;
-                    }
+                // a chunk's part of the row maximum; a NaN score makes it NaN, and with it the row
+                auto maximum = [&](const float(&x)[32]) {
 #pragma unroll
                     for (int e = 0; e < 32; e += 4) {
                         mx[0] = max3_nan(mx[0], x[e], x[e + 1]);
                         mx[1] = max3_nan(mx[1], x[e + 2], x[e + 3]);
                     }
                 };
+                // Signs and masks are put into the buffer beforehand, a chunk at a time in one small loop: code for them
+                // where the scores are used is fetched cold on every diagonal tile and cost more than this pass. On the
+                // diagonal a warp's rows see the chunks before theirs whole.
+                if (args.sign != 1.0f || diag) {
+#pragma unroll 1
+                    for (int cc = 0; cc < 4; ++cc) {
+                        if (args.sign == 1.0f && cc < q && cc * 32 >= shift) continue;
+                        load(xa, cc);
+                        tmem_ld_wait();
+                        const int hi = diag ? row - cc * 32 : 32, lo = diag ? shift - cc * 32 : 0;
+                        const uint32_t upto = hi < 0 ? 0u : (hi >= 31 ? ~0u : (2u << hi) - 1u);
+                        const uint32_t seen = upto & (lo <= 0 ? ~0u : (lo >= 32 ? 0u : ~0u << lo));
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) xa[e] = seen & (1u << e) ? xa[e] * args.sign : -INFINITY;
+                        tmem_st32(s_tmem + (uint32_t)(cc * 32), *reinterpret_cast<uint32_t(*)[32]>(&xa[0]));
+                    }
+                    tmem_st_wait();
+                }
                 // each chunk on its way while the one before is worked on; the last two stay for the exponentials
                 load(xa, 0);
                 tmem_ld_wait();
 #pragma unroll 1
                 for (int h = 0; h < 2; ++h) {
                     load(xb, 2 * h + 1);
-                    maximum(xa, 2 * h);
+                    maximum(xa);
                     tmem_ld_wait();
                     if (h == 0) load(xa, 2);
-                    maximum(xb, 2 * h + 1);
+                    maximum(xb);
                     tmem_ld_wait();
                 }
                 const float top = max3_nan(mx[0], mx[1], mx[1]) * args.sl2;
-                float mn;
-                if (j == 0) {
-                    mn = top == -INFINITY ? 0.0f : top;  // a row of nothing visible (or of -inf scores) sums to 0
-                } else {
-                    // the last unit's result before any wait on this unit's tiles: their first P V waits for its drain
-                    if (d_lt >= 0 && !(ok = drain())) break;
-                    // the tile before this one is of the same turn of the buffers, or (buffer 0) of the last
-                    if (!(ok = warp_wait(&max_bar[prev * 4 + q], w == 0 ? phase ^ 1u : phase, abort_flag))) break;
+                // The tile before this one is of the same turn of the buffers, or (buffer 0) of the last. Its reference is
+                // waited for even where it is another unit's: whoever publishes has read the one before, so that none
+                // is overwritten unread. The last unit's result is drained before any wait on this unit's tiles, whose
+                // first P V waits for it.
+                if (j > 0 && d_lt >= 0 && !(ok = drain())) break;
+                if (!(ok = warp_wait(&max_bar[prev * 4 + q], w == 0 ? phase ^ 1u : phase, abort_flag))) break;
+                float mn = top == -INFINITY ? 0.0f : top;  // a row of nothing visible (or of -inf scores) sums to 0
+                if (j > 0) {
                     const float mp = ref_m[prev * 128 + row];
                     mn = top <= mp + kLazy ? mp : top;
                     if (__any_sync(0xFFFFFFFFu, mn != mp)) {
@@ -488,8 +552,7 @@ __global__ void __launch_bounds__(FCfg<D>::kThreads, 1)
                     }
                     tmem_st16(s_tmem + (uint32_t)(64 + at * 16), pk);
                 };
-                // keys 64 to 127, whose scores are here, then the others read again (signed and masked again: the
-                // mask of a tile's first half only ever falls on the diagonal's)
+                // keys 64 to 127, whose scores are here, then the others read again
 #pragma unroll 1
                 for (int h = 0; h < 2; ++h) {
                     probability(xa, 2 * h);
@@ -498,10 +561,6 @@ __global__ void __launch_bounds__(FCfg<D>::kThreads, 1)
                     if (h == 0) {
                         load(xb, 1);
                         tmem_ld_wait();
-                        if (args.sign != 1.0f || diag) {
-                            maximum(xa, 0);
-                            maximum(xb, 1);
-                        }
                     }
                     tmem_st_wait();
                     tc_fence_before();
@@ -1059,12 +1118,12 @@ __global__ void __launch_bounds__(kThreads, 1)
                     p[2 * e] = ex2_ftz(y.x);
                     p[2 * e + 1] = ex2_ftz(y.y);
                 }
-                if (diag) {
+                // on the diagonal only the warp's own 32 columns are seen in part, those on one side not at all
+                if (diag && (C::kKeys ? w <= q : (w >= q || w * 32 < shift))) {
+                    const int at = row - w * 32, lo = shift - w * 32;
 #pragma unroll
-                    for (int e = 0; e < 32; ++e) {
-                        const int col = w * 32 + e;
-                        if (C::kKeys ? col < row : (col > row || col < shift)) p[e] = 0.0f;
-                    }
+                    for (int e = 0; e < 32; ++e)
+                        if (C::kKeys ? e < at : (e > at || e < lo)) p[e] = 0.0f;
                 }
                 uint32_t pk[16];
                 if (KIND == kDV || KIND == kDKV) {
