@@ -653,14 +653,14 @@ struct BCfg {
     static constexpr int kRingOff = (kDP ? 2 : 1) * kABytes;
     static constexpr int kBarOff = kRingOff + kStages * kSlot;
     static constexpr int kStatOff = kBarOff + 640;    // kKeys: float [2 (stage)][-lse log2 e, -delta][128]
-    static constexpr int kSmemBytes = kStatOff + (kKeys ? 2048 : 0);
+    static constexpr int kSmemBytes = kStatOff + 2048;  // kDQ: float [4][128], a row's P o dP by column quarter
     static constexpr int kVRows = kChunk / (D * 2);
 };
 
 struct BwdArgs {
     const int4* blocks;
     const float* lse;
-    const float* delta;
+    float* delta;
     int64_t ld_lse, ld_delta;
     __nv_bfloat16 *out0, *out1;        // kDQ: dq; kDKV: dv, dk; kDV: dv; kDK: dk
     int64_t tok0, head0, tok1, head1;
@@ -747,6 +747,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint64_t* acc_empty = acc_full + 1;
     uint64_t* stat_full = acc_empty + 1;         // [2]
     uint64_t* stat_empty = stat_full + 2;        // [2]
+    uint64_t* sum_bar = stat_empty + 2;          // [4] kDQ: a lane quarter's row sums written
     float* stats = reinterpret_cast<float*>(smem + C::kStatOff);
 
     const int warp = __shfl_sync(0xFFFFFFFFu, threadIdx.x >> 5, 0);
@@ -769,6 +770,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             mbar_init(&stat_full[b], 1);
             mbar_init(&stat_empty[b], kSoftWarps);
         }
+        for (int b = 0; b < 4; ++b) mbar_init(&sum_bar[b], 4);
         mbar_init(s_free, kSoftWarps);
         mbar_init(dp_full, 1);
         mbar_init(ds_full, kSoftWarps);
@@ -1041,6 +1043,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const uint32_t lane_off = (uint32_t)(q * 32) << 16;
         const uint32_t mine = tmem + lane_off + (uint32_t)(w * 32);  // this thread's columns of S (and, 128 on, of dP)
         int g = 0;
+        uint32_t sum_phase = 0;
         bool ok = true;
         // the unit whose result is still in TMEM: its number, head, first valid row, partial slot, and this row's token
         int d_lt = -1, d_h = 0, d_shift = 0, d_slot = -1;
@@ -1143,6 +1146,23 @@ __global__ void __launch_bounds__(kThreads, 1)
                     tmem_ld32(mine + (uint32_t)kBlk, *reinterpret_cast<uint32_t(*)[32]>(&d[0]));
                     tmem_ld_wait();
                     if (KIND == kDKV) tmem_st16(mine + (uint32_t)kBlk, pk);  // P beside dS, over dP
+                    if (KIND == kDQ && wk.tiles == 1) {
+                        // A sequence's first rows are all here, and delta is the row's sum of P o dP, in f32. With few
+                        // keys dP - delta cancels, and the bf16 rounding of o in sum dO o O would cost dq and dk a
+                        // quarter more error than the rounding of dS does (every later row averages it away). The sums
+                        // of the tile before have been read: its dS was complete before this dP was issued.
+                        float part = 0.0f;
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) part += p[e] != 0.0f ? p[e] * d[e] : 0.0f;
+                        stats[w * kBlk + row] = part;
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(&sum_bar[q]);
+                        if (!(ok = warp_wait(&sum_bar[q], sum_phase, abort_flag))) break;
+                        sum_phase ^= 1u;
+                        delta = (stats[row] + stats[kBlk + row]) + (stats[2 * kBlk + row] + stats[3 * kBlk + row]);
+                        // for the pass over the keys, which follows
+                        if (w == 0 && row >= shift) args.delta[wk.h * args.ld_delta + tok] = delta;
+                    }
 #pragma unroll
                     for (int e = 0; e < 16; ++e) {
                         float2 n = both(-delta);  // minus the row's delta, or the columns'
@@ -1275,7 +1295,7 @@ Split split_of(const R97bPacked& p, int Hq, int Hkv) {
 int64_t part_floats(const Split& s, int Hkv, int D) { return (int64_t)s.blocks * s.parts * Hkv * kBlk * D; }
 
 template <int D, int KIND>
-int launch_bwd(const R97bPacked& p, const R97bAttnPackedBwd& a, const float* delta, const Split& split, float* dv_parts,
+int launch_bwd(const R97bPacked& p, const R97bAttnPackedBwd& a, float* delta, const Split& split, float* dv_parts,
                float* dk_parts, cudaStream_t st) {
     using C = BCfg<D, KIND>;
     static_assert(C::kSmemBytes <= 232448, "shared memory");
@@ -1319,6 +1339,7 @@ int run_bwd(const R97bPacked& p, const R97bAttnPackedBwd& a, cudaStream_t st) {
     const Split split = split_of(p, a.Hq, a.Hkv);
     float* dv_parts = delta + a.Hq * delta_ld(p.T);
     float* dk_parts = dv_parts + part_floats(split, a.Hkv, D);
+    if (rc == R97B_OK) rc = launch_bwd<D, kDQ>(p, a, delta, split, dv_parts, dk_parts, st);
     if (rc == R97B_OK) rc = launch_bwd<D, D == 256 ? kDV : kDKV>(p, a, delta, split, dv_parts, dk_parts, st);
     if (D == 256 && rc == R97B_OK) rc = launch_bwd<D, D == 256 ? kDK : kDKV>(p, a, delta, split, dv_parts, dk_parts, st);
     if (split.blocks > 0 && rc == R97B_OK) {
@@ -1327,7 +1348,7 @@ int run_bwd(const R97bPacked& p, const R97bAttnPackedBwd& a, cudaStream_t st) {
         sum_parts_kernel<D><<<split.blocks * a.Hkv * (2 * kBlk / 8), 256, 0, st>>>(s);
         rc = launch_status();
     }
-    return rc == R97B_OK ? launch_bwd<D, kDQ>(p, a, delta, split, dv_parts, dk_parts, st) : rc;
+    return rc;
 }
 
 bool plan_ok(const R97bPacked* p) {
