@@ -626,7 +626,9 @@ typedef struct R97bHeadRows {
 /* Causal grouped-query attention inside each sequence: o_t = sum_{j <= t} softmax_j(scale q_t . k_j) v_j over the
  * sequence's own tokens; query head h reads key/value head h / (Hq / Hkv). bf16, D 128 or 256; lse f32
  * [Hq, ld_lse >= T], the natural-log log-sum-exp of each row's scaled scores. Rows behind token T are neither
- * read nor written, and a row outside a sequence never reaches that sequence's results whatever it holds.
+ * read nor written, and a row outside a sequence never reaches that sequence's results whatever it holds. (Inside
+ * one, a key or value that is not finite may reach any row: 0 times it is NaN.) Outputs must not overlap the
+ * operands or one another (R97B_EINVAL where two start at one address). At most 2^22 - 1 blocks times Hq.
  * Replaces: attention_twin, src/adjoint/host/attention.cpp:261-313, over the ragged batch of
  * include/r97/batch.h. */
 typedef struct R97bAttnPackedFwd {
@@ -640,9 +642,10 @@ typedef struct R97bAttnPackedFwd {
 int r97b_attn_packed_fwd(const R97bPacked* p, const R97bAttnPackedFwd* a, void* stream);
 
 /* Its backward from the forward's o and lse, the probabilities recomputed tile by tile: dq, dk, dv (bf16) of the
- * cotangent dout. The memory beside the operands is `ws` (256-byte aligned,
+ * cotangent dout. The row sums delta = dout . o come from o, those of a sequence's first 128 rows from the
+ * probabilities themselves (few keys: o's rounding would show). The memory beside the operands is `ws` (256-byte aligned,
  * r97b_attn_packed_bwd_workspace_bytes bytes, linear in T; calls that share it must not overlap on the GPU).
- * The same inputs give the same bits.
+ * The same inputs give the same bits. Outputs must not overlap the operands or one another.
  * Replaces: attention_host_adjoint, src/adjoint/host/attention.cpp:315-414. */
 typedef struct R97bAttnPackedBwd {
     int32_t Hq, Hkv, D;
@@ -678,7 +681,8 @@ typedef struct R97bRopePart {
 /* Up to two tensors (queries and keys) of T token rows in one launch: pos i32 [T] indexes the tables' rows; the
  * first `rot` dims of a head rotate, in pairs (i, i + rot / 2), or (2 i, 2 i + 1) when interleaved. D 64, 128 or
  * 256, rot a multiple of 16 up to D. A token whose pos is outside [0, n_pos) gets zero rows and sets bit 1 of
- * the device error word. Replaces: src/adjoint/host/qk.cpp and rope.cpp over a ragged batch's positions. */
+ * the device error word. y (the backward's dx) may be x (x or y) itself, row for row; no other overlap.
+ * Replaces: src/adjoint/host/qk.cpp and rope.cpp over a ragged batch's positions. */
 typedef struct R97bRope {
     int32_t D, rot, interleaved, n_parts;
     int64_t T, n_pos;

@@ -91,6 +91,13 @@ struct FwdArgs {
     float sign;  // of the scale: 1, -1 or 0
 };
 
+// Before the kernel ends on an abort: time for the copies and products still in flight, which nobody waits for any more,
+// to land in this CTA's own memory (a bounded wait of about two milliseconds).
+__device__ __forceinline__ void settle(const volatile int* abort) {
+    if (!*abort) return;
+    for (const long long t0 = clock64(); clock64() - t0 < 4000000;) __nanosleep(1000);
+}
+
 struct Unit {
     int h, tok0, i, n;  // head, the block's first token, its index in the sequence, its tokens
 };
@@ -589,6 +596,7 @@ __global__ void __launch_bounds__(FCfg<D>::kThreads, 1)
 
     tc_fence_before();
     __syncthreads();
+    settle(abort_flag);
     if (warp == 1) {
         tc_fence_after();
         tmem_dealloc(tmem, 512);
@@ -1189,6 +1197,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 
     tc_fence_before();
     __syncthreads();
+    settle(abort_flag);
     if (warp == 1) {
         tc_fence_after();
         tmem_dealloc(tmem, 512);
@@ -1241,8 +1250,9 @@ struct SumArgs {
 };
 template <int D>
 __global__ void __launch_bounds__(256) sum_parts_kernel(const SumArgs a) {
-    const int r = (int)((blockIdx.x * 256 + threadIdx.x) >> 5) % (2 * kBlk);
-    const int unit = (int)((blockIdx.x * 256 + threadIdx.x) >> 5) / (2 * kBlk), lane = threadIdx.x & 31;
+    constexpr int kPer = 2 * kBlk / 8;  // thread blocks a unit: 8 warps each
+    const int unit = (int)(blockIdx.x / kPer), lane = threadIdx.x & 31;
+    const int r = (int)(blockIdx.x % kPer) * 8 + (threadIdx.x >> 5);
     const int row = r >> 1, is_dk = r & 1;
     const int b = unit / a.heads, h = unit - b * a.heads;
     const int4 e = a.blocks[b];
@@ -1360,6 +1370,13 @@ bool plan_ok(const R97bPacked* p) {
 bool heads_ok(int32_t Hq, int32_t Hkv, int32_t D) {
     return Hq > 0 && Hkv > 0 && Hq % Hkv == 0 && Hq <= 65535 && (D == 128 || D == 256);
 }
+// Whether an output starts where another operand does (a result is written while others still read).
+template <int N>
+bool aliased(const void* out, const void* const (&others)[N]) {
+    for (const void* o : others)
+        if (o == out) return true;
+    return false;
+}
 bool units_ok(const R97bPacked* p, int32_t H) { return (int64_t)p->n_blocks * H <= 0x3FFFFF; }
 bool lse_ok(const float* lse, int64_t ld, int64_t T) { return lse && !(reinterpret_cast<uintptr_t>(lse) & 3) && ld >= T; }
 
@@ -1379,16 +1396,22 @@ extern "C" int32_t r97b_packed_blocks(const int32_t* cu_host, int32_t n_seq, int
     }
     if (n > 0x7FFFFFFF) return -1;
     std::vector<Block> b;
+    try {
+        b.reserve((size_t)n);
+    } catch (...) {  // no exception crosses the C boundary
+        return -1;
+    }
     for (int pass = 0; pass < 2; ++pass) {
         int32_t* out = pass == 0 ? q_blocks_host : k_blocks_host;
         if (!out) continue;
         b.clear();
-        b.reserve((size_t)n);
         for (int32_t s = 0; s < n_seq; ++s) {
             const int32_t len = cu_host[s + 1] - cu_host[s], nb = (int32_t)(((int64_t)len + 127) / 128);
             for (int32_t i = 0; i < nb; ++i) b.push_back({cu_host[s], len, i, pass == 0 ? i + 1 : nb - i});
         }
-        std::stable_sort(b.begin(), b.end(), [](const Block& x, const Block& y) { return x.cost > y.cost; });
+        std::sort(b.begin(), b.end(), [](const Block& x, const Block& y) {
+            return x.cost != y.cost ? x.cost > y.cost : (x.tok0 != y.tok0 ? x.tok0 < y.tok0 : x.i < y.i);
+        });
         for (size_t i = 0; i < b.size(); ++i) {
             const int32_t row[4] = {b[i].tok0, b[i].len, b[i].i, 0};
             memcpy(out + 4 * i, row, sizeof(row));
@@ -1404,6 +1427,7 @@ extern "C" int r97b_attn_packed_fwd(const R97bPacked* p, const R97bAttnPackedFwd
         !head_rows_ok(a->o, a->Hq, a->D) || !lse_ok(a->lse, a->ld_lse, p->T) || !units_ok(p, a->Hq))
         return R97B_EINVAL;
     if (p->T == 0) return R97B_OK;
+    if (aliased(a->o.ptr, {a->q.ptr, a->k.ptr, a->v.ptr, a->lse})) return R97B_EINVAL;
     cudaStream_t st = as_stream(stream);
     return a->D == 256 ? launch_fwd<256>(*p, *a, st) : launch_fwd<128>(*p, *a, st);
 }
@@ -1425,6 +1449,10 @@ extern "C" int r97b_attn_packed_bwd(const R97bPacked* p, const R97bAttnPackedBwd
     const int64_t need = r97b_attn_packed_bwd_workspace_bytes(p, a->Hq, a->Hkv, a->D);
     if (need < 0 || a->ws_bytes < need || (need > 0 && !a->ws) || (reinterpret_cast<uintptr_t>(a->ws) & 255)) return R97B_EINVAL;
     if (p->T == 0) return R97B_OK;
+    for (const void* out : {(const void*)a->dq.ptr, (const void*)a->dk.ptr, (const void*)a->dv.ptr, (const void*)a->ws})
+        if (aliased(out, {a->q.ptr, a->k.ptr, a->v.ptr, a->o.ptr, a->dout.ptr, a->lse})) return R97B_EINVAL;
+    if (aliased(a->dq.ptr, {a->dk.ptr, a->dv.ptr, a->ws}) || aliased(a->dk.ptr, {a->dv.ptr, a->ws}) || a->dv.ptr == a->ws)
+        return R97B_EINVAL;
     cudaStream_t st = as_stream(stream);
     return a->D == 256 ? run_bwd<256>(*p, *a, st) : run_bwd<128>(*p, *a, st);
 }

@@ -501,6 +501,9 @@ def attn_packed_fwd(q, k, v, plan, scale, o=None, lse=None, stream=None):
     token are left as they were."""
     rows, Hq, Hkv, D, dev = _packed_dims(q, k, plan)
     st = _packed_stream(stream, dev, "attn_packed_fwd")
+    if stream is not None and (o is None or lse is None):
+        with torch.cuda.stream(stream):  # what is allocated here belongs to the stream that writes it
+            return attn_packed_fwd(q, k, v, plan, scale, o, lse)
     o = torch.empty((rows, Hq, D), dtype=_BF16, device=dev) if o is None else o
     lse = torch.empty((Hq, rows), dtype=_F32, device=dev) if lse is None else lse
     T = plan.T
@@ -528,6 +531,9 @@ def attn_packed_bwd(q, k, v, o, dout, lse, plan, scale, ws=None, dq=None, dk=Non
     are left as they were."""
     rows, Hq, Hkv, D, dev = _packed_dims(q, k, plan)
     st = _packed_stream(stream, dev, "attn_packed_bwd")
+    if stream is not None and (ws is None or dq is None or dk is None or dv is None):
+        with torch.cuda.stream(stream):
+            return attn_packed_bwd(q, k, v, o, dout, lse, plan, scale, ws, dq, dk, dv)
     dq = torch.empty((rows, Hq, D), dtype=_BF16, device=dev) if dq is None else dq
     dk = torch.empty((rows, Hkv, D), dtype=_BF16, device=dev) if dk is None else dk
     dv = torch.empty((rows, Hkv, D), dtype=_BF16, device=dev) if dv is None else dv
@@ -567,6 +573,9 @@ def rope_tables(n_pos: int, rot: int, theta: float, scaling=None, device="cuda",
     if device.index is None:
         device = torch.device("cuda", torch.cuda.current_device())
     st = _packed_stream(stream, device, "rope_tables")
+    if stream is not None:
+        with torch.cuda.stream(stream):
+            return rope_tables(n_pos, rot, theta, scaling, device)
     cos = torch.empty((n_pos, rot // 2), dtype=torch.float32, device=device)
     sin = torch.empty_like(cos)
     v = {**args, **sc}
@@ -617,6 +626,10 @@ def qk_rope_fwd(parts, cos, sin, pos, *, interleaved=False, eps=1e-6, outs=None,
     or None for none; cos, sin [n_pos, rot / 2] (rope_tables; rot a multiple of 16 up to D), pos i32 [T]. Pairs
     (i, i + rot / 2), or (2 i, 2 i + 1) when interleaved. Returns one [rows, heads, D] tensor a part (`outs`, when
     given); rows behind T are left as they were."""
+    if stream is not None and outs is None and parts:
+        _packed_stream(stream, parts[0][0].device, "qk_rope_fwd")
+        with torch.cuda.stream(stream):
+            return qk_rope_fwd(parts, cos, sin, pos, interleaved=interleaved, eps=eps)
     outs = [torch.empty(x.shape, dtype=_BF16, device=x.device) for x, _ in parts] if outs is None else outs
     if len(outs) != len(parts):
         raise R97bError("qk_rope_fwd: one output a part")

@@ -212,8 +212,10 @@ def test_attention_streams_and_graph(cuda, D):
     with torch.cuda.stream(side):
         got = step(a)
     side.synchronize()
-    for x, y in zip(got, want_a):
-        assert torch.equal(x, y)
+    given = step(a, stream=side)  # the stream as an argument
+    side.synchronize()
+    for x, y, z in zip(got, want_a, given):
+        assert torch.equal(x, y) and torch.equal(x, z)
     held = [tuple(t.clone() for t in a) for _ in range(2)]
     graphs, outs = [], []
     for t in held:
@@ -235,6 +237,33 @@ def test_attention_streams_and_graph(cuda, D):
     for (got, _), want in zip(outs, (want_a, want_b)):
         for x, y in zip(got, want):
             assert torch.equal(x, y)
+
+
+def test_given_stream_owns_what_a_call_allocates(cuda):
+    """A call on a stream that is busy: its workspace and results are not handed to the current stream's next
+    allocations while it waits there."""
+    lens = [260, 77]
+    plan = PackedPlan(_cu(lens), cuda)
+    q, k, v, do = _inputs(cuda, lens, 4, 2, 128, 83)
+    cos, sin = ops.rope_tables(300, 64, 1e4)
+    side = torch.cuda.Stream()
+
+    def chain(stream):
+        (qr,) = ops.qk_rope_fwd([(q, None)], cos, sin, plan.pos, stream=stream)
+        o, lse = ops.attn_packed_fwd(qr, k, v, plan, 0.1, stream=stream)
+        return ops.attn_packed_bwd(qr, k, v, o, do, lse, plan, 0.1, stream=stream)
+
+    want = chain(None)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(40_000_000)  # some 20 ms ahead of the calls
+    got = chain(side)
+    sizes = [t.numel() * t.element_size() for t in (q, k)] + [ops.attn_packed_bwd_workspace(plan, 4, 2, 128).numel()]
+    over = [torch.full((n,), 255, dtype=torch.uint8, device=cuda) for n in sizes for _ in range(4)]
+    torch.cuda.synchronize()
+    assert all(int(t[0]) == 255 for t in over)
+    for x, y in zip(got, want):
+        assert torch.equal(x, y)
 
 
 def test_attention_far_offsets(cuda):
@@ -274,6 +303,12 @@ def test_attention_wrapper_refusals(cuda):
         ops.attn_packed_bwd(q, k, v, o, do[:, :2], lse, plan, 1.0)
     with pytest.raises(R97bError):
         ops.attn_packed_bwd(q, k, v, o, do, lse[:2], plan, 1.0)
+    with pytest.raises(R97bError):
+        ok(o=q)  # over an operand
+    dq = torch.empty_like(q)
+    for bad in (dict(dq=q), dict(dk=k), dict(dv=do[:, :2]), dict(dq=dq, dk=dq[:, :2])):
+        with pytest.raises(R97bError):
+            ops.attn_packed_bwd(q, k, v, o, do, lse, plan, 1.0, **bad)
     empty = PackedPlan([0, 0], cuda)
     o0, l0 = ops.attn_packed_fwd(q[:0], k[:0], v[:0], empty, 1.0)
     assert o0.shape == (0, 4, 128) and l0.shape == (4, 0)

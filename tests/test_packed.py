@@ -12,7 +12,8 @@ from r97training_b200 import ops
 from r97training_b200.packed import PackedPlan
 from tests import packed_ref as ref
 
-FAKE = 1 << 20  # an aligned address that no refused call dereferences
+FAKE = 1 << 20  # aligned addresses that no refused call dereferences: operands here, outputs at multiples of OUT
+OUT = 1 << 22
 
 
 def _blocks(cu):
@@ -67,15 +68,15 @@ def _rows(ptr=FAKE, tok=2048, head=256):
 
 
 def _fwd_args(**kw):
-    a = L.R97bAttnPackedFwd(8, 2, 256, 0.0625, _rows(), _rows(), _rows(), _rows(), FAKE, 300)
+    a = L.R97bAttnPackedFwd(8, 2, 256, 0.0625, _rows(), _rows(), _rows(), _rows(OUT), FAKE, 300)
     for n, v in kw.items():
         setattr(a, n, v)
     return a
 
 
 def _bwd_args(**kw):
-    a = L.R97bAttnPackedBwd(8, 2, 256, 0.0625, _rows(), _rows(), _rows(), _rows(), _rows(), FAKE, 300, _rows(), _rows(),
-                            _rows(), FAKE, 1 << 40)
+    a = L.R97bAttnPackedBwd(8, 2, 256, 0.0625, _rows(), _rows(), _rows(), _rows(), _rows(), FAKE, 300, _rows(OUT),
+                            _rows(2 * OUT), _rows(3 * OUT), 4 * OUT, 1 << 40)
     for n, v in kw.items():
         setattr(a, n, v)
     return a
@@ -109,7 +110,10 @@ def test_attention_refusals_of_one_direction():
     assert h.r97b_attn_packed_bwd(ref_, None, None) == 1
     need = h.r97b_attn_packed_bwd_workspace_bytes(ref_, 8, 2, 256)
     assert need >= 0
-    for bad in (dict(dout=_rows(None)), dict(dq=_rows(head=8)), dict(dk=_rows(FAKE + 8)), dict(dv=_rows(tok=256))):
+    assert h.r97b_attn_packed_fwd(ref_, ctypes.byref(_fwd_args(o=_rows())), None) == 1  # over an operand
+    for bad in (dict(dout=_rows(None)), dict(dq=_rows(OUT, head=8)), dict(dk=_rows(OUT + 8)), dict(dv=_rows(OUT, tok=256)),
+                dict(dq=_rows()), dict(dk=_rows()), dict(dv=_rows()), dict(dk=_rows(OUT)), dict(dv=_rows(2 * OUT)),
+                dict(ws=OUT), dict(ws=FAKE)):
         assert h.r97b_attn_packed_bwd(ref_, ctypes.byref(_bwd_args(**bad)), None) == 1
     assert h.r97b_attn_packed_bwd(ref_, ctypes.byref(_bwd_args(ws=FAKE + 16)), None) == 1
     if need:
