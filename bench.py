@@ -385,6 +385,9 @@ def profile_case(case: str) -> None:
     conv            GDN conv prep fwd + bwd at 8192 tokens, 8192 channels
     attn            one config-5 attention core (B 2, 16 / 4 heads, S 4096, D 256), forward + backward, with
                     CUDA-event timings; attn_small the same at B 1, S 2048; attn_fwd the forward alone
+    attn_packed     the packed attention over 2 sequences of 4096 tokens (16 / 4 heads of 256), forward + backward, with
+                    CUDA-event timings; attn_packed_128 over one of 8192 tokens (16 / 4 heads of 128)
+    rope_packed     the packed rotary positions with the q/k norm over the same tokens, forward + adjoint
     step            one config-5 training step after one warm-up step, inside an NVTX range "step"
     """
     import torch
@@ -606,6 +609,45 @@ def profile_case(case: str) -> None:
         print(f"attention B{B} Hq{Hq} Hkv{Hkv} S{S} D{D}: forward {min(fw):.3f} ms "
               f"({causal / min(fw) / 1e9:.0f} TFLOP/s of the causal 2-product work), backward {min(bw):.3f} ms "
               f"({2.5 * causal / min(bw) / 1e9:.0f} TFLOP/s of 2.5 x that)")
+    elif case in ("attn_packed", "attn_packed_128", "rope_packed"):
+        from r97training_b200 import ops
+        from r97training_b200.packed import PackedPlan
+        lens, Hq, Hkv, D = ([8192], 16, 4, 128) if case == "attn_packed_128" else ([4096, 4096], 16, 4, 256)
+        cu = [sum(lens[:i]) for i in range(len(lens) + 1)]
+        plan, T = PackedPlan(cu, dev), cu[-1]
+        rows = lambda h, s=1.0: (torch.randn(T, h, D, device=dev) * s).bfloat16()  # noqa: E731
+        q, k, v, do = rows(Hq), rows(Hkv), rows(Hkv), rows(Hq, 0.1)
+        cos, sin = ops.rope_tables(max(lens), 64, 1e7, device=dev)
+        gain = 1.0 + 0.1 * torch.randn(D, device=dev)
+        ws = ops.attn_packed_bwd_workspace(plan, Hq, Hkv, D)
+        dq, dk = torch.empty_like(q), torch.empty_like(k)
+        ev = [torch.cuda.Event(enable_timing=True) for _ in range(3)]
+        fw, bw = [], []
+        for _ in range(3):
+            ev[0].record()
+            if case == "rope_packed":
+                ops.qk_rope_fwd([(q, gain), (k, gain)], cos, sin, plan.pos)
+            else:
+                o, lse = ops.attn_packed_fwd(q, k, v, plan, D ** -0.5)
+            ev[1].record()
+            if case == "rope_packed":
+                ops.qk_rope_bwd([(q, gain, do, dq), (k, gain, v, dk)], cos, sin, plan.pos)
+            else:
+                ops.attn_packed_bwd(q, k, v, o, do, lse, plan, D ** -0.5, ws)
+            ev[2].record()
+            torch.cuda.synchronize()
+            fw.append(ev[0].elapsed_time(ev[1]))
+            bw.append(ev[1].elapsed_time(ev[2]))
+        if case == "rope_packed":
+            n = T * (Hq + Hkv) * D * 2
+            print(f"rotary positions of {T} tokens, {Hq} + {Hkv} heads of {D}: forward {min(fw) * 1e3:.1f} us "
+                  f"({2 * n / min(fw) / 1e6:.0f} GB/s of the rows), adjoint {min(bw) * 1e3:.1f} us "
+                  f"({3 * n / min(bw) / 1e6:.0f} GB/s)")
+        else:
+            pairs = sum(n * (n + 1) / 2 for n in lens) * Hq
+            print(f"packed attention {lens} Hq{Hq} Hkv{Hkv} D{D}: forward {min(fw):.3f} ms "
+                  f"({4 * D * pairs / min(fw) / 1e9:.0f} TFLOP/s of the two products over the visible pairs), backward "
+                  f"{min(bw):.3f} ms ({10 * D * pairs / min(bw) / 1e9:.0f} TFLOP/s of the five)")
     elif case == "step":
         from r97training_b200.model import CONFIG5, Adapter, HybridModel, TrainStep
         model = HybridModel(CONFIG5, dev)

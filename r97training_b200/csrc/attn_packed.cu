@@ -668,8 +668,10 @@ struct BCfg {
 struct BwdArgs {
     const int4* blocks;
     const float* lse;
-    float* delta;
+    float* delta;                      // written by kDQ, read by the others, which follow it
     int64_t ld_lse, ld_delta;
+    const __nv_bfloat16* o;            // kDQ: the forward's output
+    int64_t o_tok, o_head;
     __nv_bfloat16 *out0, *out1;        // kDQ: dq; kDKV: dv, dk; kDV: dv; kDK: dk
     int64_t tok0, head0, tok1, head1;
     int32_t a0_head, a1_head, b0_head, b1_head, c0_head;
@@ -765,7 +767,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         return;
     }
     if (threadIdx.x == 0) {
-        queue.init((C::kKeys ? 4 : 3) + kSoftWarps);
+        queue.init(4 + kSoftWarps);
         for (int s = 0; s < C::kStages; ++s) {
             mbar_init(&full_bar[s], 1);
             mbar_init(&empty_bar[s], 1);
@@ -1016,7 +1018,16 @@ __global__ void __launch_bounds__(kThreads, 1)
                 umma_commit_by(lead, acc_full);
                 g += n;
             }
-        } else if (C::kKeys && warp == 2) {
+        } else if (KIND == kDQ) {
+            // --------------------------------------------------------- the next unit's output rows, into L2 for delta
+            for (int u = blockIdx.x, lt = 0; u >= 0; u = queue.next(lt), ++lt) {
+                const Walk<KIND> wk(args, u);
+                if (wk.tiles == 1) continue;
+                const __nv_bfloat16* op = args.o + (int64_t)wk.tok0 * args.o_tok + wk.h * args.o_head;
+                for (int k = lane; k < wk.n * (D / 64); k += 32)
+                    prefetch_l2(op + k / (D / 64) * args.o_tok + k % (D / 64) * 64);
+            }
+        } else {
             // --------------------------------------------------------- the columns' lse and delta, a tile ahead
             int g = 0;
             bool ok = true;
@@ -1096,9 +1107,49 @@ __global__ void __launch_bounds__(kThreads, 1)
             const int shift = wk.shift();
             const int64_t tok = (int64_t)wk.tok0 + row - shift;
             float lse2 = 0.0f, delta = 0.0f;
-            if (!C::kKeys && row >= shift) {
-                lse2 = args.lse[wk.h * args.ld_lse + tok] * kLog2e;
-                delta = args.delta[wk.h * args.ld_delta + tok];
+            if (!C::kKeys && row >= shift) lse2 = args.lse[wk.h * args.ld_lse + tok] * kLog2e;
+            if (!C::kKeys && wk.tiles > 1) {
+                // delta = dO . O, this warp's quarter of its rows, while the tensor core has the first scores to go on with:
+                // kLanes lanes a row, so that a load touches whole lines. dO is in shared memory until the unit's last
+                // dP, which waits for this warp's first dS.
+                constexpr int kLanes = D / 32, kRows = 32 / kLanes;  // kRows rows a step, kLanes steps
+                const int at = w * kLanes + lane % kLanes;           // the lane's 16-byte piece of a row
+                const __nv_bfloat16* op = args.o + wk.h * args.o_head + at * 8;
+                uint4 o[kLanes];
+#pragma unroll
+                for (int c = 0; c < kLanes; ++c) {
+                    const int r = q * 32 + c * kRows + lane / kLanes - shift;
+                    o[c] = r >= 0 ? *reinterpret_cast<const uint4*>(op + ((int64_t)wk.tok0 + r) * args.o_tok)
+                                  : make_uint4(0, 0, 0, 0);
+                }
+                if (!(ok = warp_wait(&a_full[1], (uint32_t)(lt & 1), abort_flag))) break;
+                float part[kLanes];
+#pragma unroll
+                for (int c = 0; c < kLanes; ++c) {
+                    const int r = q * 32 + c * kRows + lane / kLanes;
+                    const uint4 g4 = *reinterpret_cast<const uint4*>(smem + C::kABytes + (at >> 3) * kChunk + r * 128 +
+                                                                     (((at & 7) ^ (r & 7)) << 4));  // 128-byte swizzle
+                    const __nv_bfloat162* x = reinterpret_cast<const __nv_bfloat162*>(&o[c]);
+                    const __nv_bfloat162* y = reinterpret_cast<const __nv_bfloat162*>(&g4);
+                    part[c] = 0.0f;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const float2 xf = __bfloat1622float2(x[e]), yf = __bfloat1622float2(y[e]);
+                        part[c] = fmaf(xf.x, yf.x, part[c]);
+                        part[c] = fmaf(xf.y, yf.y, part[c]);
+                    }
+                }
+                // the lanes of a row sum its pieces, each ending with another step's row; then row `lane` to each lane
+#pragma unroll
+                for (int half = kLanes / 2; half > 0; half >>= 1) {
+                    const bool upper = lane & half;
+#pragma unroll
+                    for (int c = 0; c < half; ++c) {
+                        const float give = upper ? part[c] : part[c + half];
+                        part[c] = (upper ? part[c + half] : part[c]) + __shfl_xor_sync(0xFFFFFFFFu, give, half);
+                    }
+                }
+                delta = __shfl_sync(0xFFFFFFFFu, part[0], lane % kRows * kLanes + lane / kRows);
             }
             for (int j = 0, jm = 0; j < wk.tiles; ++j, ++g) {
                 const int b = KIND == kDV ? (g & 1) : 0;
@@ -1154,21 +1205,23 @@ __global__ void __launch_bounds__(kThreads, 1)
                     tmem_ld32(mine + (uint32_t)kBlk, *reinterpret_cast<uint32_t(*)[32]>(&d[0]));
                     tmem_ld_wait();
                     if (KIND == kDKV) tmem_st16(mine + (uint32_t)kBlk, pk);  // P beside dS, over dP
-                    if (KIND == kDQ && wk.tiles == 1) {
+                    if (KIND == kDQ && j == 0) {
                         // A sequence's first rows are all here, and delta is the row's sum of P o dP, in f32. With few
                         // keys dP - delta cancels, and the bf16 rounding of o in sum dO o O would cost dq and dk a
-                        // quarter more error than the rounding of dS does (every later row averages it away). The sums
-                        // of the tile before have been read: its dS was complete before this dP was issued.
-                        float part = 0.0f;
+                        // quarter more error than the rounding of dS does (every later row averages it away).
+                        if (wk.tiles == 1) {
 #pragma unroll
-                        for (int e = 0; e < 32; ++e) part += p[e] != 0.0f ? p[e] * d[e] : 0.0f;
-                        stats[w * kBlk + row] = part;
+                            for (int e = 0; e < 32; ++e) delta += p[e] != 0.0f ? p[e] * d[e] : 0.0f;
+                        }
+                        // The quarters' sums. Those of the unit before have been read: its last dS was complete before
+                        // this dP was issued.
+                        stats[w * kBlk + row] = delta;
                         __syncwarp();
                         if (lane == 0) mbar_arrive(&sum_bar[q]);
                         if (!(ok = warp_wait(&sum_bar[q], sum_phase, abort_flag))) break;
                         sum_phase ^= 1u;
                         delta = (stats[row] + stats[kBlk + row]) + (stats[2 * kBlk + row] + stats[3 * kBlk + row]);
-                        // for the pass over the keys, which follows
+                        // for the passes over the keys, which follow
                         if (w == 0 && row >= shift) args.delta[wk.h * args.ld_delta + tok] = delta;
                     }
 #pragma unroll
@@ -1202,40 +1255,6 @@ __global__ void __launch_bounds__(kThreads, 1)
         tc_fence_after();
         tmem_dealloc(tmem, 512);
     }
-}
-
-// delta[h, t] = sum_d dO[t, h, d] O[t, h, d]: D / 8 lanes a row, 16 bytes a lane.
-struct DeltaArgs {
-    R97bHeadRows o, dout;
-    float* delta;
-    int64_t ld, rows;
-    int32_t heads;
-};
-template <int D>
-__global__ void __launch_bounds__(256) delta_kernel(const DeltaArgs a) {
-    constexpr int kLanes = D / 8;
-    const int64_t r = ((int64_t)blockIdx.x * 256 + threadIdx.x) / kLanes;
-    const int l = threadIdx.x % kLanes;
-    float s = 0.0f;
-    const int64_t t = r / a.heads;
-    const int h = (int)(r - t * a.heads);
-    if (r < a.rows) {
-        const uint4 x = *reinterpret_cast<const uint4*>(reinterpret_cast<const __nv_bfloat16*>(a.o.ptr) + t * a.o.tok +
-                                                        h * a.o.head + 8 * l);
-        const uint4 y = *reinterpret_cast<const uint4*>(reinterpret_cast<const __nv_bfloat16*>(a.dout.ptr) +
-                                                        t * a.dout.tok + h * a.dout.head + 8 * l);
-        const __nv_bfloat162* xp = reinterpret_cast<const __nv_bfloat162*>(&x);
-        const __nv_bfloat162* yp = reinterpret_cast<const __nv_bfloat162*>(&y);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float2 xf = __bfloat1622float2(xp[i]), yf = __bfloat1622float2(yp[i]);
-            s = fmaf(xf.x, yf.x, s);
-            s = fmaf(xf.y, yf.y, s);
-        }
-    }
-#pragma unroll
-    for (int o = kLanes / 2; o > 0; o >>= 1) s += __shfl_xor_sync(0xFFFFFFFFu, s, o);
-    if (r < a.rows && l == 0) a.delta[h * a.ld + t] = s;
 }
 
 int64_t delta_ld(int64_t T) { return (T + 63) / 64 * 64; }
@@ -1324,6 +1343,7 @@ int launch_bwd(const R97bPacked& p, const R97bAttnPackedBwd& a, float* delta, co
     r.blocks = reinterpret_cast<const int4*>(dq ? p.q_blocks : p.k_blocks);
     r.lse = a.lse, r.ld_lse = a.ld_lse, r.delta = delta, r.ld_delta = delta_ld(p.T);
     const R97bHeadRows &o0 = dq ? a.dq : (KIND == kDK ? a.dk : a.dv), &o1 = a.dk;
+    r.o = reinterpret_cast<const __nv_bfloat16*>(a.o.ptr), r.o_tok = a.o.tok, r.o_head = a.o.head;
     r.out0 = reinterpret_cast<__nv_bfloat16*>(o0.ptr), r.tok0 = o0.tok, r.head0 = o0.head;
     r.out1 = reinterpret_cast<__nv_bfloat16*>(o1.ptr), r.tok1 = o1.tok, r.head1 = o1.head;
     r.a0_head = (int32_t)a0.head, r.a1_head = (int32_t)a1.head, r.b0_head = (int32_t)b0.head, r.b1_head = (int32_t)b1.head;
@@ -1341,15 +1361,10 @@ int launch_bwd(const R97bPacked& p, const R97bAttnPackedBwd& a, float* delta, co
 template <int D>
 int run_bwd(const R97bPacked& p, const R97bAttnPackedBwd& a, cudaStream_t st) {
     float* delta = reinterpret_cast<float*>(a.ws);
-    const DeltaArgs d{a.o, a.dout, delta, delta_ld(p.T), p.T * a.Hq, a.Hq};
-    const int64_t grid = (d.rows * (D / 8) + 255) / 256;
-    if (grid > 0x7FFFFFFF) return R97B_EINVAL;
-    delta_kernel<D><<<(unsigned)grid, 256, 0, st>>>(d);
-    int rc = launch_status();
     const Split split = split_of(p, a.Hq, a.Hkv);
     float* dv_parts = delta + a.Hq * delta_ld(p.T);
     float* dk_parts = dv_parts + part_floats(split, a.Hkv, D);
-    if (rc == R97B_OK) rc = launch_bwd<D, kDQ>(p, a, delta, split, dv_parts, dk_parts, st);
+    int rc = launch_bwd<D, kDQ>(p, a, delta, split, dv_parts, dk_parts, st);
     if (rc == R97B_OK) rc = launch_bwd<D, D == 256 ? kDV : kDKV>(p, a, delta, split, dv_parts, dk_parts, st);
     if (D == 256 && rc == R97B_OK) rc = launch_bwd<D, D == 256 ? kDK : kDKV>(p, a, delta, split, dv_parts, dk_parts, st);
     if (split.blocks > 0 && rc == R97B_OK) {
