@@ -8,6 +8,19 @@
 //
 // All products on tcgen05 with f32 accumulators in TMEM; P and dS are rounded to bf16 for the second products (half
 // a bf16 step of each, what an output's own rounding costs), statistics and sums stay in f32.
+//
+// Blocks that end inside a tile sit at the tile's END, behind zero rows: the tensor maps address row r < 128 of the
+// block that begins at token t as (column, r, t), token and row with one stride, and a box that starts at row n - 128
+// reads zeros before the block's first token. So no load or store touches a row of another sequence or behind the last
+// one, and the same code serves every length.
+//
+// What bounds it, measured at 2 x 4096 tokens of 16/4 heads of 256 (one sequence of 8192, 16/4 heads of 128): the forward
+// 185-200 us (211) with the tensor pipe busy 76 % (64 %) of the cycles; the backward's passes 298 us dQ, 190-200 dV, 296-315
+// dK (276 dQ, 406 dK and dV) at 71, 83, 81 (75, 76) %. HBM takes 3-15 % of its rate throughout. At D = 256 the rest is
+// shared memory, which every operand byte crosses twice (the copy's write, the matrix unit's reads: dK's tile moves 4096
+// cycles' worth in 3950, its products take 3376); at D = 128 the forward's exponentials, one a score at 16 a cycle, take as
+// long as its two products. In long runs the power limit sets the clock, and the time follows the products issued: 10
+// of 128 x 128 x D a tile pair at D = 256 (S formed four times), 9 at 128, where the mathematics needs 7.
 #include "sm100.cuh"
 #include "r97b_internal.h"
 #include "fastmath.cuh"
@@ -120,8 +133,9 @@ __device__ __forceinline__ constexpr int quarter_col(int k16) { return (k16 >> 1
 
 // The next unit of a CTA, for every role of it. The grid has one CTA a unit, longest units first; a CTA starts with its
 // own and then takes over (cancels) the launch of the next one that has not started, so the units go to whichever SM is
-// free. One role asks, as it loads the last tile of the unit before; the answers pass through kSlots shared-memory slots, each read by every warp that
-// walks the units (`readers` of them).
+// free. One role asks, as it loads the last tile of the unit before (asked a unit earlier, the key passes end with whole
+// units waiting behind busy SMs); the answers pass through kSlots shared-memory slots, each read by every warp that walks
+// the units (`readers` of them).
 struct UnitQueue {
     static constexpr int kSlots = 4;
     uint4* slot;      // [kSlots]
@@ -171,6 +185,9 @@ __device__ __forceinline__ Unit unit_geom(const int4* blocks, int heads, int u) 
 // row's exponentials use is handed from tile to tile; it is moved (and O rescaled, by the threads that own the rows) only
 // when the row's maximum has outgrown it by 2^8, which f32 sums and bf16 probabilities carry without loss. A unit's
 // result is drained after the next unit's first P, which the tensor core has meanwhile been given the scores of.
+// Three buffers at D = 128 (3 x 128 + 128 of the 512 TMEM columns), two at 256. Against two warpgroups in turn on two
+// buffers with S a tile ahead inside a unit only: a chat batch of 16384 tokens, 8/2 heads of 128, 62 -> 49 us; 2 x 4096 tokens
+// of 256, 213 -> 198. A softmax loop unrolled whole lost 100 us of the 540 at 12301 tokens to instruction fetches.
 template <int D>
 __global__ void __launch_bounds__(FCfg<D>::kThreads, 1)
     fwd_kernel(const __grid_constant__ CUtensorMap tQ, const __grid_constant__ CUtensorMap tK,
@@ -641,6 +658,10 @@ int launch_fwd(const R97bPacked& p, const R97bAttnPackedFwd& a, cudaStream_t st)
 // elementwise threads write over their own columns of the scores' TMEM. Each thread owns a row and each of the four
 // warpgroups 32 of its columns; the next tile's S is issued before the accumulating products, so its exponentials run
 // beside them, and only dS (a product and a rounding) stands between dP and the products that read it.
+// kDQ goes first and leaves every row's delta = dO . O for the others: it has dO in shared memory. (A kernel of its own,
+// bound by its reads of o and dout, cost more: a chat batch of 16384 tokens, 8/2 heads of 128, 72 us for the two, 66 in one;
+// 8192 tokens of 16/4 heads of 256, 149 and 134.) At D = 128 both of a column block's products read one 32 KB copy of it:
+// 12301 tokens 1.68 -> 1.55 ms.
 enum Kind { kDQ = 0, kDKV = 1, kDV = 2, kDK = 3 };
 
 constexpr int kThreads = 640;  // warps 0, 3: TMA, warp 1: MMA, warp 2: the columns' statistics; four warpgroups after
