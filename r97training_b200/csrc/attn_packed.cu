@@ -16,10 +16,11 @@
 //
 // What bounds it, measured at 2 x 4096 tokens of 16/4 heads of 256 (one sequence of 8192, 16/4 heads of 128): the forward
 // 185-200 us (211) with the tensor pipe busy 76 % (64 %) of the cycles; the backward's passes 298 us dQ, 190-200 dV, 296-315
-// dK (276 dQ, 406 dK and dV) at 71, 83, 81 (75, 76) %. HBM takes 3-15 % of its rate throughout. At D = 256 the rest is
-// shared memory, which every operand byte crosses twice (the copy's write, the matrix unit's reads: dK's tile moves 4096
-// cycles' worth in 3950, its products take 3376); at D = 128 the forward's exponentials, one a score at 16 a cycle, take as
-// long as its two products. In long runs the power limit sets the clock, and the time follows the products issued: 10
+// dK (276 dQ, 406 dK and dV) at 71, 83, 81 (75, 76) %. HBM takes 3-15 % of its rate throughout. A tile of dQ at
+// D = 128, by the clock inside the kernel: 2040 cycles, of which the matrix unit works 1900 on products that are 3 x 512 at its
+// full rate (128-column products, both operands from shared memory at D = 128; with q and dO kept in tensor memory the tile
+// took 1 % less, and units started later), and 130 pass between dS and the product that takes it. The exponentials take
+// 980 of them beside the products; in the forward at D = 128 they take as long as its two products. In long runs the power limit sets the clock, and the time follows the products issued: 10
 // of 128 x 128 x D a tile pair at D = 256 (S formed four times), 9 at 128, where the mathematics needs 7.
 #include "sm100.cuh"
 #include "r97b_internal.h"
