@@ -454,9 +454,17 @@ def _packed_stream(stream, dev, what: str) -> int:
     one are refused."""
     if not dev.type == "cuda":
         raise R97bError(f"{what}: tensors must be on a CUDA device, got {dev}")
-    if dev.index != torch.cuda.current_device() or (stream is not None and stream.device_index != dev.index):
+    at = dev.index
+    if at != torch._C._cuda_getDevice() or (stream is not None and stream.device_index != at):
         raise R97bError(f"{what}: tensors are on {dev}, the current device is cuda:{torch.cuda.current_device()}")
-    return torch._C._cuda_getCurrentRawStream(dev.index) if stream is None else stream.cuda_stream
+    return torch._C._cuda_getCurrentRawStream(at) if stream is None else stream.cuda_stream
+
+
+def _rows_like(t, rows: int) -> torch.Tensor:
+    """An output of `rows` token rows beside t [n, heads, D] (empty_like where it fits: half the cost of empty)."""
+    if t.dim() == 3 and t.is_contiguous() and t.dtype is _BF16 and len(t) == rows:
+        return torch.empty_like(t)
+    return torch.empty((rows, *t.shape[1:]), dtype=_BF16, device=t.device)
 
 
 def _head_rows(t, name: str, heads: int, D: int, rows: int, dev):
@@ -504,7 +512,7 @@ def attn_packed_fwd(q, k, v, plan, scale, o=None, lse=None, stream=None):
     if stream is not None and (o is None or lse is None):
         with torch.cuda.stream(stream):  # what is allocated here belongs to the stream that writes it
             return attn_packed_fwd(q, k, v, plan, scale, o, lse)
-    o = torch.empty((rows, Hq, D), dtype=_BF16, device=dev) if o is None else o
+    o = _rows_like(q, rows) if o is None else o
     lse = torch.empty((Hq, rows), dtype=_F32, device=dev) if lse is None else lse
     T = plan.T
     if T == 0:
@@ -534,9 +542,9 @@ def attn_packed_bwd(q, k, v, o, dout, lse, plan, scale, ws=None, dq=None, dk=Non
     if stream is not None and (ws is None or dq is None or dk is None or dv is None):
         with torch.cuda.stream(stream):
             return attn_packed_bwd(q, k, v, o, dout, lse, plan, scale, ws, dq, dk, dv)
-    dq = torch.empty((rows, Hq, D), dtype=_BF16, device=dev) if dq is None else dq
-    dk = torch.empty((rows, Hkv, D), dtype=_BF16, device=dev) if dk is None else dk
-    dv = torch.empty((rows, Hkv, D), dtype=_BF16, device=dev) if dv is None else dv
+    dq = _rows_like(q, rows) if dq is None else dq
+    dk = _rows_like(k, rows) if dk is None else dk
+    dv = _rows_like(k, rows) if dv is None else dv
     T = plan.T
     if T == 0:
         return dq, dk, dv
@@ -597,7 +605,8 @@ def _rope_call(tensors, cos, sin, pos, interleaved, eps, stream, what):
     lead = tensors[0][2]
     dev, T = lead.device, pos.numel()
     st = _packed_stream(stream, dev, what)
-    if cos.dtype is not _F32 or sin.dtype is not _F32 or cos.dim() != 2 or cos.shape != sin.shape or \
+    table = cos.shape
+    if cos.dtype is not _F32 or sin.dtype is not _F32 or len(table) != 2 or table != sin.shape or \
             cos.device != dev or sin.device != dev or not cos.is_contiguous() or not sin.is_contiguous():
         raise R97bError(f"cos and sin must be contiguous [n_pos, rot / 2] f32 tables on {dev}")
     if pos.dtype is not torch.int32 or pos.dim() != 1 or not pos.is_contiguous() or pos.device != dev:
@@ -616,7 +625,7 @@ def _rope_call(tensors, cos, sin, pos, interleaved, eps, stream, what):
                   *(_NO_ROWS if dx is None else _head_rows(dx, "dx", heads, D, T, dev)))
     if len(tensors) == 1:
         parts += (0,) * 11
-    return _ROPE.pack(D, 2 * cos.shape[1], 1 if interleaved else 0, len(tensors), T, cos.shape[0], eps, 0, cos.data_ptr(),
+    return _ROPE.pack(D, 2 * table[1], 1 if interleaved else 0, len(tensors), T, table[0], eps, 0, cos.data_ptr(),
                       sin.data_ptr(), pos.data_ptr(), *parts), st
 
 
@@ -630,7 +639,7 @@ def qk_rope_fwd(parts, cos, sin, pos, *, interleaved=False, eps=1e-6, outs=None,
         _packed_stream(stream, parts[0][0].device, "qk_rope_fwd")
         with torch.cuda.stream(stream):
             return qk_rope_fwd(parts, cos, sin, pos, interleaved=interleaved, eps=eps)
-    outs = [torch.empty(x.shape, dtype=_BF16, device=x.device) for x, _ in parts] if outs is None else outs
+    outs = [_rows_like(x, len(x)) for x, _ in parts] if outs is None else outs
     if len(outs) != len(parts):
         raise R97bError("qk_rope_fwd: one output a part")
     if pos.numel() == 0:
