@@ -20,8 +20,10 @@
 // D = 128, by the clock inside the kernel: 2040 cycles, of which the matrix unit works 1900 on products that are 3 x 512 at its
 // full rate (128-column products, both operands from shared memory at D = 128; with q and dO kept in tensor memory the tile
 // took 1 % less, and units started later), and 130 pass between dS and the product that takes it. The exponentials take
-// 980 of them beside the products; in the forward at D = 128 they take as long as its two products. In long runs the power limit sets the clock, and the time follows the products issued: 10
-// of 128 x 128 x D a tile pair at D = 256 (S formed four times), 9 at 128, where the mathematics needs 7.
+// 980 of them beside the products; in the forward at D = 128 they take as long as its two products. A unit's start costs dQ
+// two microseconds more: delta's loads and sums, before the first dS. In long runs the power limit sets the clock, and the
+// time follows the products issued: 10 of 128 x 128 x D a tile at D = 256, forward and backward together (S formed four
+// times), 9 at 128, where the mathematics needs 7.
 #include "sm100.cuh"
 #include "r97b_internal.h"
 #include "fastmath.cuh"
