@@ -703,9 +703,16 @@ struct BwdArgs {
     // keys: the first split_blocks blocks' query heads go to `parts` units each, launched behind the first_blocks
     // blocks after them (whose whole units are longer)
     int32_t split_blocks, parts, first_blocks;
-    float *part0, *part1;              // and their sums, f32 [split block][head][part][128][D], here
+    float *part0, *part1;              // and their sums, f32 [split block][head][part] x part_at, here
     float sl2, scale;
 };
+
+// Where a unit's f32 sums of four columns (the cg-th four of row `row`) stand, in float4: the rows of a column group are
+// neighbours, as the threads that write and read them are.
+template <int D>
+__device__ __forceinline__ int64_t part_at(int64_t slot, int cg, int row) {
+    return (slot * (D / 4) + cg) * kBlk + row;
+}
 
 // A unit's tiles: kDQ walks the key blocks up to its own; the others every query block from their own on, head by head.
 template <int KIND>
@@ -1109,11 +1116,11 @@ __global__ void __launch_bounds__(kThreads, 1)
                     tmem_ld_wait();
                     if (row < d_shift) continue;
                     if (C::kKeys && d_slot >= 0) {
-                        float4* pp = reinterpret_cast<float4*>((r ? args.part1 : args.part0) +
-                                                               ((int64_t)d_slot * kBlk + row) * D + w * (D / 4) + cc * 32);
+                        float4* pp = reinterpret_cast<float4*>(r ? args.part1 : args.part0) +
+                                     part_at<D>(d_slot, w * (D / 16) + cc * 8, row);
 #pragma unroll
                         for (int k = 0; k < 8; ++k)
-                            pp[k] = make_float4(__uint_as_float(v[4 * k]), __uint_as_float(v[4 * k + 1]),
+                            pp[k * kBlk] = make_float4(__uint_as_float(v[4 * k]), __uint_as_float(v[4 * k + 1]),
                                                 __uint_as_float(v[4 * k + 2]), __uint_as_float(v[4 * k + 3]));
                     } else {
                         store_row32(op + w * (D / 4) + cc * 32, v, f);
@@ -1283,7 +1290,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 
 int64_t delta_ld(int64_t T) { return (T + 63) / 64 * 64; }
 
-// dk, dv rows of the split blocks: their parts summed in order. One warp a row and tensor, 16 bytes of bf16 a lane.
+// dk, dv rows of the split blocks: their parts summed in order. A thread sums 8 columns of a row, a warp those of 32 rows.
 struct SumArgs {
     const int4* blocks;
     const float *dv_parts, *dk_parts;
@@ -1293,26 +1300,26 @@ struct SumArgs {
 };
 template <int D>
 __global__ void __launch_bounds__(256) sum_parts_kernel(const SumArgs a) {
-    constexpr int kPer = 2 * kBlk / 8;  // thread blocks a unit: 8 warps each
-    const int unit = (int)(blockIdx.x / kPer), lane = threadIdx.x & 31;
-    const int r = (int)(blockIdx.x % kPer) * 8 + (threadIdx.x >> 5);
-    const int row = r >> 1, is_dk = r & 1;
+    constexpr int kPer = 2 * kBlk * (D / 8) / 256;  // thread blocks a unit
+    const int unit = (int)(blockIdx.x / kPer), at = (int)(blockIdx.x % kPer) * 256 + threadIdx.x;
+    const int row = at % kBlk, c8 = at / kBlk % (D / 8), is_dk = at / (kBlk * (D / 8));
     const int b = unit / a.heads, h = unit - b * a.heads;
     const int4 e = a.blocks[b];
     const int shift = kBlk - min(kBlk, e.y - e.z * kBlk);
-    if (row < shift || lane * 8 >= D) return;
-    const float* p = (is_dk ? a.dk_parts : a.dv_parts) + ((int64_t)unit * a.parts * kBlk + row) * D + lane * 8;
+    if (row < shift) return;
+    const float4* p = reinterpret_cast<const float4*>(is_dk ? a.dk_parts : a.dv_parts) +
+                      part_at<D>((int64_t)unit * a.parts, c8 * 2, row);
     float v[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = 0.0f;
-    for (int k = 0; k < a.parts; ++k, p += kBlk * D) {
-        const float4 x = *reinterpret_cast<const float4*>(p), y = *reinterpret_cast<const float4*>(p + 4);
+    for (int k = 0; k < a.parts; ++k, p += kBlk * (D / 4)) {
+        const float4 x = p[0], y = p[kBlk];
         v[0] += x.x, v[1] += x.y, v[2] += x.z, v[3] += x.w, v[4] += y.x, v[5] += y.y, v[6] += y.z, v[7] += y.w;
     }
     const float f = is_dk ? a.scale : 1.0f;
     const R97bHeadRows& o = is_dk ? a.dk : a.dv;
     const int64_t tok = (int64_t)e.x + e.z * kBlk + row - shift;
-    *reinterpret_cast<uint4*>(reinterpret_cast<__nv_bfloat16*>(o.ptr) + tok * o.tok + h * o.head + lane * 8) =
+    *reinterpret_cast<uint4*>(reinterpret_cast<__nv_bfloat16*>(o.ptr) + tok * o.tok + h * o.head + c8 * 8) =
         make_uint4(pack_bf16(v[0] * f, v[1] * f), pack_bf16(v[2] * f, v[3] * f), pack_bf16(v[4] * f, v[5] * f),
                    pack_bf16(v[6] * f, v[7] * f));
 }
@@ -1394,7 +1401,7 @@ int run_bwd(const R97bPacked& p, const R97bAttnPackedBwd& a, cudaStream_t st) {
     if (split.blocks > 0 && rc == R97B_OK) {
         const SumArgs s{reinterpret_cast<const int4*>(p.k_blocks), dv_parts, dk_parts, a.dv, a.dk, a.scale, a.Hkv,
                         split.parts};
-        sum_parts_kernel<D><<<split.blocks * a.Hkv * (2 * kBlk / 8), 256, 0, st>>>(s);
+        sum_parts_kernel<D><<<split.blocks * a.Hkv * (2 * kBlk * (D / 8) / 256), 256, 0, st>>>(s);
         rc = launch_status();
     }
     return rc;
