@@ -118,16 +118,36 @@ struct Unit {
     int h, tok0, i, n;  // head, the block's first token, its index in the sequence, its tokens
 };
 
-// 32 accumulator values of a thread's row, times f, as 64 bytes of bf16.
-__device__ __forceinline__ void store_row32(__nv_bfloat16* p, const uint32_t (&r)[32], float f) {
+// 32 accumulator values of each lane's row, times f, as 64 bytes of bf16 at p, for the rows from `shift` on. Four lanes trade
+// 16-byte pieces first, so that they write a row's 64 bytes together: a store of 32 rows takes 32 cycles for its 32 lines.
+__device__ __forceinline__ void store_rows32(__nv_bfloat16* p, int64_t tok, int row, int shift, const uint32_t (&r)[32],
+                                             float f) {
+    uint32_t x[4][4];
 #pragma unroll
-    for (int v = 0; v < 4; ++v) {
-        uint32_t pk[4];
+    for (int v = 0; v < 4; ++v)
 #pragma unroll
         for (int k = 0; k < 4; ++k)
-            pk[k] = pack_bf16(__uint_as_float(r[v * 8 + k * 2]) * f, __uint_as_float(r[v * 8 + k * 2 + 1]) * f);
-        *reinterpret_cast<uint4*>(p + v * 8) = make_uint4(pk[0], pk[1], pk[2], pk[3]);
+            x[v][k] = pack_bf16(__uint_as_float(r[v * 8 + k * 2]) * f, __uint_as_float(r[v * 8 + k * 2 + 1]) * f);
+    const int a = threadIdx.x & 3;
+#pragma unroll
+    for (int bit = 1; bit <= 2; bit *= 2) {  // the 4 x 4 transpose, piece v of lane a for piece a of lane v
+        const bool up = a & bit;
+#pragma unroll
+        for (int v = 0; v < 4; ++v) {
+            if (v & bit) continue;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const uint32_t got = __shfl_xor_sync(0xFFFFFFFFu, up ? x[v][k] : x[v + bit][k], bit);
+                x[v][k] = up ? got : x[v][k];
+                x[v + bit][k] = up ? x[v + bit][k] : got;
+            }
+        }
     }
+    p += a * (8 - tok);
+#pragma unroll
+    for (int v = 0; v < 4; ++v)
+        if (row - a + v >= shift)
+            *reinterpret_cast<uint4*>(p + v * tok) = make_uint4(x[v][0], x[v][1], x[v][2], x[v][3]);
 }
 
 // The TMEM column of 16 consecutive k (k16-th) of a bf16 A operand whose writers own 32 f32 columns each and leave their
@@ -473,7 +493,7 @@ __global__ void __launch_bounds__(FCfg<D>::kThreads, 1)
                 __syncwarp();
                 tmem_ld32(o_tmem + (uint32_t)(cc * 32), r);
                 tmem_ld_wait();
-                if (row >= d_shift) store_row32(op + cc * 32, r, inv);
+                store_rows32(op + cc * 32, args.o_tok, row, d_shift, r, inv);
             }
             tc_fence_before();
             __syncwarp();
@@ -1105,6 +1125,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int r = 0; r < (KIND == kDKV ? 2 : 1); ++r) {
                 // dV takes no scale; dS is kept unscaled in bf16, so dQ and dK take it here
                 const float f = (KIND == kDV || (KIND == kDKV && r == 0)) ? 1.0f : args.scale;
+                const int64_t tok = r ? args.tok1 : args.tok0;
                 __nv_bfloat16* op = r ? args.out1 + d_tok * args.tok1 + d_h * args.head1
                                       : args.out0 + d_tok * args.tok0 + d_h * args.head0;
                 const uint32_t src = (r ? acc1 : acc0) + lane_off + (uint32_t)(w * (D / 4));
@@ -1114,8 +1135,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                     __syncwarp();
                     tmem_ld32(src + (uint32_t)(cc * 32), v);
                     tmem_ld_wait();
-                    if (row < d_shift) continue;
                     if (C::kKeys && d_slot >= 0) {
+                        if (row < d_shift) continue;
                         float4* pp = reinterpret_cast<float4*>(r ? args.part1 : args.part0) +
                                      part_at<D>(d_slot, w * (D / 16) + cc * 8, row);
 #pragma unroll
@@ -1123,7 +1144,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                             pp[k * kBlk] = make_float4(__uint_as_float(v[4 * k]), __uint_as_float(v[4 * k + 1]),
                                                 __uint_as_float(v[4 * k + 2]), __uint_as_float(v[4 * k + 3]));
                     } else {
-                        store_row32(op + w * (D / 4) + cc * 32, v, f);
+                        store_rows32(op + w * (D / 4) + cc * 32, tok, row, d_shift, v, f);
                     }
                 }
             }
