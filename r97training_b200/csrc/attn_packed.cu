@@ -15,8 +15,8 @@
 // one, and the same code serves every length.
 //
 // What bounds it, measured at 2 x 4096 tokens of 16/4 heads of 256 (one sequence of 8192, 16/4 heads of 128): the forward
-// 185-200 us (211) with the tensor pipe busy 76 % (64 %) of the cycles; the backward's passes 298 us dQ, 190-200 dV, 296-315
-// dK (276 dQ, 406 dK and dV) at 71, 83, 81 (75, 76) %. HBM takes 3-15 % of its rate throughout. A tile of dQ at
+// 189-195 us (211-238) with the tensor pipe busy 80 % (64 %) of the cycles; the backward's passes 307 us dQ, 200 dV, 313 dK
+// (276-297 dQ, 406-427 dK and dV) at 74, 84, 82 (76, 76) %. HBM takes 3-13 % of its rate throughout. A tile of dQ at
 // D = 128, by the clock inside the kernel: 2040 cycles, of which the matrix unit works 1900 on products that are 3 x 512 at its
 // full rate (128-column products, both operands from shared memory at D = 128; with q and dO kept in tensor memory the tile
 // took 1 % less, and units started later), and 130 pass between dS and the product that takes it. The exponentials take
@@ -119,7 +119,8 @@ struct Unit {
 };
 
 // 32 accumulator values of each lane's row, times f, as 64 bytes of bf16 at p, for the rows from `shift` on. Four lanes trade
-// 16-byte pieces first, so that they write a row's 64 bytes together: a store of 32 rows takes 32 cycles for its 32 lines.
+// 16-byte pieces first, so that they write a row's 64 bytes together: a store to 32 rows takes 32 cycles for its 32 lines. (2 x
+// 4096 tokens, 16/4 heads of 256: forward 197 -> 189 us; a chat batch of 8192: forward 87 -> 80, dQ 133 -> 125.)
 __device__ __forceinline__ void store_rows32(__nv_bfloat16* p, int64_t tok, int row, int shift, const uint32_t (&r)[32],
                                              float f) {
     uint32_t x[4][4];
@@ -683,7 +684,7 @@ int launch_fwd(const R97bPacked& p, const R97bAttnPackedFwd& a, cudaStream_t st)
 // beside them, and only dS (a product and a rounding) stands between dP and the products that read it.
 // kDQ goes first and leaves every row's delta = dO . O for the others: it has dO in shared memory. (A kernel of its own,
 // bound by its reads of o and dout, cost more: a chat batch of 16384 tokens, 8/2 heads of 128, 72 us for the two, 66 in one;
-// 8192 tokens of 16/4 heads of 256, 149 and 134.) At D = 128 both of a column block's products read one 32 KB copy of it:
+// 8192 tokens of 16/4 heads of 256, 149 and 134, then.) At D = 128 both of a column block's products read one 32 KB copy of it:
 // 12301 tokens 1.68 -> 1.55 ms.
 enum Kind { kDQ = 0, kDKV = 1, kDV = 2, kDK = 3 };
 
@@ -728,7 +729,7 @@ struct BwdArgs {
 };
 
 // Where a unit's f32 sums of four columns (the cg-th four of row `row`) stand, in float4: the rows of a column group are
-// neighbours, as the threads that write and read them are.
+// neighbours, as the threads that write and read them are (row by row, a unit's stores took 4.5 us at D = 256).
 template <int D>
 __device__ __forceinline__ int64_t part_at(int64_t slot, int cg, int row) {
     return (slot * (D / 4) + cg) * kBlk + row;
