@@ -1348,10 +1348,10 @@ __global__ void __launch_bounds__(256) sum_parts_kernel(const SumArgs a) {
 
 // How the key blocks' units are split over their query heads: a block takes as many tiles as its query blocks times the
 // group's heads, and the longest unit bounds the pass where the SMs' average share is less. The blocks (a prefix of the
-// longest-first table) whose units are above 1.25 of that share go to `parts` units each, with their f32 sums in the
+// longest-first table) whose units are above 1.15 of that share go to `parts` units each, with their f32 sums in the
 // workspace and one more launch to add them. Measured, dK and dV with the sums: a chat batch of 8192 tokens, 16/4 heads of
-// 256: 186 us at 1.25, 187 at 1, 206 at 1.5, 222 at 0.75, 230 unsplit; 2 x 4096 tokens, whose longest unit is 1.12 of the
-// share: 511 us unsplit, 523 split (power, not the longest unit, bounds it).
+// 256: 177 us at 1.15, 181 at 1.25, 179 at 1, 196 at 0.8, 213 at 0.6; of 16384 tokens, 8/2 heads of 128: 66.3, 67.8, 66.6, 74, 79;
+// 2 x 4096 tokens, whose longest unit is 1.12 of the share: 517 us unsplit, 528 split (power, not the longest unit, bounds it).
 struct Split {
     int blocks, parts, first;
 };
@@ -1364,7 +1364,7 @@ Split split_of(const R97bPacked& p, int Hq, int Hkv) {
     };
     int64_t tiles = 0;
     for (int b = 0; b < p.n_blocks; ++b) tiles += queries(b);
-    const double limit = 1.25 * (double)(tiles * Hq) / num_sms();
+    const double limit = 1.15 * (double)(tiles * Hq) / num_sms();
     const double longest = (double)(queries(0) * grp);
     if (longest <= limit) return Split{0, 1, 0};
     Split s{0, grp, 0};
