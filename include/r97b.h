@@ -120,8 +120,8 @@ enum {
  * cores with f32 accumulation in TMEM. K2 = 0 drops the second segment; when present, a2/b2 have the
  * same majorness as a1/b1. `splits` > 1 splits the reduction (atomic epilogues, and R97B_EPI_SPLIT_BF16
  * with a workspace `ws` of at least r97b_gemm_workspace_bytes(g) bytes, 256-byte aligned, zeroed once
- * before its first use: its tile counters return to zero at the end of every call, so it stays reusable,
- * but calls that share one workspace must not overlap on the GPU). `bn` picks the
+ * before its first use: its tile counters return to zero at the end of every call, so calls of any shapes share
+ * one, but they must not overlap on the GPU; a call of more than 4096 tiles is not split). `bn` picks the
  * tile: 64, 128 or 256 wide on one SM (128 rows), 512 for a 256 x 256 tile computed by a pair of SMs
  * (tcgen05 cta_group::2, half the operand bytes per multiply-add); 0 picks by shape (the pair for
  * M, N > 128).

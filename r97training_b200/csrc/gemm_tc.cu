@@ -34,6 +34,8 @@ constexpr int kBM = 128;
 constexpr int kBK = 64;               // one 128-byte swizzle row of bf16
 constexpr int kThreads = 256;         // 8 warps: 0 TMA, 1 MMA, 4..7 epilogue
 constexpr int kABytes = kBM * kBK * 2;  // 16 KiB
+constexpr int kSplitTiles = 4096;     // the most tiles a split-K call counts; their counters fit the first partial tile
+static_assert(kSplitTiles * 4 <= kBM * 64 * 4, "counters");
 
 struct KernelArgs {
     int32_t M, N;
@@ -444,6 +446,13 @@ __global__ void __launch_bounds__(kThreads, 1)
                         for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(v[i]);
                         epilogue32(args, kEpiStoreBf16, m, n0, r);
                     }
+                    // a later call of more tiles has counters where this one's first partial tile lies: each thread
+                    // leaves the row that it has read zero
+                    if (tile == 0 && row * BN * 4 < kSplitTiles * 4) {
+                        float4* left = reinterpret_cast<float4*>(args.ws_part + (int64_t)row * BN);
+#pragma unroll 1
+                        for (int i = 0; i < BN / 4; ++i) left[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                    }
                 }
                 continue;
             }
@@ -763,15 +772,6 @@ int num_sms() {
 
 namespace {
 
-// How launch() splits the reduction: k blocks per split and the resulting number of splits.
-void split_geometry(const R97bGemm& g, int& kb_per_split, int& splits) {
-    const int k_total = (int)((g.K1 + kBK - 1) / kBK) + (g.K2 > 0 ? (int)((g.K2 + kBK - 1) / kBK) : 0);
-    int sp = g.splits > 1 ? g.splits : 1;
-    if (sp > k_total) sp = k_total;
-    kb_per_split = (k_total + sp - 1) / sp;
-    splits = (k_total + kb_per_split - 1) / kb_per_split;
-}
-
 int pick_bn(const R97bGemm& g) {
     int bn = g.bn;
     if (bn == 0) bn = g.N <= 64 ? 64 : (g.N <= 128 ? 128 : (g.M <= 128 ? 256 : 512));
@@ -779,8 +779,22 @@ int pick_bn(const R97bGemm& g) {
     return bn;
 }
 
+// How launch() splits the reduction: k blocks per split and the resulting number of splits.
+void split_geometry(const R97bGemm& g, int& kb_per_split, int& splits) {
+    const int k_total = (int)((g.K1 + kBK - 1) / kBK) + (g.K2 > 0 ? (int)((g.K2 + kBK - 1) / kBK) : 0);
+    int sp = g.splits > 1 ? g.splits : 1;
+    if (sp > k_total) sp = k_total;
+    if (g.mode == kEpiSplitBf16) {  // (28 waves of tiles and more gain nothing from a split)
+        const int bn = pick_bn(g);
+        if (((g.M + kBM - 1) / kBM) * ((g.N + bn - 1) / bn) > kSplitTiles) sp = 1;
+    }
+    kb_per_split = (k_total + sp - 1) / sp;
+    splits = (k_total + kb_per_split - 1) / kb_per_split;
+}
+
 // The split-K workspace of kEpiSplitBf16: per-tile counters (rounded up to 256 bytes), then the f32
-// partial tiles [splits][tiles][kBM][bn]. 0 when the call does not split.
+// partial tiles [splits][tiles][kBM][bn]. 0 when the call does not split. A call leaves the first kSplitTiles counters'
+// bytes zero, its own counters and the partial sums that lay among them alike, so that calls of any sizes share one.
 int64_t split_ws_bytes(const R97bGemm& g, int64_t* cnt_bytes) {
     if (g.mode != kEpiSplitBf16) return 0;
     const int bn = pick_bn(g);

@@ -140,7 +140,8 @@ def grad_tiling(M: int, N: int, K: int = 8192, sms: int = 148) -> tuple:
 
 class SplitWorkspace:
     """A zero-initialised device buffer for EPI_SPLIT_BF16 GEMMs on one stream: its tile counters return
-    to zero after every call, so consecutive calls share it; calls on different streams need their own."""
+    to zero after every call, so consecutive calls of any shapes share it; calls on different streams need their
+    own."""
 
     def __init__(self, device, nbytes: int = 64 << 20):
         self.buf = torch.zeros(nbytes // 4, dtype=torch.int32, device=device)
