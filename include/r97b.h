@@ -663,8 +663,10 @@ int64_t r97b_attn_packed_bwd_workspace_bytes(const R97bPacked* p, int32_t Hq, in
 
 /* Rotary tables: cos_tab, sin_tab f32 [n_pos, rot / 2] = amp cos / sin(pos * inv_i), formed in f64.
  * inv_i = theta^(-2 i / rot), then by `scaling`: R97B_ROPE_NONE; R97B_ROPE_LINEAR: inv_i / factor;
- * R97B_ROPE_YARN: inv_i (1 - ramp_i) + inv_i / factor ramp_i, ramp rising from 0 to 1 between the pairs that
- * turn beta_fast and beta_slow times over `original` positions, and amp = 0.1 ln(factor) + 1 (else 1).
+ * R97B_ROPE_YARN: inv_i (1 - ramp_i) + inv_i / factor ramp_i, ramp_i = (i - low) / (high - low) held to [0, 1], where the
+ * pair p(b) = rot ln(original / (2 pi b)) / (2 ln theta) turns b times over `original` positions, low =
+ * max(floor p(beta_fast), 0) and high = min(ceil p(beta_slow), rot - 1) (a step behind low where high <= low), and
+ * amp = 0.1 ln(factor) + 1 (else 1).
  * rot even, factor >= 1 (YaRN: original > 0, beta_fast > beta_slow > 0). */
 enum { R97B_ROPE_NONE = 0, R97B_ROPE_LINEAR = 1, R97B_ROPE_YARN = 2 };
 int r97b_rope_tables(float* cos_tab, float* sin_tab, int64_t n_pos, int32_t rot, double theta, int32_t scaling,

@@ -283,7 +283,8 @@ extern "C" int r97b_rope_tables(float* cos_tab, float* sin_tab, int64_t n_pos, i
         auto pair_of = [&](double beta) {
             return rot * log(original / (2.0 * 3.14159265358979323846 * beta)) / (2.0 * log(theta));
         };
-        const double low = fmax(floor(pair_of(beta_fast)), 0.0), high = fmin(ceil(pair_of(beta_slow)), rot / 2 - 1.0);
+        // the slow end may lie past the last pair, whose ramp then stays short of 1; it is held to the rotated width's dims
+        const double low = fmax(floor(pair_of(beta_fast)), 0.0), high = fmin(ceil(pair_of(beta_slow)), rot - 1.0);
         t.low = low;
         t.width = fmax(high - low, 1e-3);  // a step where both ends fall on one pair
         t.amp = 0.1 * log(factor) + 1.0;
