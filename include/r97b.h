@@ -627,7 +627,8 @@ typedef struct R97bHeadRows {
  * sequence's own tokens; query head h reads key/value head h / (Hq / Hkv). bf16, D 128 or 256; lse f32
  * [Hq, ld_lse >= T], the natural-log log-sum-exp of each row's scaled scores. Rows behind token T are neither
  * read nor written, and a row outside a sequence never reaches that sequence's results whatever it holds. (Inside
- * one, a key or value that is not finite may reach any row: 0 times it is NaN.) Outputs must not overlap the
+ * one, a key or value that is not finite may reach any row: 0 times it is NaN.) A score that falls below f32's range
+ * has the probability 0; a row of such scores alone is NaN with an lse of -inf. Outputs must not overlap the
  * operands or one another (R97B_EINVAL where two start at one address). At most 2^22 - 1 blocks times Hq.
  * Replaces: attention_twin, src/adjoint/host/attention.cpp:261-313, over the ragged batch of
  * include/r97/batch.h. */

@@ -474,7 +474,8 @@ __global__ void __launch_bounds__(FCfg<D>::kThreads, 1)
             if (!warp_wait(&fin_bar[(d_lt & 1) * 4 + q], (uint32_t)((d_lt >> 1) & 1), abort_flag)) return false;
             // the row's sums, moved to the last tile's reference, the last tile's buffer first (which buffer that is
             // differs with the units a CTA has had before, the order of the sum does not)
-            const float m = sums[d_last * 128 + row].x;
+            float m = sums[d_last * 128 + row].x;
+            m = m == -INFINITY ? 0.0f : m;
             float sum = 0.0f;
 #pragma unroll
             for (int back = 0, b = d_last; back < NB; ++back) {
@@ -561,7 +562,7 @@ __global__ void __launch_bounds__(FCfg<D>::kThreads, 1)
                 // first P V waits for it.
                 if (j > 0 && d_lt >= 0 && !(ok = drain())) break;
                 if (!(ok = warp_wait(&max_bar[prev * 4 + q], w == 0 ? phase ^ 1u : phase, abort_flag))) break;
-                float mn = top == -INFINITY ? 0.0f : top;  // a row of nothing visible (or of -inf scores) sums to 0
+                float mn = top;  // -inf while the row has seen nothing (or scores of -inf alone), whatever comes after
                 if (j > 0) {
                     const float mp = ref_m[prev * 128 + row];
                     mn = top <= mp + kLazy ? mp : top;
@@ -569,7 +570,7 @@ __global__ void __launch_bounds__(FCfg<D>::kThreads, 1)
                         // O still holds sums relative to mp: wait for the last P V, then move it to mn
                         if (!(ok = warp_wait(&pv_done[prev], w == 0 ? phase ^ 1u : phase, abort_flag))) break;
                         tc_fence_after();
-                        const float f = ex2_ftz(mp - mn);
+                        const float f = mn == mp ? 1.0f : ex2_ftz(mp - mn);
 #pragma unroll 1
                         for (int cc = 0; cc < D / 32; ++cc) {
                             uint32_t r[32];
@@ -584,10 +585,10 @@ __global__ void __launch_bounds__(FCfg<D>::kThreads, 1)
                 ref_m[w * 128 + row] = mn;
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&max_bar[w * 4 + q]);
-                if (j >= NB) l *= ex2_ftz(m - mn);
+                if (j >= NB && m != mn) l *= ex2_ftz(m - mn);
                 m = mn;
                 float2 s[2] = {both(0.0f), both(0.0f)};
-                const float2 sl2 = both(args.sl2), off = both(-m);
+                const float2 sl2 = both(args.sl2), off = both(m == -INFINITY ? 0.0f : -m);
                 // a chunk's P, as the at-th 16 of the buffer's last 64 columns: the scores there are read by then
                 auto probability = [&](float(&x)[32], int at) {
                     uint32_t pk[16];
