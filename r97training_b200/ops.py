@@ -579,7 +579,7 @@ def rope_tables(n_pos: int, rot: int, theta: float, scaling=None, device="cuda",
     if n_pos < 1 or rot < 2 or rot % 2:
         raise R97bError(f"rope_tables: n_pos {n_pos}, rot {rot}")
     device = torch.device(device)
-    if device.index is None:
+    if device.type == "cuda" and device.index is None:
         device = torch.device("cuda", torch.cuda.current_device())
     st = _packed_stream(stream, device, "rope_tables")
     if stream is not None:
