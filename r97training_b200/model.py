@@ -607,12 +607,9 @@ class TrainStep:
         """The fixed frame's q/k norm and rotation and the attention core: (q, k, v, output, (output, lse))."""
         cfg, S = self.cfg, self.cfg.seq
         Hq, Hkv, Dh, B = cfg.attn_heads, cfg.attn_kv_heads, cfg.attn_head_dim, cfg.micro_batch
-        x = y
-        if cfg.rope_interleaved:
-            raise ops.R97bError("interleaved rotary pairs are for packed batches")
-        qr = torch.empty((B, Hq, S, Dh), dtype=torch.bfloat16, device=x.device)
-        kr = torch.empty((B, Hkv, S, Dh), dtype=torch.bfloat16, device=x.device)
-        vt = torch.empty((B, Hkv, S, Dh), dtype=torch.bfloat16, device=x.device)
+        qr = torch.empty((B, Hq, S, Dh), dtype=torch.bfloat16, device=y.device)
+        kr = torch.empty((B, Hkv, S, Dh), dtype=torch.bfloat16, device=y.device)
+        vt = torch.empty((B, Hkv, S, Dh), dtype=torch.bfloat16, device=y.device)
         ops.qk_norm_rope_fwd(y, 2 * Dh, Hq, Dh, blk["q_norm"], self.model.rope_cos, self.model.rope_sin,
                              cfg.rotary_dim, S, cfg.eps, qr)
         ops.qk_norm_rope_fwd(y[:, qn:], Dh, Hkv, Dh, blk["k_norm"], self.model.rope_cos, self.model.rope_sin,
@@ -707,6 +704,8 @@ class TrainStep:
         if batch is None:
             if self.packed is not None:
                 raise ops.R97bError("the step is in a packed run")
+            if self.cfg.rope_interleaved and "attn" in self.cfg.kinds:
+                raise ops.R97bError("interleaved rotary pairs are for packed batches")
             return self._run(ids, targets, n_scored)
         if ids.numel() != batch.T or (targets is not None and targets.numel() != batch.T):
             raise ops.R97bError(f"a packed batch of {batch.T} tokens, {ids.numel()} ids")
