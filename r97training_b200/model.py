@@ -706,15 +706,25 @@ class TrainStep:
                 raise ops.R97bError("the step is in a packed run")
             if self.cfg.rope_interleaved and "attn" in self.cfg.kinds:
                 raise ops.R97bError("interleaved rotary pairs are for packed batches")
-            return self._run(ids, targets, n_scored)
+            return self._joined(ids, targets, n_scored)
         if ids.numel() != batch.T or (targets is not None and targets.numel() != batch.T):
             raise ops.R97bError(f"a packed batch of {batch.T} tokens, {ids.numel()} ids")
         keep = self.T, self.cu_dev, self.plan
         self.T, self.cu_dev, self.plan, self.packed = batch.T, batch.cu_dev, batch.gdn, batch
         try:
-            return self._run(ids, targets, n_scored)
+            return self._joined(ids, targets, n_scored)
         finally:
             (self.T, self.cu_dev, self.plan), self.packed = keep, None
+
+    def _joined(self, *args):
+        """_run; where it raises, the caller's stream waits for the decodes still on the side stream, whose buffers may
+        go with the step."""
+        try:
+            return self._run(*args)
+        except BaseException:
+            if self.side is not None and not torch.cuda.is_current_stream_capturing():
+                torch.cuda.current_stream().wait_stream(self.side)
+            raise
 
     def _run(self, ids, targets, n_scored):
         cfg, model, T = self.cfg, self.model, self.T
