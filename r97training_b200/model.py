@@ -330,8 +330,8 @@ class PackedBatch:
         self.T = self.plan.T
         if self.T == 0:
             raise ops.R97bError("a packed batch needs a token")
-        if self.plan.max_len > model.rope_cos.shape[0]:
-            raise ops.R97bError(f"a sequence of {self.plan.max_len} tokens for {model.rope_cos.shape[0]} positions")
+        self.heads = cfg.gdn_heads, cfg.gdn_qk_heads
+        self.check(model)
         cu = self.plan.cu
         self.cu_dev = torch.from_numpy(cu).to(model.device)
         self.gdn = GdnPlan(cu, cfg.gdn_heads, cfg.gdn_qk_heads, model.device)
@@ -340,6 +340,16 @@ class PackedBatch:
         nxt[cu[1:][self.plan.lens > 0] - 1] = -1
         self.next = torch.from_numpy(nxt).to(model.device)
         self.n_next = int((nxt >= 0).sum())
+
+    def check(self, model: HybridModel):
+        """Raises where the batch's tables are not of `model`'s positions, GDN heads and device: its kernels would read
+        past them."""
+        cfg, table = model.cfg, model.rope_cos
+        if self.plan.max_len > table.shape[0]:
+            raise ops.R97bError(f"a sequence of {self.plan.max_len} tokens for {table.shape[0]} positions")
+        if self.heads != (cfg.gdn_heads, cfg.gdn_qk_heads) or self.plan.device != table.device:
+            raise ops.R97bError(f"a packed batch for {self.heads} GDN heads on {self.plan.device}, the model has "
+                                f"{(cfg.gdn_heads, cfg.gdn_qk_heads)} on {table.device}")
 
 
 class Workspace:
@@ -707,6 +717,7 @@ class TrainStep:
             if self.cfg.rope_interleaved and "attn" in self.cfg.kinds:
                 raise ops.R97bError("interleaved rotary pairs are for packed batches")
             return self._joined(ids, targets, n_scored)
+        batch.check(self.model)
         if ids.numel() != batch.T or (targets is not None and targets.numel() != batch.T):
             raise ops.R97bError(f"a packed batch of {batch.T} tokens, {ids.numel()} ids")
         keep = self.T, self.cu_dev, self.plan
