@@ -56,8 +56,8 @@ class HybridConfig:
     lr: float = 1e-4
     seed: int = 1234
     lora_mlp: bool = True      # adapters on the MLP projections too (config 4 names only the mixers')
-    # rotary positions of packed batches: the longest sequence (0: seq), the scaling of far positions
-    # (ops.rope_tables) and the pairing (the fixed frame takes neighbouring halves, unscaled)
+    # rotary positions: the longest sequence of a packed batch (0: seq); the scaling of far positions (ops.rope_tables),
+    # which the fixed frame and the C++ step follow too; the pairing (interleaved pairs are for packed batches alone)
     max_pos: int = 0
     rope_scaling: dict | None = None
     rope_interleaved: bool = False
