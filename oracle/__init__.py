@@ -48,6 +48,10 @@ def oracle_lib():
     return _oracle
 
 
+class ReferenceAbsent(FileNotFoundError):
+    """The reference's host library is asked for where neither it nor the sources to build it from are present."""
+
+
 def ref_available() -> bool:
     return os.path.exists(os.path.join(HERE, "_ref", "libr97ref.so")) or os.path.isdir(
         os.path.join(REF_TREE, "src"))
@@ -60,7 +64,7 @@ def ref_lib():
         path = os.path.join(HERE, "_ref", "libr97ref.so")
         if not os.path.exists(path):
             if not os.path.isdir(os.path.join(REF_TREE, "src")):
-                raise FileNotFoundError("oracle/_ref/libr97ref.so is not built and the reference tree is absent")
+                raise ReferenceAbsent("oracle/_ref/libr97ref.so is not built and the reference tree is absent")
             build(ref=True)
         # global: a device-row plugin loaded after it binds to this registry by name
         lib = ctypes.CDLL(path, mode=ctypes.RTLD_GLOBAL)

@@ -19,6 +19,17 @@ def pytest_configure(config):
         oracle.ref_lib()
 
 
+@pytest.hookimpl(wrapper=True)
+def pytest_runtest_call(item):
+    """A test that compares with the reference's own host rows is skipped where they cannot be had, whichever of the
+    oracle's calls meets it first."""
+    import oracle
+    try:
+        return (yield)
+    except oracle.ReferenceAbsent as e:
+        pytest.skip(str(e))
+
+
 @pytest.fixture(scope="session")
 def cuda():
     import torch
