@@ -12,7 +12,10 @@
 // Blocks that end inside a tile sit at the tile's END, behind zero rows: the tensor maps address row r < 128 of the
 // block that begins at token t as (column, r, t), token and row with one stride, and a box that starts at row n - 128
 // reads zeros before the block's first token. So no load or store touches a row of another sequence or behind the last
-// one, and the same code serves every length.
+// one, and the same code serves every length. The maps claim the batch's own rows alone, which leaves out the blocks that
+// begin in its last 127 tokens. A second map, which claims the last block's n tokens from each token on, holds that block and
+// any other of n tokens at most; what is left (short sequences at the end, longer than the last one's last block) the producer
+// warps copy themselves, 16 bytes a lane.
 //
 // What bounds it, measured at 2 x 4096 tokens of 16/4 heads of 256 (one sequence of 8192, 16/4 heads of 128): the forward
 // 189-195 us (211-238) with the tensor pipe busy 80 % (64 %) of the cycles; the backward's passes 307 us dQ, 200 dV, 313 dK
@@ -27,6 +30,7 @@
 #include "sm100.cuh"
 #include "r97b_internal.h"
 #include "fastmath.cuh"
+#include "wmma16.cuh"
 
 #include <algorithm>
 #include <cuda_bf16.h>
@@ -94,6 +98,7 @@ struct FCfg {
     static constexpr int kFinOff = kMaxOff + kBufs * 512;  // float2 [2 (unit parity)][kBufs][128]: (reference, sum)
     static constexpr int kSmemBytes = kFinOff + 2 * kBufs * 1024 + 1024;
     static constexpr int kVRows = kChunk / (D * 2);      // keys of one V chunk
+    static constexpr int kVLog2 = kVRows == 64 ? 6 : 5;
 };
 
 struct FwdArgs {
@@ -101,8 +106,11 @@ struct FwdArgs {
     __nv_bfloat16* o;
     float* lse;
     int64_t o_tok, o_head, ld_lse;
-    int32_t Hq, grp;
+    int32_t Hq, grp, T;
     int32_t q_head, k_head, v_head;
+    int32_t tail_n;                  // tokens of the batch's last block
+    const __nv_bfloat16 *q, *k, *v;  // the operands again, for copy_chunk
+    int64_t q_tok, k_tok, v_tok;
     float sl2;   // |scale| log2 e (1 for a scale of 0), so that the row maximum is the scores'
     float sign;  // of the scale: 1, -1 or 0
 };
@@ -112,6 +120,30 @@ struct FwdArgs {
 __device__ __forceinline__ void settle(const volatile int* abort) {
     if (!*abort) return;
     for (const long long t0 = clock64(); clock64() - t0 < 4000000;) __nanosleep(1000);
+}
+
+// By a whole warp: a chunk that TMA boxes of 2^log2_rows rows and 64 columns would fill (128-byte swizzle), the tile's rows
+// from row0 on and, when those are not the whole tile, its further columns box by box. The block's tokens, the first at p with
+// `tok` elements from one to the next, are the tile's rows from `shift` on; those before are zero.
+__device__ __forceinline__ void copy_chunk(uint8_t* chunk, const __nv_bfloat16* p, int64_t tok, int log2_rows, int row0, int shift) {
+#pragma unroll 2
+    for (int k = threadIdx.x & 31; k < kChunk / 16; k += 32) {
+        const int r = k >> 3, c = k & 7, t = row0 + (r & ((1 << log2_rows) - 1)) - shift;
+        cp_async16(chunk + r * 128 + ((c ^ (r & 7)) << 4), p + (t >= 0 ? t : 0) * tok + (r >> log2_rows) * 64 + c * 8, t >= 0);
+    }
+}
+// The warp's copies have landed and may be read by the tensor core: completes the barrier that a box's bytes would.
+__device__ __forceinline__ void copies_done(uint64_t* bar, uint32_t lead) {
+    cp_async_commit();
+    cp_async_wait_all();
+    fence_proxy_async_smem();
+    __syncwarp();
+    if (lead) mbar_arrive(bar);
+}
+
+// Which of an operand's two maps holds the block of n tokens at `tok`: 0, 1, or -1 for neither.
+__device__ __forceinline__ int map_of(int tok, int n, int T, int tail_n) {
+    return rows_map_has(tok, T) ? 0 : (n <= tail_n ? 1 : -1);
 }
 
 struct Unit {
@@ -215,7 +247,8 @@ __device__ __forceinline__ Unit unit_geom(const int4* blocks, int heads, int u) 
 template <int D>
 __global__ void __launch_bounds__(FCfg<D>::kThreads, 1)
     fwd_kernel(const __grid_constant__ CUtensorMap tQ, const __grid_constant__ CUtensorMap tK,
-               const __grid_constant__ CUtensorMap tV, const FwdArgs args) {
+               const __grid_constant__ CUtensorMap tV, const __grid_constant__ CUtensorMap tQ1,
+               const __grid_constant__ CUtensorMap tK1, const __grid_constant__ CUtensorMap tV1, const FwdArgs args) {
     using C = FCfg<D>;
     constexpr int ND = D / 64, NB = C::kBufs;
     constexpr int kVC = kBlk / C::kVRows;  // V chunks of a tile
@@ -297,22 +330,29 @@ __global__ void __launch_bounds__(FCfg<D>::kThreads, 1)
         int waiting = 0, led = 0, lt = 0;
         bool more = true, fresh = true;  // a unit for `ahead`; its Q not loaded yet
         int u = blockIdx.x;
+        // Rolled, and with one call for keys and values: the warps share an instruction cache, which a second copy of this (the
+        // code for the batch's last blocks) overfilled (2 x 4096 tokens of 16/4 heads of 256: 229 -> 239 us back to back).
         auto load = [&](bool v, const Cursor& c) {
             const int tok = c.seq0 + c.j * kBlk, r0 = c.j == c.i ? -c.shift : 0;
-            const int x = c.x * (v ? args.v_head : args.k_head);
-#pragma unroll
+            const int at = map_of(tok, kBlk + r0, args.T, args.tail_n);
+            const CUtensorMap* map = v ? (at == 1 ? &tV1 : &tV) : (at == 1 ? &tK1 : &tK);
+#pragma unroll 1
             for (int ch = p; ch < (v ? kVC : ND); ch += 2) {
-                if (!(ok = ok && warp_wait(&empty_bar[stage], phase ^ 1u, abort_flag))) return;
-                if (lead) {
-                    uint8_t* st = ring + stage * kChunk;
+                if (!(ok = warp_wait(&empty_bar[stage], phase ^ 1u, abort_flag))) return;
+                uint8_t* st = ring + stage * kChunk;
+                const int row0 = v ? (ch + kVC / 2) % kVC * C::kVRows : 0;  // keys 64 on first
+                const int col = c.x * (v ? args.v_head : args.k_head) + (v ? 0 : 64 * ch);
+                if (at < 0) {
+                    const int64_t step = v ? args.v_tok : args.k_tok;
+                    copy_chunk(st, (v ? args.v : args.k) + tok * step + col, step, v ? C::kVLog2 : 7, row0, -r0);
+                    copies_done(&full_bar[stage], lead);
+                } else if (lead) {
                     mbar_expect_tx(&full_bar[stage], kChunk);
+                    tma_load_3d(st, map, &full_bar[stage], col, r0 + row0, tok);
                     if (v) {
 #pragma unroll
-                        for (int n = 0; n < ND; ++n)
-                            tma_load_3d(st + n * (C::kVRows * 128), &tV, &full_bar[stage], x + 64 * n,
-                                        r0 + (ch + kVC / 2) % kVC * C::kVRows, tok);  // keys 64 on first
-                    } else {
-                        tma_load_3d(st, &tK, &full_bar[stage], x + 64 * ch, r0, tok);
+                        for (int n = 1; n < ND; ++n)
+                            tma_load_3d(st + n * (C::kVRows * 128), map, &full_bar[stage], col + 64 * n, r0 + row0, tok);
                     }
                 }
                 if ((stage += 2) >= C::kStages) {
@@ -331,10 +371,17 @@ __global__ void __launch_bounds__(FCfg<D>::kThreads, 1)
                     ahead = Cursor{un.h / args.grp, un.tok0 - un.i * kBlk, un.i, kBlk - un.n, 0};
                     const int qs = lt % C::kQStages;
                     if (!(ok = warp_wait(&q_empty[qs], (uint32_t)((lt / C::kQStages) & 1) ^ 1u, abort_flag))) break;
-                    if (lead) {
+                    const int at = map_of(un.tok0, un.n, args.T, args.tail_n);
+                    if (at < 0) {
+#pragma unroll 1
+                        for (int s = p; s < ND; s += 2)
+                            copy_chunk(smem + qs * C::kQBytes + s * kChunk,
+                                       args.q + un.tok0 * args.q_tok + un.h * args.q_head + 64 * s, args.q_tok, 7, 0, ahead.shift);
+                        copies_done(&q_full[qs], lead);
+                    } else if (lead) {
                         mbar_expect_tx(&q_full[qs], C::kQBytes / 2);
                         for (int s = p; s < ND; s += 2)
-                            tma_load_3d(smem + qs * C::kQBytes + s * kChunk, &tQ, &q_full[qs], un.h * args.q_head + 64 * s,
+                            tma_load_3d(smem + qs * C::kQBytes + s * kChunk, at ? &tQ1 : &tQ, &q_full[qs], un.h * args.q_head + 64 * s,
                                         -ahead.shift, un.tok0);
                     }
                     if (waiting == 0) {
@@ -348,18 +395,22 @@ __global__ void __launch_bounds__(FCfg<D>::kThreads, 1)
                     ++lt;
                 }
             }
-            if (more) {
-                if (p && ahead.j == ahead.i && !(ok = queue.ask(lt - 1, lead))) break;
-                load(false, ahead);
-                fresh = ++ahead.j > ahead.i;
-                if (++led < NB) continue;
-            }
-            if (led == 0) break;
-            load(true, behind);
-            --led;
-            if (++behind.j > behind.i) {
-                behind = w0, w0 = w1;
-                --waiting;
+            if (!more && led == 0) break;
+#pragma unroll 1
+            for (int v = more ? 0 : 1; v < 2; ++v) {  // K of the tile ahead, V of the one behind
+                if (!v && p && ahead.j == ahead.i && !(ok = queue.ask(lt - 1, lead))) break;
+                load(v, v ? behind : ahead);
+                if (!ok) break;
+                if (!v) {
+                    fresh = ++ahead.j > ahead.i;
+                    if (++led < NB) break;
+                } else {
+                    --led;
+                    if (++behind.j > behind.i) {
+                        behind = w0, w0 = w1;
+                        --waiting;
+                    }
+                }
             }
         }
     } else if (warp == 1) {
@@ -645,25 +696,46 @@ __global__ void __launch_bounds__(FCfg<D>::kThreads, 1)
     }
 }
 
+// The tokens of the batch's last block, 128 when it is full.
+int tail_tokens(const R97bPacked& p) {
+    for (int b = p.n_blocks - 1; b >= 0; --b) {  // (short sequences stand last)
+        const int32_t* e = p.k_blocks_host + 4 * (int64_t)b;
+        if ((int64_t)e[0] + e[1] == p.T) return (e[1] - 1) % kBlk + 1;
+    }
+    return 0;
+}
+// An operand's maps: the batch's, and the last block's (the first again where that is full).
+bool make_maps(CUtensorMap* m, const R97bHeadRows& r, int64_t heads, int32_t D, int64_t T, int tail, int box_rows) {
+    if (!make_rows_map(&m[0], r, heads, D, T, kBlk, box_rows)) return false;
+    m[1] = m[0];
+    return tail == 0 || tail == kBlk || make_rows_map(&m[1], r, heads, D, T, tail, box_rows);
+}
+
 template <int D>
 int launch_fwd(const R97bPacked& p, const R97bAttnPackedFwd& a, cudaStream_t st) {
     using C = FCfg<D>;
     static_assert(C::kSmemBytes <= 232448, "shared memory");
-    CUtensorMap q, k, v;
-    if (!make_rows_map(&q, a.q, a.Hq, D, p.T, kBlk) || !make_rows_map(&k, a.k, a.Hkv, D, p.T, kBlk) ||
-        !make_rows_map(&v, a.v, a.Hkv, D, p.T, C::kVRows))
+    const int tail = tail_tokens(p);
+    CUtensorMap q[2], k[2], v[2];
+    if (!make_maps(q, a.q, a.Hq, D, p.T, tail, kBlk) || !make_maps(k, a.k, a.Hkv, D, p.T, tail, kBlk) ||
+        !make_maps(v, a.v, a.Hkv, D, p.T, tail, C::kVRows))
         return R97B_EINVAL;
     FwdArgs r{};
+    r.tail_n = tail;
     r.blocks = reinterpret_cast<const int4*>(p.q_blocks);
     r.o = reinterpret_cast<__nv_bfloat16*>(a.o.ptr);
     r.lse = a.lse;
     r.o_tok = a.o.tok, r.o_head = a.o.head, r.ld_lse = a.ld_lse;
     r.Hq = a.Hq, r.grp = a.Hq / a.Hkv;
+    r.T = (int32_t)p.T;
     r.q_head = (int32_t)a.q.head, r.k_head = (int32_t)a.k.head, r.v_head = (int32_t)a.v.head;
+    r.q = reinterpret_cast<const __nv_bfloat16*>(a.q.ptr), r.q_tok = a.q.tok;
+    r.k = reinterpret_cast<const __nv_bfloat16*>(a.k.ptr), r.k_tok = a.k.tok;
+    r.v = reinterpret_cast<const __nv_bfloat16*>(a.v.ptr), r.v_tok = a.v.tok;
     r.sl2 = a.scale == 0.0f ? 1.0f : fabsf(a.scale) * kLog2e;
     r.sign = a.scale == 0.0f ? 0.0f : (a.scale < 0.0f ? -1.0f : 1.0f);
     if (!smem_opt_in(fwd_kernel<D>, C::kSmemBytes)) return R97B_ELAUNCH;
-    fwd_kernel<D><<<p.n_blocks * a.Hq, C::kThreads, C::kSmemBytes, st>>>(q, k, v, r);
+    fwd_kernel<D><<<p.n_blocks * a.Hq, C::kThreads, C::kSmemBytes, st>>>(q[0], k[0], v[0], q[1], k[1], v[1], r);
     return launch_status();
 }
 
@@ -711,6 +783,9 @@ struct BCfg {
     static constexpr int kVRows = kChunk / (D * 2);
 };
 
+struct TailMaps {
+    CUtensorMap a0, a1, b0, b1, c0;
+};
 struct BwdArgs {
     const int4* blocks;
     const float* lse;
@@ -721,6 +796,9 @@ struct BwdArgs {
     __nv_bfloat16 *out0, *out1;        // kDQ: dq; kDKV: dv, dk; kDV: dv; kDK: dk
     int64_t tok0, head0, tok1, head1;
     int32_t a0_head, a1_head, b0_head, b1_head, c0_head;
+    int32_t T, tail_n;                 // tokens of the batch, and of its last block
+    const __nv_bfloat16 *a0, *a1, *b0, *b1, *c0;  // the operands again, for copy_chunk
+    int64_t a0_tok, a1_tok, b0_tok, b1_tok, c0_tok;
     int32_t heads, grp;                // the rows' heads (query heads for kDQ, key/value heads else)
     // keys: the first split_blocks blocks' query heads go to `parts` units each, launched behind the first_blocks
     // blocks after them (whose whole units are longer)
@@ -786,7 +864,7 @@ template <int D, int KIND>
 __global__ void __launch_bounds__(kThreads, 1)
     bwd_kernel(const __grid_constant__ CUtensorMap tA0, const __grid_constant__ CUtensorMap tA1,
                const __grid_constant__ CUtensorMap tB0, const __grid_constant__ CUtensorMap tB1,
-               const __grid_constant__ CUtensorMap tC0, const BwdArgs args) {
+               const __grid_constant__ CUtensorMap tC0, const __grid_constant__ TailMaps tails, const BwdArgs args) {
     using C = BCfg<D, KIND>;
     constexpr int ND = D / 64;
     constexpr int kVC = kBlk / C::kVRows;
@@ -874,27 +952,43 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const Walk<KIND> wk(args, u);
                 if (p == 0 || C::kDP) {  // a resident operand each
                     if (!(ok = warp_wait(&a_empty[p], (uint32_t)(lt & 1) ^ 1u, abort_flag))) break;
-                    if (lead) {
+                    const int x = wk.h * (p ? args.a1_head : args.a0_head), at = map_of(wk.tok0, wk.n, args.T, args.tail_n);
+                    if (at < 0) {
+                        const int64_t step = p ? args.a1_tok : args.a0_tok;
+#pragma unroll 1
+                        for (int s = 0; s < ND; ++s)
+                            copy_chunk(smem + p * C::kABytes + s * kChunk, (p ? args.a1 : args.a0) + wk.tok0 * step + x + 64 * s,
+                                       step, 7, 0, wk.shift());
+                        copies_done(&a_full[p], lead);
+                    } else if (lead) {
+                        const CUtensorMap* map = p ? (at ? &tails.a1 : &tA1) : (at ? &tails.a0 : &tA0);
                         mbar_expect_tx(&a_full[p], C::kABytes);
                         for (int s = 0; s < ND; ++s)
-                            tma_load_3d(smem + p * C::kABytes + s * kChunk, p ? &tA1 : &tA0, &a_full[p],
-                                        wk.h * (p ? args.a1_head : args.a0_head) + 64 * s, -wk.shift(), wk.tok0);
+                            tma_load_3d(smem + p * C::kABytes + s * kChunk, map, &a_full[p], x + 64 * s, -wk.shift(), wk.tok0);
                     }
                 }
                 int blk0 = 0, head0 = 0, blk1 = wk.first_block(), head1 = wk.first_head();  // of tiles j and j + 1
                 if constexpr (C::kWhole) {
                     // each of the two warps its operand's blocks, in slots taken in turn
-                    const CUtensorMap* map = p ? &tB1 : &tB0;
                     const int head_stride = p ? args.b1_head : args.b0_head;
                     for (int j = 0; j < wk.tiles && ok; ++j) {
                         if (p && j + 1 == wk.tiles && !(ok = queue.ask(lt, lead))) break;
                         if (!(ok = warp_wait(&empty_bar[stage], phase ^ 1u, abort_flag))) break;
-                        if (lead) {
+                        const int tok = wk.seq0 + blk1 * kBlk, shift = wk.shift_of(blk1), x = head1 * head_stride;
+                        const int at = map_of(tok, kBlk - shift, args.T, args.tail_n);
+                        if (at < 0) {
+                            const int64_t step = p ? args.b1_tok : args.b0_tok;
+#pragma unroll 1
+                            for (int ch = 0; ch < ND; ++ch)
+                                copy_chunk(ring + stage * C::kSlot + ch * kChunk, (p ? args.b1 : args.b0) + tok * step + x + 64 * ch,
+                                           step, 7, 0, shift);
+                            copies_done(&full_bar[stage], lead);
+                        } else if (lead) {
+                            const CUtensorMap* map = p ? (at ? &tails.b1 : &tB1) : (at ? &tails.b0 : &tB0);
                             mbar_expect_tx(&full_bar[stage], C::kSlot);
 #pragma unroll
                             for (int ch = 0; ch < ND; ++ch)
-                                tma_load_3d(ring + stage * C::kSlot + ch * kChunk, map, &full_bar[stage],
-                                            head1 * head_stride + 64 * ch, -wk.shift_of(blk1), wk.seq0 + blk1 * kBlk);
+                                tma_load_3d(ring + stage * C::kSlot + ch * kChunk, map, &full_bar[stage], x + 64 * ch, -shift, tok);
                         }
                         if ((stage += 2) >= C::kStages) {
                             stage -= C::kStages;
@@ -914,15 +1008,23 @@ __global__ void __launch_bounds__(kThreads, 1)
                             const bool mn = s == 1;
                             const int tile = mn ? j : j + 1;
                             if (tile < 0 || tile >= wk.tiles || (s == 2 && !C::kDP)) continue;
-                            const CUtensorMap* map = s == 0 ? &tB0 : (s == 1 ? &tC0 : &tB1);
                             const int head_stride = s == 0 ? args.b0_head : (s == 1 ? args.c0_head : args.b1_head);
                             const int blk = mn ? blk0 : blk1, x = (mn ? head0 : head1) * head_stride;
                             const int r0 = -wk.shift_of(blk), tok = wk.seq0 + blk * kBlk;
+                            const int at = map_of(tok, kBlk + r0, args.T, args.tail_n);
+                            const CUtensorMap* map = at == 1 ? (s == 0 ? &tails.b0 : (s == 1 ? &tails.c0 : &tails.b1))
+                                                             : (s == 0 ? &tB0 : (s == 1 ? &tC0 : &tB1));
 #pragma unroll 1
                             for (int ch = p; ch < (mn ? kVC : ND); ch += 2) {
                                 if (!(ok = warp_wait(&empty_bar[stage], phase ^ 1u, abort_flag))) break;
-                                if (lead) {
-                                    uint8_t* st = ring + stage * kChunk;
+                                uint8_t* st = ring + stage * kChunk;
+                                if (at < 0) {
+                                    const int64_t step = s == 0 ? args.b0_tok : (s == 1 ? args.c0_tok : args.b1_tok);
+                                    const __nv_bfloat16* rows = s == 0 ? args.b0 : (s == 1 ? args.c0 : args.b1);
+                                    copy_chunk(st, rows + tok * step + x + (mn ? 0 : 64 * ch), step, mn ? (C::kVRows == 64 ? 6 : 5) : 7,
+                                               mn ? ch * C::kVRows : 0, -r0);
+                                    copies_done(&full_bar[stage], lead);
+                                } else if (lead) {
                                     mbar_expect_tx(&full_bar[stage], kChunk);
                                     if (mn) {
 #pragma unroll
@@ -1378,7 +1480,7 @@ Split split_of(const R97bPacked& p, int Hq, int Hkv) {
 int64_t part_floats(const Split& s, int Hkv, int D) { return (int64_t)s.blocks * s.parts * Hkv * kBlk * D; }
 
 template <int D, int KIND>
-int launch_bwd(const R97bPacked& p, const R97bAttnPackedBwd& a, float* delta, const Split& split, float* dv_parts,
+int launch_bwd(const R97bPacked& p, const R97bAttnPackedBwd& a, float* delta, const Split& split, int tail, float* dv_parts,
                float* dk_parts, cudaStream_t st) {
     using C = BCfg<D, KIND>;
     static_assert(C::kSmemBytes <= 232448, "shared memory");
@@ -1387,13 +1489,16 @@ int launch_bwd(const R97bPacked& p, const R97bAttnPackedBwd& a, float* delta, co
     const R97bHeadRows &a0 = dq ? a.q : a.k, &a1 = dq ? a.dout : a.v, &b0 = dq ? a.k : a.q, &b1 = dq ? a.v : a.dout;
     const R97bHeadRows& c0 = dq ? a.k : (KIND == kDK ? a.q : a.dout);  // (kWhole: the accumulating products reuse b0, b1)
     const int ha = dq ? a.Hq : a.Hkv, hb = dq ? a.Hkv : a.Hq;
-    CUtensorMap m[5];
-    if (!make_rows_map(&m[0], a0, ha, D, p.T, kBlk) || !make_rows_map(&m[2], b0, hb, D, p.T, kBlk)) return R97B_EINVAL;
-    m[1] = m[0], m[3] = m[2], m[4] = m[2];  // where the kind has no such stream
-    if (C::kDP && (!make_rows_map(&m[1], a1, ha, D, p.T, kBlk) || !make_rows_map(&m[3], b1, hb, D, p.T, kBlk)))
+    CUtensorMap m[5][2];
+    auto same = [&](int i, int j) { m[i][0] = m[j][0], m[i][1] = m[j][1]; };
+    if (!make_maps(m[0], a0, ha, D, p.T, tail, kBlk) || !make_maps(m[2], b0, hb, D, p.T, tail, kBlk)) return R97B_EINVAL;
+    same(1, 0), same(3, 2), same(4, 2);  // where the kind has no such stream
+    if (C::kDP && (!make_maps(m[1], a1, ha, D, p.T, tail, kBlk) || !make_maps(m[3], b1, hb, D, p.T, tail, kBlk)))
         return R97B_EINVAL;
-    if (!C::kWhole && !make_rows_map(&m[4], c0, hb, D, p.T, C::kVRows)) return R97B_EINVAL;
+    if (!C::kWhole && !make_maps(m[4], c0, hb, D, p.T, tail, C::kVRows)) return R97B_EINVAL;
+    const TailMaps tails{m[0][1], m[1][1], m[2][1], m[3][1], m[4][1]};
     BwdArgs r{};
+    r.tail_n = tail;
     r.blocks = reinterpret_cast<const int4*>(dq ? p.q_blocks : p.k_blocks);
     r.lse = a.lse, r.ld_lse = a.ld_lse, r.delta = delta, r.ld_delta = delta_ld(p.T);
     const R97bHeadRows &o0 = dq ? a.dq : (KIND == kDK ? a.dk : a.dv), &o1 = a.dk;
@@ -1402,13 +1507,17 @@ int launch_bwd(const R97bPacked& p, const R97bAttnPackedBwd& a, float* delta, co
     r.out1 = reinterpret_cast<__nv_bfloat16*>(o1.ptr), r.tok1 = o1.tok, r.head1 = o1.head;
     r.a0_head = (int32_t)a0.head, r.a1_head = (int32_t)a1.head, r.b0_head = (int32_t)b0.head, r.b1_head = (int32_t)b1.head;
     r.c0_head = (int32_t)c0.head;
+    r.T = (int32_t)p.T;
+    auto rows = [](const R97bHeadRows& x) { return reinterpret_cast<const __nv_bfloat16*>(x.ptr); };
+    r.a0 = rows(a0), r.a1 = rows(a1), r.b0 = rows(b0), r.b1 = rows(b1), r.c0 = rows(c0);
+    r.a0_tok = a0.tok, r.a1_tok = a1.tok, r.b0_tok = b0.tok, r.b1_tok = b1.tok, r.c0_tok = c0.tok;
     r.heads = ha, r.grp = a.Hq / a.Hkv;
     r.split_blocks = dq ? 0 : split.blocks, r.parts = split.parts, r.first_blocks = dq ? 0 : split.first;
     r.part0 = KIND == kDK ? dk_parts : dv_parts, r.part1 = dk_parts;
     r.sl2 = a.scale * kLog2e, r.scale = a.scale;
     const int units = (p.n_blocks + (dq ? 0 : split.blocks * (split.parts - 1))) * ha;
     if (!smem_opt_in(bwd_kernel<D, KIND>, C::kSmemBytes)) return R97B_ELAUNCH;
-    bwd_kernel<D, KIND><<<units, kThreads, C::kSmemBytes, st>>>(m[0], m[1], m[2], m[3], m[4], r);
+    bwd_kernel<D, KIND><<<units, kThreads, C::kSmemBytes, st>>>(m[0][0], m[1][0], m[2][0], m[3][0], m[4][0], tails, r);
     return launch_status();
 }
 
@@ -1416,11 +1525,12 @@ template <int D>
 int run_bwd(const R97bPacked& p, const R97bAttnPackedBwd& a, cudaStream_t st) {
     float* delta = reinterpret_cast<float*>(a.ws);
     const Split split = split_of(p, a.Hq, a.Hkv);
+    const int tail = tail_tokens(p);
     float* dv_parts = delta + a.Hq * delta_ld(p.T);
     float* dk_parts = dv_parts + part_floats(split, a.Hkv, D);
-    int rc = launch_bwd<D, kDQ>(p, a, delta, split, dv_parts, dk_parts, st);
-    if (rc == R97B_OK) rc = launch_bwd<D, D == 256 ? kDV : kDKV>(p, a, delta, split, dv_parts, dk_parts, st);
-    if (D == 256 && rc == R97B_OK) rc = launch_bwd<D, D == 256 ? kDK : kDKV>(p, a, delta, split, dv_parts, dk_parts, st);
+    int rc = launch_bwd<D, kDQ>(p, a, delta, split, tail, dv_parts, dk_parts, st);
+    if (rc == R97B_OK) rc = launch_bwd<D, D == 256 ? kDV : kDKV>(p, a, delta, split, tail, dv_parts, dk_parts, st);
+    if (D == 256 && rc == R97B_OK) rc = launch_bwd<D, D == 256 ? kDK : kDKV>(p, a, delta, split, tail, dv_parts, dk_parts, st);
     if (split.blocks > 0 && rc == R97B_OK) {
         const SumArgs s{reinterpret_cast<const int4*>(p.k_blocks), dv_parts, dk_parts, a.dv, a.dk, a.scale, a.Hkv,
                         split.parts};

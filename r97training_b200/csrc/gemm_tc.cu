@@ -736,9 +736,10 @@ bool make_map(CUtensorMap* map, const void* ptr, int64_t inner, int64_t outer, i
     return r == CUDA_SUCCESS;
 }
 
-bool make_rows_map(CUtensorMap* map, const R97bHeadRows& r, int64_t heads, int32_t D, int64_t T, int box_rows) {
+bool make_rows_map(CUtensorMap* map, const R97bHeadRows& r, int64_t heads, int32_t D, int64_t T, int claim, int box_rows) {
     if (!encode_fn()) return false;
-    cuuint64_t dims[3] = {(cuuint64_t)((heads - 1) * r.head + D), 128, (cuuint64_t)T};
+    const RowsExtent e = rows_extent(heads, r.head, D, T, claim);
+    cuuint64_t dims[3] = {(cuuint64_t)e.cols, (cuuint64_t)e.rows, (cuuint64_t)e.blocks};
     cuuint64_t strides[2] = {(cuuint64_t)(r.tok * 2), (cuuint64_t)(r.tok * 2)};
     cuuint32_t box[3] = {64, (cuuint32_t)box_rows, 1};
     cuuint32_t estr[3] = {1, 1, 1};

@@ -26,7 +26,18 @@ bool make_map(CUtensorMap* map, const void* ptr, int64_t inner, int64_t outer, i
 // (64, box_rows, 1) box: the block at token t is (x, r, t), r < 128, row r of it being token t + r. The rows and
 // the tokens step by the same stride, so a box that starts at a negative r is zero there: a block of n < 128 tokens
 // is loaded from r = n - 128 and lies at the end of its tile, with zero rows -- never a neighbour's -- before it.
-bool make_rows_map(CUtensorMap* map, const R97bHeadRows& r, int64_t heads, int32_t D, int64_t T, int box_rows);
+// For the rows before r = 0 the copy engine reads, and discards, other rows that the map claims; so it claims rows of
+// the T tokens alone: r < claim (128, or fewer for blocks of that many tokens) from the tokens t <= T - claim on.
+struct RowsExtent {
+    int64_t cols, rows, blocks;
+};
+inline RowsExtent rows_extent(int64_t heads, int64_t head, int32_t D, int64_t T, int claim) {
+    const int64_t rows = T < claim ? T : claim;
+    return RowsExtent{(heads - 1) * head + D, rows, T - rows + 1};
+}
+// Whether the map that claims 128 rows holds the block at `tok`.
+__host__ __device__ inline bool rows_map_has(int64_t tok, int64_t T) { return tok + 128 <= T; }
+bool make_rows_map(CUtensorMap* map, const R97bHeadRows& r, int64_t heads, int32_t D, int64_t T, int claim, int box_rows);
 int num_sms();
 // Opts kernel `fn` into at least `bytes` of dynamic shared memory on the device that is current. The
 // runtime keeps this attribute per device; it is raised (never lowered) per (kernel, device), under a lock;
