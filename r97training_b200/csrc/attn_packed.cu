@@ -11,22 +11,22 @@
 //
 // Blocks that end inside a tile sit at the tile's END, behind zero rows: the tensor maps address row r < 128 of the
 // block that begins at token t as (column, r, t), token and row with one stride, and a box that starts at row n - 128
-// reads zeros before the block's first token. So no load or store touches a row of another sequence or behind the last
-// one, and the same code serves every length. The maps claim the batch's own rows alone, which leaves out the blocks that
-// begin in its last 127 tokens. A second map, which claims the last block's n tokens from each token on, holds that block and
-// any other of n tokens at most; what is left (short sequences at the end, longer than the last one's last block) the producer
-// warps copy themselves, 16 bytes a lane.
+// has zeros before the block's first token. So no row of another sequence reaches a tile, nothing behind the last one
+// is touched, and the same code serves every length. The maps claim the batch's own rows alone (the copy engine may
+// read what they claim), which leaves out the blocks that begin in its last 127 tokens. A second map, which claims the
+// last block's n tokens from each token on, holds that block and any other of n tokens at most; what is left (short
+// sequences at the end, longer than the last one's last block) the producer warps copy themselves, 16 bytes a lane.
 //
-// What bounds it, measured at 2 x 4096 tokens of 16/4 heads of 256 (one sequence of 8192, 16/4 heads of 128): the forward
-// 189-195 us (211-238) with the tensor pipe busy 80 % (64 %) of the cycles; the backward's passes 307 us dQ, 200 dV, 313 dK
-// (276-297 dQ, 406-427 dK and dV) at 74, 84, 82 (76, 76) %. HBM takes 3-13 % of its rate throughout. A tile of dQ at
-// D = 128, by the clock inside the kernel: 2040 cycles, of which the matrix unit works 1900 on products that are 3 x 512 at its
-// full rate (128-column products, both operands from shared memory at D = 128; with q and dO kept in tensor memory the tile
-// took 1 % less, and units started later), and 130 pass between dS and the product that takes it. The exponentials take
-// 980 of them beside the products; in the forward at D = 128 they take as long as its two products. A unit's start costs dQ
-// two microseconds more: delta's loads and sums, before the first dS. In long runs the power limit sets the clock, and the
-// time follows the products issued: 10 of 128 x 128 x D a tile at D = 256, forward and backward together (S formed four
-// times), 9 at 128, where the mathematics needs 7.
+// What bounds it, measured a launch at a time at 2 x 4096 tokens of 16/4 heads of 256 (one sequence of 8192, 16/4 heads
+// of 128): the forward 189-195 us (211-238) with the tensor pipe busy 80 % (64 %) of the cycles; the backward's passes
+// 307 us dQ, 200 dV, 313 dK (276-297 dQ, 406-427 dK and dV) at 74, 84, 82 (76, 76) %. HBM takes 3-13 % of its rate
+// throughout. A tile of dQ at D = 128, by the clock inside the kernel: 2040 cycles, of which the matrix unit works 1900
+// on products that are 3 x 512 at its full rate (128-column products, both operands from shared memory at D = 128; with
+// q and dO kept in tensor memory the tile took 1 % less, and units started later), and 130 pass between dS and the
+// product that takes it. The exponentials take 980 of them beside the products; in the forward at D = 128 they take as
+// long as its two products. A unit's start costs dQ two microseconds more: delta's loads and sums, before the first dS.
+// In long runs the power limit sets the clock, and the time follows the products issued: 10 of 128 x 128 x D a tile at
+// D = 256, forward and backward together (S formed four times), 9 at 128, where the mathematics needs 7.
 #include "sm100.cuh"
 #include "r97b_internal.h"
 #include "fastmath.cuh"
@@ -1455,6 +1455,11 @@ __global__ void __launch_bounds__(256) sum_parts_kernel(const SumArgs a) {
 // workspace and one more launch to add them. Measured, dK and dV with the sums: a chat batch of 8192 tokens, 16/4 heads of
 // 256: 177 us at 1.15, 181 at 1.25, 179 at 1, 196 at 0.8, 213 at 0.6; of 16384 tokens, 8/2 heads of 128: 66.3, 67.8, 66.6, 74, 79;
 // 2 x 4096 tokens, whose longest unit is 1.12 of the share: 517 us unsplit, 528 split (power, not the longest unit, bounds it).
+// The whole backward unsplit and by this rule, captured (runs differ by 5 %): 16/4 heads of 256, one token 31.6, 24.1 us,
+// turns of 1, 9 and 130 46.9, 32.3, 20 turns of 16 to 400 (ratio 1.35) 105, 113, 4096 + 2 x 2048 (1.48) 739, 662; 16/2 heads,
+// 6000 tokens (3.1) 1647, 1016; of 128, 8/2 heads, the 20 turns (2.7) 42.7, 43.4; 8/1 heads, 3 x 4096 (3.0) 558, 350. At
+// ratios of 1.02 to 1.14 (8 x 1024, 4 x 2048, 2 x 4096, 8192; both head dims) unsplit and split from 1 on are within 5 %
+// of one another, either way.
 struct Split {
     int blocks, parts, first;
 };

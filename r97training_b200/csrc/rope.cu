@@ -29,6 +29,10 @@ constexpr int kBlockThreads = 128;
 // 8192 tokens of 16 + 4 heads of 256 (forward / adjoint) and the adjoint of 32749 tokens, 16 + 4 heads of 128, rotated
 // whole: 5 rows at 7 / 6 blocks 39.7 / 54.8 / 101 us; 10 rows at 8 / 6 41.8 / 56.8 / 102; 4 rows at 8 / 6 44.4 / 60.4 / 121;
 // 10 / 8 blocks (spills) 70 / 82 / 141. The copy-rate times of the same bytes are 25.9 / 38.7 / 79.6 us.
+// 5 divides those 20 heads evenly; a head count that it does not leaves a token's last warp short. Other heads, forward /
+// adjoint, at 5 rows, 4 and 10: 12 + 4 of 256, 8192 tokens 37.6 / 50.0, 35.6 / 48.0, 33.6 / 48.3 us (copy rate 20.7 / 31);
+// 24 + 8 of 128 interleaved, rotated whole, 16384 tokens 70.5 / 91.0, 66.5 / 85.2, 64.3 / 81.3; 32 + 8 of 256, 4096 tokens
+// 41.7 / 56.3, 42.2 / 56.3, 40.0 / 58.4.
 constexpr int kWarpRows = 5;
 constexpr int kFwdBlocks = 7, kBwdBlocks = 6;
 

@@ -265,9 +265,10 @@ __device__ __forceinline__ void umma_f16(uint32_t d_tmem, uint64_t adesc, uint64
         : "memory");
 }
 
-// One lane of the (converged) warp: true there, false in the others.
+// The line at p into L2.
 __device__ __forceinline__ void prefetch_l2(const void* p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
 
+// One lane of the (converged) warp: true there, false in the others.
 __device__ __forceinline__ uint32_t elect_one() {
     uint32_t p;
     asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xFFFFFFFF;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(p));
